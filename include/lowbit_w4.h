@@ -309,6 +309,50 @@ int lowbit_f16_gemv_pick(const void* x, const void* w, void* y, int64_t N, int64
                          size_t workspace_bytes, int64_t* tokens, int64_t* positions, int64_t* out_tokens,
                          int64_t out_capacity, int32_t* out_count, const void* embed, void* h_out, void* stream);
 
+/* ---- a batch of sequences over a paged KV cache, and what their logits say of given tokens (no counterpart in the
+ * reference, which decodes one sequence through transformers) ----
+ * Caches are [pages][Hkv][page_size][D] (contiguous; D 64 or 128; page_size a power of two from 16 to 65536); row r of page
+ * p is slot p * page_size + r. dtype: LOWBIT_DTYPE_F16 or _BF16, of q, k, v, weights and caches alike. */
+
+/* The q and k heads of M rows of a fused q|k|v projection (row m at qkv + m * qkv_stride values; qkv_stride >= (Hq + 2 Hkv) *
+ * D, a multiple of 8): y = x / sqrt(mean(x^2) + eps) * weight for each head ([D] weights; both NULL: y = x), then the
+ * rotate-half position rotation of the pairs (i, i + D / 2) by positions[m] * inv_freq[i] (the angle in 64 bits), all in 32
+ * bits and rounded once; q -> q_out [M][Hq][D], k and the v heads as they are -> the caches' slot slots[m]. A slot outside
+ * the cache (a padded row's, e.g. -1) leaves the caches as they are; of several rows with one slot any one's values may
+ * stay in any of its heads. permuted != 0: each head's D values lie in the RoPE-permuted order of lowbit_rope_kv (16-row
+ * tiles: dims 8 t .. 8 t + 7, then D / 2 + 8 t ..). Outputs must not overlap inputs. */
+int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const void* q_weight, const void* k_weight,
+                           float eps, const int64_t* positions, const float* inv_freq, const int64_t* slots,
+                           void* q_out, void* k_cache, void* v_cache, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
+                           int64_t pages, int64_t page_size, int permuted, void* stream);
+
+/* Causal GQA attention of B sequences' new tokens over their pages: sequence b's new tokens are rows q_starts[b] ..
+ * q_starts[b + 1] - 1 of q and out [T][Hq][D] (q_starts [B + 1], not falling; rows of no sequence are not touched), its keys
+ * 0 .. kv_lens[b] - 1, the last of them the new tokens' own, key j in row j % page_size of page page_table[b][j / page_size]
+ * (page_table [B][table_width]; keys past the table are not attended, a page outside 0 .. pages - 1 reads as zeros). New
+ * token i attends the keys up to kv_lens[b] - new + i; one that is left none (kv_lens[b] < new) gets zeros. Scores scaled by
+ * `scale`; softmax, its sums and the output's sums in 32 bits. Keys up to kv_lens[b] - 1 must hold finite values; rows past
+ * them may hold anything. max_new and max_keys: bounds on a sequence's new tokens and keys that size the launch (a captured
+ * graph keeps them); results do not depend on them beyond the order of sums. workspace (optional, 16-byte aligned, no
+ * initial contents): lets few rows split their keys over the GPU; calls that overlap must
+ * not share one. The same bits on every call for given lengths and bounds. */
+int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                           int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
+                           int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
+                           int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* For M rows of logits [V] (float32, float16 or bfloat16; row m at logits + m * row_stride values, any alignment of the
+ * type): logprob[m] = log_softmax(logits[m])[targets[m]] (0 where the target is negative: none asked; NaN where it is V or
+ * more), entropy[m] = - sum p log p (0 log 0 = 0), and the `top` <= 32 largest logits of the row in falling order, equal
+ * ones by index (-0 equal to +0, a NaN above every number): top_ids [M][top] and their log probabilities top_values
+ * [M][top]. Sums in 32 bits. A row with a NaN, a +inf, or nothing above -inf has NaN results, its top_ids by the same
+ * order. workspace (optional, 16-byte aligned, no initial contents): lets few rows split over the GPU; calls that overlap
+ * must not share one. */
+int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* targets, float* logprob,
+                          float* entropy, float* top_values, int64_t* top_ids, int64_t M, int64_t V, int top,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- HBM bandwidth probes (the measured peak that kernel bandwidths are quoted against) ----
  * The reference measures its peak with a torch device copy and a torch sum over 256 MiB (bench/gpu_run.py:133-141);
  * these are streaming kernels of this library for the same two figures. hbm_read reads `bytes` (a multiple of 16,

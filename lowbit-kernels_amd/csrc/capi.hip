@@ -639,6 +639,86 @@ int lowbit_f16_gemv_pick(const void* x, const void* w, void* y, int64_t N, int64
                     "f16_gemv_pick");
 }
 
+// the parts of the paged calls' checks that they share
+static int check_paged(const char* what, int dtype, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size) {
+  if (dtype != LOWBIT_DTYPE_F16 && dtype != LOWBIT_DTYPE_BF16) return fail(LOWBIT_ERR_ARG, "%s: dtype is F16 or BF16", what);
+  if (D != 64 && D != 128) return fail(LOWBIT_ERR_SHAPE, "%s takes a head_dim of 64 or 128", what);
+  if (Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > 65536) return fail(LOWBIT_ERR_SHAPE, "%s: Hq and Hkv (dividing Hq) must be positive", what);
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))
+    return fail(LOWBIT_ERR_SHAPE, "%s: the page size must be a power of two from 16 to 65536", what);
+  if (pages < 1 || !fits_int(pages)) return fail(LOWBIT_ERR_SHAPE, "%s: pages must be positive", what);
+  return LOWBIT_OK;
+}
+
+int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const void* q_weight, const void* k_weight,
+                           float eps, const int64_t* positions, const float* inv_freq, const int64_t* slots,
+                           void* q_out, void* k_cache, void* v_cache, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
+                           int64_t pages, int64_t page_size, int permuted, void* stream) {
+  if (!qkv || !positions || !inv_freq || !slots || !q_out || !k_cache || !v_cache)
+    return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (!q_weight != !k_weight) return fail(LOWBIT_ERR_ARG, "norm_rope_paged: q_weight goes with k_weight");
+  if (int rc = check_paged("norm_rope_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
+  const int64_t width = (Hq + 2 * Hkv) * D;
+  if (M < 1 || !fits_int(M) || !fits_int(M * (Hq + 2 * Hkv))) return fail(LOWBIT_ERR_SHAPE, "norm_rope_paged: M must be positive");
+  if (qkv_stride < width || qkv_stride % 8 || !fits_int(qkv_stride))
+    return fail(LOWBIT_ERR_SHAPE, "norm_rope_paged: rows of qkv must hold (Hq + 2 Hkv) * D values and start on 16 bytes");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_weight) ||
+      !aligned16(k_weight))
+    return fail(LOWBIT_ERR_ALIGN, "norm_rope_paged needs 16-byte aligned qkv, weights, q_out and caches");
+  if ((reinterpret_cast<uintptr_t>(inv_freq) & 3) ||
+      ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots)) & 7))
+    return fail(LOWBIT_ERR_ALIGN, "norm_rope_paged needs naturally aligned positions, slots and inv_freq");
+  if (int rc = check_device()) return rc;
+  const NormRopeArgs a{qkv, qkv_stride, dtype == LOWBIT_DTYPE_BF16, q_weight, k_weight, eps, positions, inv_freq, slots, q_out,
+                       k_cache, v_cache, (int)M, (int)Hq, (int)Hkv, (int)D, pages, (int)page_size, permuted != 0};
+  return hip_status(norm_rope_paged_launch(a, static_cast<hipStream_t>(stream)), "norm_rope_paged");
+}
+
+int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                           int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
+                           int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
+                           int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
+    return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (int rc = check_paged("attention_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
+  if (T < 1 || B < 1 || table_width < 1 || !fits_int(T * Hq) || !fits_int(B) || !fits_int(table_width * page_size))
+    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive");
+  if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return fail(LOWBIT_ERR_ALIGN, "attention_paged needs 16-byte aligned q, caches and out");
+  if ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(q_starts) |
+       reinterpret_cast<uintptr_t>(kv_lens)) & 3)
+    return fail(LOWBIT_ERR_ALIGN, "attention_paged needs naturally aligned page_table, q_starts and kv_lens");
+  if (workspace && !aligned16(workspace)) return fail(LOWBIT_ERR_ARG, "attention_paged: the workspace must be 16-byte aligned");
+  if (int rc = check_device()) return rc;
+  const PagedAttentionArgs a{q, k_cache, v_cache, out,
+                             PagedBatch{page_table, q_starts, kv_lens, (int)T, (int)B, (int)table_width, (int)page_size, pages},
+                             dtype == LOWBIT_DTYPE_BF16, (int)Hq, (int)Hkv, (int)D, (int)std::min(max_new, T),
+                             (int)std::min(max_keys, table_width * page_size), scale, workspace, workspace ? workspace_bytes : 0};
+  return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
+}
+
+int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* targets, float* logprob,
+                          float* entropy, float* top_values, int64_t* top_ids, int64_t M, int64_t V, int top,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_values || !top_ids)))
+    return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (dtype < LOWBIT_DTYPE_F32 || dtype > LOWBIT_DTYPE_BF16) return fail(LOWBIT_ERR_ARG, "token_logprobs: dtype is F32, F16 or BF16");
+  if (M < 1 || V < 1 || !fits_int(M) || !fits_int(V + 65536) || row_stride < 0 || row_stride > ((int64_t)1 << 40))
+    return fail(LOWBIT_ERR_SHAPE, "token_logprobs: M and V must be positive, the row stride not negative");
+  if (top < 0 || top > kMaxTop || top > V) return fail(LOWBIT_ERR_SHAPE, "token_logprobs: top must be 0..%d and at most V", kMaxTop);
+  if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LOWBIT_DTYPE_F32 ? 3 : 1)) ||
+      ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(top_ids)) & 7) ||
+      ((reinterpret_cast<uintptr_t>(logprob) | reinterpret_cast<uintptr_t>(entropy) | reinterpret_cast<uintptr_t>(top_values)) & 3))
+    return fail(LOWBIT_ERR_ALIGN, "token_logprobs needs naturally aligned arguments");
+  if (workspace && !aligned16(workspace)) return fail(LOWBIT_ERR_ARG, "token_logprobs: the workspace must be 16-byte aligned");
+  if (int rc = check_device()) return rc;
+  const LogprobArgs a{logits, dtype, row_stride, targets, logprob, entropy, top_values, top_ids, (int)M, (int)V, top, workspace,
+                      workspace ? workspace_bytes : 0};
+  return hip_status(token_logprobs_launch(a, static_cast<hipStream_t>(stream)), "token_logprobs");
+}
+
 int lowbit_hbm_read(const void* src, int64_t bytes, void* sink, int64_t blocks, void* stream) {
   if (!src || !sink) return fail(LOWBIT_ERR_ARG, "null pointer argument");
   if (bytes < 16 || bytes % 16) return fail(LOWBIT_ERR_SHAPE, "hbm_read: bytes must be a positive multiple of 16");

@@ -358,6 +358,61 @@ hipError_t attention_launch(const f16* q, const f16* k, const f16* v, const int6
 hipError_t attention_partials_launch(const f16* q, const f16* k, const f16* v, const int64_t* pos, f16* out, int Hq,
                                      int Hkv, int L, int max_keys, float scale, void* ws, size_t ws_bytes, int* parts,
                                      hipStream_t st);
+
+// ---- a batch of sequences over a paged KV cache (paged.hip): caches [pages][Hkv][page_size][D], D 64 or 128 ----
+struct NormRopeArgs {
+  const void* qkv;                 // M rows, `stride` values apart
+  int64_t stride;
+  bool bf16;                       // else fp16
+  const void *q_weight, *k_weight; // [D], or nullptr: no norm
+  float eps;
+  const int64_t* positions;
+  const float* inv_freq;           // [D / 2]
+  const int64_t* slots;            // page * page_size + row, anything outside the cache: k and v are not written
+  void *q_out, *k_cache, *v_cache;
+  int M, Hq, Hkv, D;
+  int64_t pages;
+  int page_size;
+  bool permuted;
+};
+hipError_t norm_rope_paged_launch(const NormRopeArgs& a, hipStream_t st);
+// sequence b's new tokens are rows q_starts[b] .. q_starts[b + 1] - 1 of q and out (rows of no sequence are not touched), its
+// keys 0 .. kv_lens[b] - 1, the new tokens' among them at the end, in pages table[b][0 ..]
+struct PagedBatch {
+  const int* table;
+  const int* q_starts;
+  const int* kv_lens;
+  int T, B, table_width, page_size;
+  int64_t pages;
+};
+struct PagedAttentionArgs {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  PagedBatch batch;
+  bool bf16;                       // else fp16
+  int Hq, Hkv, D;
+  int max_new, max_keys;           // the caller's bounds: they size the launch
+  float scale;
+  void* ws;
+  size_t ws_bytes;
+};
+hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st);
+
+// ---- log probabilities (logprobs.hip) ----
+constexpr int kMaxTop = 32;
+struct LogprobArgs {
+  const void* logits;
+  int dtype;                       // LOWBIT_DTYPE_*
+  int64_t stride;
+  const int64_t* targets;
+  float *logprob, *entropy, *top_value;
+  int64_t* top_id;
+  int M, V, top;
+  void* ws;
+  size_t ws_bytes;
+};
+hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st);
+
 hipError_t dequant_launch(const uint8_t* w, const f16* s, f16* out, int N, int K, int G, bool mfma, hipStream_t st);
 hipError_t relayout_launch(const uint8_t* src, uint8_t* dst, int N, int K, bool mfma, hipStream_t st);
 hipError_t quantize_launch(const void* w, int dtype, uint8_t* packed, f16* scales, int N, int K, int G,

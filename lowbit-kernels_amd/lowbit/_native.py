@@ -63,6 +63,12 @@ SIGNATURES = {
     "lowbit_f16_linear_fused": ([_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, ctypes.c_float, _vp], _int),
     "lowbit_f16_qkv_rope": ([_vp, _vp, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                              _i64, _vp], _int),
+    "lowbit_norm_rope_paged": ([_vp, _i64, _int, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                _i64, _i64, _i64, _int, _vp], _int),
+    "lowbit_attention_paged": ([_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _i64, _i64, ctypes.c_float, _vp, ctypes.c_size_t, _vp], _int),
+    "lowbit_token_logprobs": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, ctypes.c_size_t, _vp],
+                              _int),
     "lowbit_hbm_read": ([_vp, _i64, _vp, _i64, _vp], _int),
     "lowbit_hbm_copy": ([_vp, _vp, _i64, _i64, _vp], _int),
     "lowbit_host_quantize": ([_vp, _vp, _vp, _i64, _i64, _i64], _int),
@@ -669,6 +675,108 @@ class NativeExt:
                                                ptr(nw) if nw is not None else None, float(eps), ptr(positions),
                                                ptr(inv_freq), ptr(q_out), ptr(k_cache), ptr(v_cache), hq, hkv,
                                                k_cache.shape[1], _stream(x.device)))
+
+    # ---- a batch of sequences over a paged cache (lowbit_norm_rope_paged, lowbit_attention_paged), and what logits say of
+    # given tokens (lowbit_token_logprobs) ----
+
+    def _paged_dtype(self, t):
+        if t.dtype is torch.float16:
+            return DTYPE_F16
+        if t.dtype is torch.bfloat16:
+            return DTYPE_BF16
+        raise RuntimeError(f"float16 or bfloat16 tensors are taken, got {t.dtype}")
+
+    def _check_pages(self, k_cache, v_cache, like, hkv, dim):
+        """Both caches [pages, hkv, page_size, dim] beside `like`; returns (pages, page_size)."""
+        shape = k_cache.shape
+        if len(shape) != 4 or v_cache.shape != shape or shape[1] != hkv or shape[3] != dim:
+            raise RuntimeError(f"the caches must be [pages, {hkv}, page_size, {dim}], got {list(shape)} and {list(v_cache.shape)}")
+        for t in (k_cache, v_cache):
+            if t.dtype is not like.dtype or not t.is_contiguous() or t.get_device() != like.get_device():
+                raise RuntimeError(f"the caches must be contiguous {like.dtype} tensors on the same GPU")
+        return shape[0], shape[2]
+
+    def norm_rope_paged(self, qkv, q_weight, k_weight, eps, positions, inv_freq, slots, q_out, k_cache, v_cache, hq, hkv,
+                        permuted=False):
+        """The q and k heads of qkv [M, (hq + 2 hkv) D] (rows may lie apart), RMS-normalized with q_weight and k_weight [D]
+        (both None: not), rotated by positions (int64 [M]; inv_freq float32 [D / 2]): q -> q_out [M, hq, D], k and v -> the
+        caches [pages, hkv, page_size, D] at slots (int64 [M]: page * page_size + row, negative: not written). D is 64 or
+        128; permuted: the head's values in fused.rope_permutation's order."""
+        if not qkv.is_cuda or qkv.dim() != 2 or q_out.dim() != 3:
+            raise RuntimeError("qkv [M, (Hq + 2 Hkv) D] and q_out [M, Hq, D] must be CUDA tensors")
+        dtype, index, m, dim = self._paged_dtype(qkv), qkv.get_device(), qkv.shape[0], q_out.shape[2]
+        if qkv.shape[1] != (hq + 2 * hkv) * dim or qkv.stride(1) != 1:
+            raise RuntimeError(f"rows of qkv must hold (Hq + 2 Hkv) * D = {(hq + 2 * hkv) * dim} values side by side")
+        device = qkv.device
+        _need(q_out, "q_out", qkv.dtype, (m, hq, dim), device)
+        if (q_weight is None) != (k_weight is None):
+            raise RuntimeError("q_weight goes with k_weight")
+        if q_weight is not None:
+            _need(q_weight, "q_weight", qkv.dtype, (dim,), device)
+            _need(k_weight, "k_weight", qkv.dtype, (dim,), device)
+        _need(positions, "positions", torch.int64, (m,), device)
+        _need(slots, "slots", torch.int64, (m,), device)
+        _need(inv_freq, "inv_freq", torch.float32, (dim // 2,), device)
+        pages, page_size = self._check_pages(k_cache, v_cache, qkv, hkv, dim)
+        if m == 0:
+            return
+        _launch(index, lambda stream, ws, nbytes: self.lib.lowbit_norm_rope_paged(
+            qkv.data_ptr(), qkv.stride(0) if m > 1 else qkv.shape[1], dtype,
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), float(eps),
+            positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), m, hq, hkv, dim, pages, page_size, 1 if permuted else 0, stream))
+
+    def attention_paged(self, q, k_cache, v_cache, page_table, q_starts, kv_lens, out, max_new, max_keys, scale, split=True):
+        """Causal GQA attention of a batch: sequence b's new tokens are rows q_starts[b] .. q_starts[b + 1] of q and out
+        [T, hq, D] (q_starts int32 [B + 1]), its keys the first kv_lens[b] (int32 [B], the new tokens' included) in the pages
+        page_table[b] (int32 [B, width]) of the caches [pages, hkv, page_size, D]. Rows of no sequence are not touched, rows
+        left without a key are zeros. max_new, max_keys: bounds on a sequence's new tokens and keys, which size the launch.
+        split=False keeps every row's keys in one workgroup, without a workspace."""
+        if not q.is_cuda or q.dim() != 3 or k_cache.dim() != 4 or page_table.dim() != 2:
+            raise RuntimeError("q [T, Hq, D], the caches [pages, Hkv, page_size, D] and page_table [B, width] must be CUDA tensors")
+        dtype, index = self._paged_dtype(q), q.get_device()
+        t, hq, dim = q.shape
+        batch, width = page_table.shape
+        hkv = k_cache.shape[1]
+        device = q.device
+        _need(q, "q", q.dtype, (t, hq, dim), device)
+        _need(out, "out", q.dtype, (t, hq, dim), device)
+        _need(page_table, "page_table", torch.int32, (batch, width), device)
+        _need(q_starts, "q_starts", torch.int32, (batch + 1,), device)
+        _need(kv_lens, "kv_lens", torch.int32, (batch,), device)
+        pages, page_size = self._check_pages(k_cache, v_cache, q, hkv, dim)
+        if t == 0 or batch == 0:
+            return
+        _launch(index, lambda stream, ws, nbytes: self.lib.lowbit_attention_paged(
+            q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),
+            kv_lens.data_ptr(), out.data_ptr(), t, batch, hq, hkv, dim, pages, page_size, int(max_new), int(max_keys),
+            float(scale), ws, nbytes, stream))
+
+    def token_logprobs(self, logits, targets, top=0):
+        """Of logits [M, V] (float32, float16 or bfloat16; rows may lie apart): (log probability of targets [M] (int64;
+        negative: 0), entropy, log probabilities and ids of the `top` <= 32 most likely tokens): float32 [M], float32 [M],
+        float32 [M, top], int64 [M, top]. Equal logits rank by index."""
+        dtypes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+        if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in dtypes:
+            raise RuntimeError("logits must be a 2-D float32, float16 or bfloat16 CUDA tensor [M, V]")
+        m, v = logits.shape
+        if v > 1 and logits.stride(1) != 1:
+            raise RuntimeError("a row of logits must lie side by side")
+        index, device = logits.get_device(), logits.device
+        _need(targets, "targets", torch.int64, (m,), device)
+        if top < 0 or top > min(v, 32):
+            raise RuntimeError(f"top must be 0..32 and at most V = {v}, got {top}")
+        sums = torch.empty((2, m), dtype=torch.float32, device=device)
+        values = torch.empty((m, top), dtype=torch.float32, device=device)
+        ids = torch.empty((m, top), dtype=torch.int64, device=device)
+        if m == 0:
+            return sums[0], sums[1], values, ids
+        if v == 0:
+            raise RuntimeError("token_logprobs needs at least one logit a row")
+        _launch(index, lambda stream, ws, nbytes: self.lib.lowbit_token_logprobs(
+            logits.data_ptr(), dtypes[logits.dtype], logits.stride(0) if m > 1 else v, targets.data_ptr(), sums.data_ptr(),
+            sums.data_ptr() + 4 * m, values.data_ptr(), ids.data_ptr(), m, v, int(top), ws, nbytes, stream))
+        return sums[0], sums[1], values, ids
 
     # ---- bandwidth probes (lowbit_hbm_read, lowbit_hbm_copy) ----
     def hbm_read(self, buf, sink, blocks):
