@@ -659,7 +659,8 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
   if (!q_weight != !k_weight) return fail(LOWBIT_ERR_ARG, "norm_rope_paged: q_weight goes with k_weight");
   if (int rc = check_paged("norm_rope_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
   const int64_t width = (Hq + 2 * Hkv) * D;
-  if (M < 1 || !fits_int(M) || !fits_int(M * (Hq + 2 * Hkv))) return fail(LOWBIT_ERR_SHAPE, "norm_rope_paged: M must be positive");
+  if (M < 1 || M > (1 << 25) / (Hq + 2 * Hkv))
+    return fail(LOWBIT_ERR_SHAPE, "norm_rope_paged: M must be positive, M * (Hq + 2 Hkv) at most 2^25");
   if (qkv_stride < width || qkv_stride % 8 || !fits_int(qkv_stride))
     return fail(LOWBIT_ERR_SHAPE, "norm_rope_paged: rows of qkv must hold (Hq + 2 Hkv) * D values and start on 16 bytes");
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_weight) ||
@@ -682,8 +683,10 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
   if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
     return fail(LOWBIT_ERR_ARG, "null pointer argument");
   if (int rc = check_paged("attention_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
-  if (T < 1 || B < 1 || table_width < 1 || !fits_int(T * Hq) || !fits_int(B) || !fits_int(table_width * page_size))
-    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive");
+  // (the launch's workgroups and the keys' numbers stay within 32 bits)
+  if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > (1 << 22) / Hkv || table_width > (1 << 30) / page_size)
+    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B * Hkv "
+                "2^22 and the table's keys 2^30");
   if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return fail(LOWBIT_ERR_ALIGN, "attention_paged needs 16-byte aligned q, caches and out");

@@ -163,6 +163,7 @@ WORKSPACE_COUNTER_BYTES = 16384
 WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (16 << 20)     # LOWBIT_WORKSPACE_BYTES
 PREFILL_WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (64 << 20)
 ATTENTION_WORKSPACE_BYTES = 4 << 20
+PAGED_SPLIT_KEYS = 256                  # attention_paged cuts longer sequences into parts of at least as many keys
 PICK_WORKSPACE_BYTES = 1 << 20          # the greedy pick's keys: 8 bytes per 8 head rows
 _WORKSPACES = {}
 _CAPTURE_STREAMS = {}
@@ -747,10 +748,17 @@ class NativeExt:
         pages, page_size = self._check_pages(k_cache, v_cache, q, hkv, dim)
         if t == 0 or batch == 0:
             return
-        _launch(index, lambda stream, ws, nbytes: self.lib.lowbit_attention_paged(
+        # the split tiles' records, from the caching allocator for this call alone: calls on several streams and captured
+        # graphs share none (LOWBIT_PAGED_WORKSPACE_BYTES(rows, D))
+        nbytes = 0
+        if split and max_keys > PAGED_SPLIT_KEYS:
+            rows = 32 if max_new * hq <= 32 * hkv else 128
+            nbytes = (768 if rows == 32 else 1536) * rows * (dim + 4) * 4
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged(
             q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),
             kv_lens.data_ptr(), out.data_ptr(), t, batch, hq, hkv, dim, pages, page_size, int(max_new), int(max_keys),
-            float(scale), ws, nbytes, stream))
+            float(scale), ws.data_ptr() if nbytes else None, nbytes, stream))
 
     def token_logprobs(self, logits, targets, top=0):
         """Of logits [M, V] (float32, float16 or bfloat16; rows may lie apart): (log probability of targets [M] (int64;
