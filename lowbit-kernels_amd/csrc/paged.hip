@@ -81,13 +81,19 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const T* __restrict__ qk
 //   a sequence has tiles of rows, and its keys are cut into `parts` alike for all its tiles, `parts` being its blocks of keys
 //   over a share that the whole call's blocks give each of the GPU's workgroup slots. A tile of one part writes its output,
 //   the parts of another write records of the workspace that paged_attention_merge joins in order.
+struct FastDiv {                                              // n / d = high word of n m >> s for 0 <= n < 2^31 (m 0: d is 1)
+  uint32_t m;
+  int s;
+};
+__device__ __forceinline__ int div(int n, const FastDiv& d) { return d.m ? (int)(__umulhi((uint32_t)n, d.m) >> d.s) : n; }
+
 struct PagedPlan {
-  int rows;          // query rows of a tile
-  int block;         // keys of a block
   int slots;         // workgroups that the GPU holds at once
   int least;         // blocks of a part at least
   int cap;           // parts of a tile at most (1: no split)
   int most;          // parts of split tiles in all at most (what the workspace holds, twice its share)
+  int Hq, Hkv, G;
+  FastDiv by_hkv, by_g;
 };
 struct PagedUnit {
   int seq, first, nq, len, tiles, parts, tile, hk, pid, rec;   // first: the sequence's first row of q; rec: the part's records
@@ -104,50 +110,54 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// What lane l knows of sequence b0 + l (all zero past the last one): its rows of q, keys, tiles and blocks of keys.
+// What lane l knows of sequence b0 + l (all zero past the last one): its rows of q, keys, tiles of kRows and blocks of kBlock.
 struct PagedSeq {
   int first, nq, len, tiles, blocks;
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, const PagedPlan& p, int G, int seq) {
+template <int kRows, int kBlock>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int seq) {
   PagedSeq s{};
   if (seq >= b.B) return s;
-  s.first = min(max(b.q_starts[seq], 0), b.T);
-  s.nq = min(max(b.q_starts[seq + 1], s.first), b.T) - s.first;
-  s.len = max(b.kv_lens[seq], 0);
-  s.tiles = (s.nq * G + p.rows - 1) / p.rows;
-  s.blocks = s.nq ? (min(s.len, b.table_width * b.page_size) + p.block - 1) / p.block : 0;
+  const int q0 = b.q_starts[seq], q1 = b.q_starts[seq + 1], n = b.kv_lens[seq];
+  s.first = min(max(q0, 0), b.T);
+  s.nq = min(max(q1, s.first), b.T) - s.first;
+  s.len = max(n, 0);
+  s.tiles = (s.nq * G + kRows - 1) / kRows;
+  s.blocks = s.nq ? (min(s.len, b.table_width * b.page_size) + kBlock - 1) / kBlock : 0;
   return s;
 }
 
 // The parts' share in blocks: total blocks over the slots that tiles of one part leave free in the call's rounds of
-// workgroups (half a round at least), so that the parts, each sequence's rounded up, fill whole rounds.
-__device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, int G, int Hkv, int lane) {
+// workgroups (half a round at least), so that the parts, each sequence's rounded up, fill whole rounds. s0: the first 64
+// sequences.
+template <int kRows, int kBlock>
+__device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {
   if (p.cap == 1) return 0x3FFFFFFF;
-  float total = 0.f, units = 0.f;
-  for (int b0 = 0; b0 < b.B; b0 += 64) {
-    const PagedSeq s = paged_seq(b, p, G, b0 + lane);
+  float total = wave_sum((float)s0.tiles * (float)s0.blocks), units = wave_sum((float)s0.tiles);
+  for (int b0 = 64; b0 < b.B; b0 += 64) {
+    const PagedSeq s = paged_seq<kRows, kBlock>(b, p.G, b0 + lane);
     total += wave_sum((float)s.tiles * (float)s.blocks);
     units += wave_sum((float)s.tiles);
   }
-  total *= (float)Hkv;
-  units *= (float)Hkv;
+  total *= (float)p.Hkv;
+  units *= (float)p.Hkv;
   const float slots = (float)p.slots, rounds = ceilf((units + 0.5f * slots) / slots);
   const float free = fminf(rounds * slots - units, (float)(p.most / 2));
   return max(p.least, (int)fminf(ceilf(total / free), 1e9f));
 }
 
-// The unit of work `idx` (split: counted among the split tiles alone, without their parts). False past the last one.
-template <bool kSplitTiles>
-__device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan& p, int G, int Hkv, int idx, int lane,
-                                           PagedUnit& u) {
-  const int share = paged_share(b, p, G, Hkv, lane);
-  int before = 0, recs = 0;                                  // units and record groups of the sequences before
+// The part of work `idx`; false past the last one. kMerge > 0: the chunk `idx` of kMerge rows (a divisor of kRows) of the split
+// tiles, pid counting the chunk in its tile and rec the tile's first part.
+template <int kRows, int kBlock, int kMerge>
+__device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int share, int idx,
+                                           int lane, PagedUnit& u) {
+  int before = 0, recs = 0;                                  // work and record groups of the sequences before
   for (int b0 = 0; b0 < b.B; b0 += 64) {
-    const PagedSeq s = paged_seq(b, p, G, b0 + lane);
-    const int parts = max(1, min(p.cap, (s.blocks + share - 1) / share));
-    const int tiles = s.tiles * Hkv, split = parts > 1 ? tiles * parts : 0;
-    const int mine = kSplitTiles ? (parts > 1 ? tiles : 0) : tiles * parts;
-    const int upto = wave_scan(mine), recs_upto = wave_scan(split);
+    const PagedSeq s = b0 == 0 ? s0 : paged_seq<kRows, kBlock>(b, p.G, b0 + lane);
+    const int parts = p.cap == 1 ? 1 : max(1, min(p.cap, (s.blocks + share - 1) / share));
+    const int tiles = s.tiles * p.Hkv, split = parts > 1 ? tiles * parts : 0;
+    const int mine = kMerge == 0 ? tiles * parts : parts > 1 ? (s.nq * p.G + max(kMerge, 1) - 1) / max(kMerge, 1) * p.Hkv : 0;
+    const int upto = wave_scan(mine), recs_upto = p.cap == 1 ? 0 : wave_scan(split);
     const uint64_t hit = __ballot(idx - before < upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -157,19 +167,22 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
       u.nq = pick(s.nq);
       u.len = pick(s.len);
       u.tiles = pick(s.tiles);
-      u.parts = pick(parts);
-      int at = idx - before - pick(upto - mine);
-      const int rec = recs + pick(recs_upto - split);
-      u.hk = at % Hkv;                                       // KV heads fastest: a head's keys stay in the L2 of its XCDs
-      at /= Hkv;
-      u.pid = kSplitTiles ? 0 : at % u.parts;
-      at = kSplitTiles ? at : at / u.parts;
-      u.tile = u.tiles - 1 - at;                             // the last rows, which have the most keys, first
-      u.rec = rec + ((u.tile * Hkv + u.hk) * u.parts + u.pid);
+      u.parts = p.cap == 1 ? 1 : pick(parts);
+      const int at = idx - before - pick(upto - mine), rest = div(at, p.by_hkv);
+      u.hk = at - rest * p.Hkv;                              // KV heads fastest: a head's keys stay in the L2 of its XCDs
+      if constexpr (kMerge == 0) {
+        const int t = u.parts == 1 ? rest : (int)((uint32_t)rest / (uint32_t)u.parts);
+        u.pid = rest - t * u.parts;
+        u.tile = u.tiles - 1 - t;                            // the last rows, which have the most keys, first
+      } else {
+        u.tile = rest / (kRows / kMerge);
+        u.pid = rest % (kRows / kMerge);
+      }
+      u.rec = p.cap == 1 ? 0 : recs + pick(recs_upto - split) + (u.tile * p.Hkv + u.hk) * u.parts + (kMerge == 0 ? u.pid : 0);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
-    recs += __builtin_amdgcn_readlane(recs_upto, 63);
+    if (p.cap > 1) recs += __builtin_amdgcn_readlane(recs_upto, 63);
   }
   return false;
 }
@@ -202,13 +215,21 @@ struct Mfma<bf16> {
   }
 };
 
+// four values of a row's output; a row without a key gets zeros
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, const f32x4& num, float den, bool some) {
+  const float inv = 1.f / den;
+  *reinterpret_cast<uint2*>(dst) = some ? make_uint2(Mfma<T>::pack(num[0] * inv, num[1] * inv), Mfma<T>::pack(num[2] * inv, num[3] * inv))
+                                        : make_uint2(0u, 0u);
+}
+
 // blocks ahead that K and V are requested, and the slots of LDS that takes
 template <int KG>
 constexpr int paged_ahead() { return KG == 4 ? 1 : 2; }
 template <int D, int RG, int KG>
 constexpr size_t paged_lds() {
   const size_t ring = (size_t)(paged_ahead<KG>() + 1) * 2 * 32 * KG * D * 2;
-  const size_t merge = (size_t)(KG - 1) * RG * (D / 2 + 2) * 256;
+  const size_t merge = KG > 1 ? (size_t)4 * 32 * (D + 4) * 4 : 0;
   return ring > merge ? ring : merge;
 }
 template <int D>
@@ -235,32 +256,37 @@ constexpr float kLag = 4.f;
 template <typename T, int D, int RG, int KG, int NR>
 __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attention(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, PagedBatch bt, PagedPlan plan,
-    T* __restrict__ out, float* __restrict__ part, int Hq, int Hkv, int shift, float scale) {
+    T* __restrict__ out, float* __restrict__ part, int shift, float scale) {
   static_assert(RG * KG == 4, "four waves");
   constexpr int RB = D * 2;                                  // bytes of a row
   constexpr int PR = RB / 16;                                // its pieces
   constexpr int KL = 64 / PR;                                // keys of a wave-load
   constexpr int BK = 32 * KG;
   constexpr int BB = BK * RB;                                // bytes of a block of K, and of V
-  constexpr int NP = BK / (4 * KL);                          // wave-loads of a wave and block, for K and for V
+  constexpr int KW = BK / 4;                                 // keys of a block that a wave loads
+  constexpr int NG = (KW + 15) / 16, LG = KW / NG / KL;      // groups of them, wave-loads of a group
+  constexpr int NP = NG * LG;                                // wave-loads of a wave and block, for K and for V
   constexpr int AH = paged_ahead<KG>(), N = AH + 1;          // slots: [N] K blocks, [N] V blocks
   constexpr bool kOwn = RG == 1;                             // a wave loads its own keys
   constexpr int DT = D / 32, KS = D / 16;
   constexpr int kRows = 32 * NR * RG;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int G = Hq / Hkv;
+  args_in_sgprs(q, k_cache, v_cache, bt.table, bt.q_starts, bt.kv_lens, bt.B, bt.T, bt.table_width, bt.page_size, plan.slots,
+                plan.cap, plan.G, plan.by_hkv.m, plan.by_g.m, out, part, shift);
+  const int Hq = plan.Hq, Hkv = plan.Hkv, G = plan.G;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 31, h = lane >> 5;
   PagedUnit un;
-  if (!paged_unit<false>(bt, plan, G, Hkv, blockIdx.x, lane, un)) return;
+  const PagedSeq s0 = paged_seq<kRows, BK>(bt, G, lane);
+  if (!paged_unit<kRows, BK, 0>(bt, plan, s0, paged_share<kRows, BK>(bt, plan, s0, lane), blockIdx.x, lane, un)) return;
   const int rgrp = wave % RG, kgrp = wave / RG;
   const int cap = bt.table_width * bt.page_size;
   const int len = min(un.len, cap);                  // keys that can be read
   const int rows = un.nq * G;
-  const int tok_last = (min(rows, (un.tile + 1) * kRows) - 1) / G;
+  const int tok_last = div(min(rows, (un.tile + 1) * kRows) - 1, plan.by_g);
   const int keys = min(un.len - un.nq + tok_last + 1, cap);  // of the tile's last row (none: 0 or less)
   const int nblk = (max(keys, 0) + BK - 1) / BK;
-  const int per = (nblk + un.parts - 1) / un.parts;
+  const int per = un.parts == 1 ? nblk : (int)((uint32_t)(nblk + un.parts - 1) / (uint32_t)un.parts);
   const int b0 = min(nblk, un.pid * per), b1 = min(nblk, b0 + per);
   const int kend = min(keys, b1 * BK);
   // the rows' last keys, least and most of a row group, and q
@@ -274,7 +300,7 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
   for (int r = 0; r < NR; ++r) {
     const int row = un.tile * kRows + 32 * (NR * rgrp + r) + j;
     live[r] = row < rows;
-    const int c = min(row, rows - 1), tok = c / G, g = c - tok * G;
+    const int c = min(row, rows - 1), tok = div(c, plan.by_g), g = c - tok * G;
     pr[r] = live[r] ? min(un.len - un.nq + tok, cap - 1) : -1;
     wmin[r] = live[r] ? pr[r] : INT_MAX;
 #pragma unroll
@@ -291,48 +317,69 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
   const bool busy = wmin[0] != INT_MAX;                      // a wave whose rows are all past the end only loads
 
   // ---- loads ----
-  // page numbers of window [win, win + 64) pages, a lane each; the next window requested when one is begun
+  // where the 128 pages from `win` on begin in a cache, lane l holding pages win + l and win + 64 + l: byte offsets of this KV
+  // head's rows, bit 63 set for a page outside the cache. They are waited for where they are fetched (the empty asm uses
+  // them), so that no later use waits for the loads into LDS that were requested in between
   const int* table = bt.table + (int64_t)un.seq * bt.table_width;
   int win = (b0 * BK) >> shift;
-  auto fetch = [&](int first) { return first + lane < bt.table_width ? table[first + lane] : -1; };
-  int cur = fetch(win), nxt = fetch(win + 64);
-  const uint64_t head_bytes = (uint64_t)bt.page_size * RB;   // a head's rows of a page
+  uint32_t wlo[2], whi[2];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = win + 64 * i + lane;
+      const int id = at < bt.table_width ? table[at] : -1;
+      const uint64_t off = ((uint64_t)(uint32_t)id * (uint32_t)Hkv + (uint32_t)un.hk) * (uint32_t)bt.page_size * RB;
+      wlo[i] = (uint32_t)off;
+      whi[i] = id >= 0 && id < bt.pages ? (uint32_t)(off >> 32) : 0x80000000u;
+    }
+    asm volatile("" : "+v"(wlo[0]), "+v"(wlo[1]), "+v"(whi[0]), "+v"(whi[1]));
+  };
+  fetch();
   const uint32_t lds0 = lds_addr(smem);
-  // lane's row of a wave-load and its slot there
+  // A wave loads keys KW wave .. + KW - 1 of every block (with KG == 4 the keys it takes), in groups of at most 16, which lie
+  // in one page; a wave-load takes KL keys, lane l the 16-byte slot l % PR of key l / PR
   const int lk = lane / PR, ls = lane % PR;
   auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
   auto vswz = [](int key) { return D == 128 ? 4 * (key & 3) + 2 * ((key >> 2) & 1) : 4 * ((key >> 1) & 1); };
-  auto load_key = [&](int u) { return kOwn ? 32 * kgrp + KL * u : KL * (4 * u + wave); };   // first key of wave-load u
-  struct Pages {
-    int id[NP];
-  };
-  auto pages_of = [&](int blk) {
-    Pages p;
+  int koff[LG], voff[LG];
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-      const int key = blk * BK + load_key(u), pg = key >> shift;
-      if (pg - win >= 64) {
-        win += 64;
-        cur = nxt;
-        nxt = fetch(win + 64);
-      }
-      const int id = __builtin_amdgcn_readlane(cur, (pg - win) & 63);
-      p.id[u] = blk < b1 && key < len && id >= 0 && id < bt.pages ? id : -1;
+  for (int u = 0; u < LG; ++u) {
+    const int k = KW * wave + KL * u + lk;                    // (groups of 16 repeat)
+    koff[u] = (KL * u + lk) * RB + 16 * (ls ^ kswz(k));
+    voff[u] = (KL * u + lk) * RB + 16 * (ls ^ vswz(k));
+  }
+  struct Rows {
+    uint32_t lo[NG], hi[NG], bytes[NG];                       // a group's rows: offset in a cache, bytes that exist
+  };
+  auto rows_of = [&](int blk) {
+    if ((((blk + 1) * BK - 1) >> shift) - win >= 128) {       // (uniform)
+      win = (blk * BK) >> shift;
+      fetch();
+    }
+    Rows p;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int key = blk * BK + KW * wave + 16 * g, at = (key >> shift) - win;
+      const uint32_t lo0 = __builtin_amdgcn_readlane(wlo[0], at & 63), lo1 = __builtin_amdgcn_readlane(wlo[1], at & 63);
+      const uint32_t hi0 = __builtin_amdgcn_readlane(whi[0], at & 63), hi1 = __builtin_amdgcn_readlane(whi[1], at & 63);
+      const uint32_t lo = at & 64 ? lo1 : lo0, hi = at & 64 ? hi1 : hi0;
+      const uint64_t off = (((uint64_t)hi << 32) | lo) + (uint32_t)((key & (bt.page_size - 1)) * RB);
+      p.lo[g] = (uint32_t)off;
+      p.hi[g] = (uint32_t)(off >> 32);
+      p.bytes[g] = blk < b1 && (int)hi >= 0 ? (uint32_t)(min(max(len - key, 0), KL * LG) * RB) : 0u;
     }
     return p;
   };
-  auto load = [&](const T* cache, const Pages& p, int blk, uint32_t at, bool is_k) {
+  const uint64_t kbase = reinterpret_cast<uint64_t>(k_cache), vbase = reinterpret_cast<uint64_t>(v_cache);
+  auto load = [&](uint64_t cache, const Rows& p, const int (&off)[LG], uint32_t at) {
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-      const int lkey = load_key(u), key = blk * BK + lkey, row = key & (bt.page_size - 1);
-      const int n = p.id[u] < 0 ? 0 : min(len - key, KL);    // rows that exist
-      const uint64_t off = ((uint64_t)(uint32_t)max(p.id[u], 0) * (uint32_t)Hkv + (uint32_t)un.hk) * head_bytes + (uint64_t)(uint32_t)row * RB;
-      const uint64_t base = reinterpret_cast<uint64_t>(cache) + off;
+    for (int g = 0; g < NG; ++g) {
+      const uint64_t base = cache + (((uint64_t)p.hi[g] << 32) | p.lo[g]);
       const uint64_t ub = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(base >> 32)) << 32) |
-                          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base);
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(reinterpret_cast<const void*>(ub), (uint32_t)__builtin_amdgcn_readfirstlane(n * RB));
-      const int k = lkey + lk, piece = ls ^ (is_k ? kswz(k) : vswz(k));
-      dma16(rs, lk * RB + 16 * piece, lds0 + at + lkey * RB);
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base);   // (uniform; the compiler keeps it scalar then)
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(reinterpret_cast<const void*>(ub), (uint32_t)__builtin_amdgcn_readfirstlane((int)p.bytes[g]));
+#pragma unroll
+      for (int u = 0; u < LG; ++u) dma16(rs, off[u], lds0 + at + (uint32_t)((KW * wave + 16 * g + KL * u) * RB));
     }
   };
   auto slot = [](int i) { return (uint32_t)(i * BB); };
@@ -429,13 +476,13 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
       else
         lds_wait_barrier<decltype(n)::value>();
     };
-    Pages pg = pages_of(b0);
-    load(k_cache, pg, b0, slot(0), true);
+    Rows at = rows_of(b0);
+    load(kbase, at, koff, slot(0));
 #pragma unroll
     for (int t = 0; t < AH; ++t) {
-      load(v_cache, pg, b0 + t, kV + slot(t), false);
-      pg = pages_of(b0 + t + 1);
-      load(k_cache, pg, b0 + t + 1, slot((t + 1) % N), true);
+      load(vbase, at, voff, kV + slot(t));
+      at = rows_of(b0 + t + 1);
+      load(kbase, at, koff, slot((t + 1) % N));
     }
     sync(std::integral_constant<int, 2 * NP * AH>{});
     if (busy) scores(slot(0), 0, KS);
@@ -443,9 +490,9 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
     int a = 0;                                                // i % N
     for (int i = b0; i < b1; ++i) {
       const int a1 = a + 1 == N ? 0 : a + 1, am = a == 0 ? N - 1 : a - 1;
-      load(v_cache, pg, i + AH, kV + slot(am), false);
-      pg = pages_of(i + 1 + AH);
-      load(k_cache, pg, i + 1 + AH, slot(a), true);
+      load(vbase, at, voff, kV + slot(am));
+      at = rows_of(i + 1 + AH);
+      load(kbase, at, koff, slot(a));
       if (busy) block(slot(a1), slot(a), i * BK + 32 * kgrp);
       sync(std::integral_constant<int, 2 * NP * (AH - 1)>{});
       a = a1;
@@ -454,49 +501,65 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
   }
 #pragma unroll
   for (int r = 0; r < NR; ++r) lsum[r] += __shfl_xor(lsum[r], 32, 64);
-  if constexpr (KG > 1) {                                     // the key groups' sums, through LDS, into key group 0
+  if constexpr (KG > 1) {
+    // the key groups' sums meet in LDS as rows, reference and weight sum behind each, and leave 16 bytes of a row a lane
     static_assert(NR == 1, "one row group a wave");
-    constexpr int kRec = (D / 2 + 2) * 64 * 4;
-    float* mine = reinterpret_cast<float*>(smem + (size_t)((kgrp - 1) * RG + rgrp) * kRec) + lane;
-    if (kgrp > 0) {
+    constexpr int kPitch = D + 4, kLanes = D / 4;
+    float* sums = reinterpret_cast<float*>(smem);
+    float* mine = sums + (size_t)(wave * 32 + j) * kPitch;
+    if (live[0]) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) mine[64 * (16 * dt + v)] = o[0][dt][v];
-      mine[64 * (D / 2)] = ref[0];
-      mine[64 * (D / 2 + 1)] = lsum[0];
+        for (int v = 0; v < 16; v += 4)
+          *reinterpret_cast<f32x4*>(mine + 32 * dt + 2 * v + 4 * h) = f32x4{o[0][dt][v], o[0][dt][v + 1], o[0][dt][v + 2], o[0][dt][v + 3]};
+      if (h == 0) {
+        mine[D] = ref[0];
+        mine[D + 1] = lsum[0];
+      }
     }
     lds_barrier();
-    if (kgrp > 0) return;
-    for (int g2 = 1; g2 < KG; ++g2) {
-      const float* theirs = reinterpret_cast<const float*>(smem + (size_t)((g2 - 1) * RG + rgrp) * kRec) + lane;
-      const float r2 = theirs[64 * (D / 2)], nm = fmaxf(ref[0], r2);
-      const float f0 = ref[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[0] - nm);
-      const float f1 = r2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r2 - nm);
-      ref[0] = nm;
-      lsum[0] = lsum[0] * f0 + theirs[64 * (D / 2 + 1)] * f1;
+    const int d = 4 * (tid % kLanes);
+    for (int r = tid / kLanes; r < min(kRows, rows - un.tile * kRows); r += 256 / kLanes) {
+      const float* at = sums + (size_t)((r >> 5) * 32 + (r & 31)) * kPitch;   // row group r / 32: waves r / 32 + RG k
+      float top = -INFINITY, den = 0.f;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int k = 0; k < KG; ++k) top = fmaxf(top, at[k * RG * 32 * kPitch + D]);
+      f32x4 num = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int v = 0; v < 16; ++v) o[0][dt][v] = o[0][dt][v] * f0 + theirs[64 * (16 * dt + v)] * f1;
+      for (int k = 0; k < KG; ++k) {
+        const float* theirs = at + k * RG * 32 * kPitch;
+        const float m = theirs[D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(theirs + d);
+        den = fmaf(f, theirs[D + 1], den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[e], num[e]);
+      }
+      const int row = un.tile * kRows + r, tok = div(row, plan.by_g), g = row - tok * G;
+      if (un.parts == 1) {
+        store_row<T>(out + ((int64_t)(un.first + tok) * Hq + un.hk * G + g) * D + d, num, den, un.len - un.nq + tok >= 0);
+      } else {
+        float* rec = part + ((size_t)un.rec * kRows + r) * paged_rec<D>();
+        if (d == 0) {
+          rec[0] = top;
+          rec[1] = den;
+        }
+        *reinterpret_cast<f32x4*>(rec + 4 + d) = num;
+      }
     }
+    return;
   }
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     if (!live[r]) continue;
     // lane (j, h) holds O^T[32 dt + 8 (v / 4) + 4 h + v % 4][row j]
     if (un.parts == 1) {
-      const bool some = pr[r] >= 0;                           // a row without a key: zeros
-      const float inv = some ? 1.f / lsum[r] : 0.f;
       T* dst = out + qrow[r] + 4 * h;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-          const uint32_t lo = some ? Mfma<T>::pack(o[r][dt][v] * inv, o[r][dt][v + 1] * inv) : 0u;
-          const uint32_t hi = some ? Mfma<T>::pack(o[r][dt][v + 2] * inv, o[r][dt][v + 3] * inv) : 0u;
-          *reinterpret_cast<uint2*>(dst + 32 * dt + 2 * v) = make_uint2(lo, hi);
-        }
+        for (int v = 0; v < 16; v += 4)
+          store_row<T>(dst + 32 * dt + 2 * v, f32x4{o[r][dt][v], o[r][dt][v + 1], o[r][dt][v + 2], o[r][dt][v + 3]}, lsum[r], pr[r] >= 0);
     } else {
       float* rec = part + ((size_t)un.rec * kRows + 32 * (NR * rgrp + r) + j) * paged_rec<D>();
       if (h == 0) {
@@ -512,47 +575,82 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
   }
 }
 
-// The outputs of the split tiles: a workgroup takes tile blockIdx.x of them and 1024 / D of its rows, D / 4 lanes a row; the
-// parts are joined in order, their weights 2^(reference - largest reference) against the sum's.
-template <typename T, int D>
+// The outputs of the split tiles: a workgroup takes chunks of paged_merge_rows rows, four lane groups a row, each joining
+// every fourth part in order, their weights 2^(reference - largest reference); then the four groups' sums.
+template <int D>
+constexpr int paged_merge_rows() { return 256 / D; }
+template <typename T, int D, int kRows, int kBlock>
 __global__ __launch_bounds__(256) void paged_attention_merge(const float* __restrict__ part, PagedBatch bt, PagedPlan plan,
-                                                             T* __restrict__ out, int Hq, int Hkv) {
-  constexpr int kLanes = D / 4, kRowsHere = 256 / kLanes, kRec = paged_rec<D>();
-  const int G = Hq / Hkv;
+                                                             T* __restrict__ out) {
+  constexpr int kLanes = D / 4, kHere = paged_merge_rows<D>(), kRec = paged_rec<D>();
+  __shared__ f32x4 s_num[256];
+  __shared__ float s_top[256 / kLanes], s_den[256 / kLanes];
+  args_in_sgprs(part, bt.table, bt.q_starts, bt.kv_lens, bt.B, bt.T, bt.table_width, bt.page_size, plan.slots, plan.cap, plan.G,
+                plan.by_hkv.m, plan.by_g.m, out);
+  const int lane = threadIdx.x & 63, grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  const PagedSeq s0 = paged_seq<kRows, kBlock>(bt, plan.G, lane);
+  const int share = paged_share<kRows, kBlock>(bt, plan, s0, lane);
   PagedUnit un;
-  if (!paged_unit<true>(bt, plan, G, Hkv, blockIdx.x, threadIdx.x & 63, un)) return;
-  const int r = blockIdx.y * kRowsHere + threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
-  const int row = un.tile * plan.rows + r, tok = row / G, g = row - tok * G;
-  if (row >= un.nq * G) return;
-  const float* rec = part + ((size_t)un.rec * plan.rows + r) * kRec;
-  const size_t step = (size_t)plan.rows * kRec;
-  float top = -INFINITY;
-  for (int p = 0; p < un.parts; ++p) top = fmaxf(top, rec[p * step]);
-  f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  float den = 0.f;
-  for (int p0 = 0; p0 < un.parts; p0 += 8) {                  // eight records' loads in flight
-    f32x4 v[8];
-    float m[8], l[8];
+  for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
+    const int r = un.pid * kHere + (grp >> 2), row = un.tile * kRows + r;
+    const float* rec = part + ((size_t)un.rec * kRows + r) * kRec;
+    const size_t step = (size_t)kRows * kRec;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f, top = -INFINITY;
+    if (row < un.nq * plan.G) {
+      for (int p0 = grp & 3; p0 < un.parts; p0 += 32) {       // eight records' loads in flight
+        f32x4 v[8];
+        float m[8], l[8], nm = top;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float* at = rec + (size_t)min(p0 + i, un.parts - 1) * step;
-      m[i] = at[0];
-      l[i] = at[1];
-      v[i] = *reinterpret_cast<const f32x4*>(at + 4 + d);
+        for (int i = 0; i < 8; ++i) {
+          const float* at = rec + (size_t)min(p0 + 4 * i, un.parts - 1) * step;
+          m[i] = at[0];
+          l[i] = at[1];
+          v[i] = *reinterpret_cast<const f32x4*>(at + 4 + 4 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (p0 + 4 * i >= un.parts) m[i] = -INFINITY;
+          nm = fmaxf(nm, m[i]);
+        }
+        const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - nm);
+        den *= f0;
+        num *= f0;
+        top = nm;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (m[i] == -INFINITY) continue;                    // (a part that saw no key)
+          const float f = __builtin_amdgcn_exp2f(m[i] - top);
+          den = fmaf(f, l[i], den);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[i][e], num[e]);
+        }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (p0 + i >= un.parts || m[i] == -INFINITY) continue;  // (a part that saw no key)
-      const float f = __builtin_amdgcn_exp2f(m[i] - top);
-      den = fmaf(f, l[i], den);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[i][e], num[e]);
+    s_num[threadIdx.x] = num;
+    if (c == 0) {
+      s_top[grp] = top;
+      s_den[grp] = den;
     }
+    __syncthreads();
+    if ((grp & 3) == 0 && row < un.nq * plan.G) {
+#pragma unroll
+      for (int i = 1; i < 4; ++i) top = fmaxf(top, s_top[grp + i]);
+      num = f32x4{0.f, 0.f, 0.f, 0.f};
+      den = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        den = fmaf(f, s_den[grp + i], den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + i * kLanes][e], num[e]);
+      }
+      const int tok = div(row, plan.by_g), g = row - tok * plan.G;
+      store_row<T>(out + ((int64_t)(un.first + tok) * plan.Hq + un.hk * plan.G + g) * D + 4 * c, num, den,
+                   un.len - un.nq + tok >= 0);
+    }
+    __syncthreads();
   }
-  const bool some = un.len - un.nq + tok >= 0;                // a row without a key: zeros
-  const float inv = some ? 1.f / den : 0.f;
-  T* dst = out + ((int64_t)(un.first + tok) * Hq + un.hk * G + g) * D + d;
-  *reinterpret_cast<uint2*>(dst) = some ? make_uint2(Mfma<T>::pack(num[0] * inv, num[1] * inv), Mfma<T>::pack(num[2] * inv, num[3] * inv)) : make_uint2(0u, 0u);
 }
 
 namespace {
@@ -569,17 +667,24 @@ hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t st) {
 constexpr int kPagedParts = 256;                             // of a tile at most
 constexpr int kPagedLeast = 256;                             // keys of a part at least
 
+FastDiv fast_div(int d) {
+  if (d == 1) return {0, 0};
+  int l = 1;
+  while ((int64_t)1 << l < d) ++l;
+  return {(uint32_t)((((uint64_t)1 << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), l - 1};
+}
+
 template <typename T, int D, int RG, int KG, int NR>
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   constexpr size_t lds = paged_lds<D, RG, KG>();
+  constexpr int kRows = 32 * NR * RG, kBlock = 32 * KG;
   const int G = a.Hq / a.Hkv;
-  PagedPlan p{32 * NR * RG, 32 * KG, 256 * (KG == 4 || NR > 1 ? 1 : 2), 0, 1, 0};
-  p.least = std::max(1, kPagedLeast / p.block);
-  const int64_t units = (((int64_t)a.batch.T * G + p.rows - 1) / p.rows + std::min(a.batch.B, a.batch.T)) * a.Hkv;
-  const size_t group = (size_t)p.rows * paged_rec<D>() * sizeof(float);
-  p.most = (int)std::min<size_t>(3 * (size_t)p.slots, a.ws_bytes / group);
+  PagedPlan p{256 * (KG == 4 || NR > 1 ? 1 : 2), std::max(1, kPagedLeast / kBlock), 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
+  const int64_t seqs = std::min(a.batch.B, a.batch.T);        // with new tokens
+  const int64_t units = (((int64_t)a.batch.T * G + kRows - 1) / kRows + seqs) * a.Hkv;
+  p.most = (int)std::min<size_t>(3 * (size_t)p.slots, a.ws_bytes / ((size_t)kRows * paged_rec<D>() * sizeof(float)));
   if (a.ws && p.most >= 2)
-    p.cap = std::min(kPagedParts, (int)((((int64_t)a.max_keys + p.block - 1) / p.block + p.least - 1) / p.least));
+    p.cap = std::min(kPagedParts, (int)((((int64_t)a.max_keys + kBlock - 1) / kBlock + p.least - 1) / p.least));
   const int64_t grid = p.cap == 1 ? units : std::min<int64_t>(units * p.cap, units + p.most / 2 + 1);
   if (lds > 65536) {
     static std::atomic<uint64_t> done{0};
@@ -589,11 +694,12 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   while ((1 << shift) < a.batch.page_size) ++shift;
   hipError_t e = launch(paged_attention<T, D, RG, KG, NR>, dim3((unsigned)grid), dim3(256), lds, st,
                         static_cast<const T*>(a.q), static_cast<const T*>(a.k_cache), static_cast<const T*>(a.v_cache),
-                        a.batch, p, static_cast<T*>(a.out), static_cast<float*>(a.ws), a.Hq, a.Hkv, shift, a.scale);
+                        a.batch, p, static_cast<T*>(a.out), static_cast<float*>(a.ws), shift, a.scale);
   if (e != hipSuccess || p.cap == 1) return e;
-  const int64_t split = std::min<int64_t>(units, p.most / 2 + 1);
-  return launch(paged_attention_merge<T, D>, dim3((unsigned)split, (unsigned)(p.rows * D / 1024)), dim3(256), 0, st,
-                static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.Hq, a.Hkv);
+  constexpr int kHere = paged_merge_rows<D>();
+  const int64_t chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
+  return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 512)), dim3(256), 0, st,
+                static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out));
 }
 
 template <typename T, int D>
