@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const T* __restrict__ qk
 }
 
 // ---- attention_paged ----
-// A workgroup takes 32 NR RG query rows of one sequence and KV head (row = new token * G + head in the group) and walks a
+// A workgroup takes 32 RG query rows of one sequence and KV head (row = new token * G + head in the group) and walks a
 // range of the sequence's keys; see paged_attention. The work of a call is numbered along blockIdx.x, and every workgroup
 // finds its own part from the sequences' lengths, so that a captured launch serves any lengths:
 //   a sequence has tiles of rows, and its keys are cut into `parts` alike for all its tiles, `parts` being its blocks of keys
@@ -127,9 +127,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int se
   return s;
 }
 
-// The parts' share in blocks: total blocks over the slots that tiles of one part leave free in the call's rounds of
-// workgroups (half a round at least), so that the parts, each sequence's rounded up, fill whole rounds. s0: the first 64
-// sequences.
+// The parts' share in blocks. While tiles of one part leave a quarter of the GPU's slots free, the total over the free ones,
+// so that the parts, each sequence's rounded up, run at once; else the total over one and a half rounds of slots, so that only
+// keys far above the mean are cut (64 decode tokens on 300 .. 8000 keys, us: over the slots that two rounds leave free 132,
+// one round 133, one and a half 125, two 128; a prompt of 2000 tokens, 28 / 4 heads: 73, 60 and 78 with half a round, one and
+// two). s0: the first 64 sequences.
 template <int kRows, int kBlock>
 __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {
   if (p.cap == 1) return 0x3FFFFFFF;
@@ -141,8 +143,8 @@ __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan&
   }
   total *= (float)p.Hkv;
   units *= (float)p.Hkv;
-  const float slots = (float)p.slots, rounds = ceilf((units + 0.5f * slots) / slots);
-  const float free = fminf(rounds * slots - units, (float)(p.most / 2));
+  const float slots = (float)p.slots;
+  const float free = fminf(units < 0.75f * slots ? slots - units : 1.5f * slots, (float)(p.most / 2));
   return max(p.least, (int)fminf(ceilf(total / free), 1e9f));
 }
 
@@ -202,6 +204,9 @@ struct Mfma<f16> {
     typedef f16 x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, x2));
   }
+  static __device__ __forceinline__ float sum2(uint32_t p, float c) {   // c + the two values
+    return dot2(as_f16x2(p), f16x2{(f16)1.f, (f16)1.f}, c);
+  }
 };
 template <>
 struct Mfma<bf16> {
@@ -212,6 +217,9 @@ struct Mfma<bf16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     typedef bf16 x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, x2));
+  }
+  static __device__ __forceinline__ float sum2(uint32_t p, float c) {
+    return c + (__builtin_bit_cast(float, p << 16) + __builtin_bit_cast(float, p & 0xFFFF0000u));
   }
 };
 
@@ -224,52 +232,61 @@ __device__ __forceinline__ void store_row(T* dst, const f32x4& num, float den, b
 }
 
 // blocks ahead that K and V are requested, and the slots of LDS that takes
-template <int KG>
-constexpr int paged_ahead() { return KG == 4 ? 1 : 2; }
+template <int RG, int KG>
+constexpr int paged_ahead() { return KG == 4 || RG * KG == 1 ? 1 : 3; }
 template <int D, int RG, int KG>
 constexpr size_t paged_lds() {
-  const size_t ring = (size_t)(paged_ahead<KG>() + 1) * 2 * 32 * KG * D * 2;
+  const size_t ring = (size_t)(paged_ahead<RG, KG>() + 1) * 2 * 32 * KG * D * 2;
   const size_t merge = KG > 1 ? (size_t)4 * 32 * (D + 4) * 4 : 0;
   return ring > merge ? ring : merge;
 }
+template <int RG, int KG>
+constexpr int paged_per_cu() { return KG > 1 ? 1 : RG == 1 ? 5 : 2; }   // workgroups, by their LDS at D = 128
 template <int D>
 constexpr int paged_rec() { return D + 4; }                  // floats of a row's record: reference, weight sum, -, -, output
 
-// Four waves: RG row groups of 32 NR rows times KG key groups; a block is 32 KG keys, wave (rg, kg) taking the block's 32 keys
-// of key group kg for its rows. Per 32 keys (32x32x16 MFMA, lane l: j = l % 32, h = l / 32):
+// RG row groups of 32 rows times KG key groups, a wave each (4 x 1, 2 x 2, 1 x 4 or 1 x 1); a block is 32 KG keys, wave (rg, kg)
+// taking the block's 32 keys of key group kg for its rows. Per 32 keys (32x32x16 MFMA, lane l: j = l % 32, h = l / 32):
 //   S^T = K Q^T: A = 32 keys x 16 dims from LDS, B = 32 rows (registers); lane (j, h) holds row j's scores of keys 8 (v / 4) +
 //   4 h + v % 4, v < 16.
 //   Softmax in base 2 against a reference that follows the running maximum only when a score passes it by more than kLag, so
 //   that the output's registers are rescaled in the first blocks only. Weights are 2^(score - reference + 15 - kLag), the
 //   largest between 2^(15 - kLag) and 2^15, rounded to T for the second product: half a step of T for each weight, the same
-//   relative step as the output's own rounding (fp16: down to 2^-14, i.e. 2^-25 of the largest weight, and half of 2^-24
-//   below); their sum is of the unrounded weights in 32 bits.
+//   relative step as the output's own rounding; in fp16 those below 2^-14 are off by 2^-25, i.e. 2^-32 of the largest. Their
+//   sum, in 32 bits, is of the rounded weights, as the output's is.
 //   O^T += V^T P^T: B = the weights as the lane holds them, A = V^T from LDS by transposing reads.
-// K and V go from the pages straight to LDS, rows as they are: a wave-load takes 1 KB, 512 / D keys, which lie in one page, so
-// that its page number, address and bound are scalar; rows past the sequence's keys and pages outside the cache read as zeros
-// through the bound, so nothing unwritten meets the products. The 16-byte pieces of a row are permuted by the key: K's so
-// that the 32 rows of a fragment read meet different banks, V's so that the four rows of a transposing read do. K's are
-// requested paged_ahead + 1 blocks before their scores' softmax, V's paged_ahead, and a block's scores are multiplied while
-// the vector unit evaluates the block before. With KG == 4 a wave loads the keys it takes itself and no barrier is needed.
-constexpr float kLag = 4.f;
+// K and V go from the pages straight to LDS, rows as they are: a wave-load takes 1 KB, 512 / D keys, in groups of up to 16 keys
+// of one page, so that address and bound are scalar and looked up once a group; rows past the sequence's keys and pages
+// outside the cache read as zeros through the bound, so nothing unwritten meets the products. The 16-byte pieces of a row are
+// permuted by the key: K's so that the 32 rows of a fragment read meet different banks, V's so that the four rows of a
+// transposing read do (no conflict is counted). K is requested paged_ahead + 1 blocks before its scores' weights, V
+// paged_ahead, and a block's scores are multiplied while the vector unit evaluates the block before. With one row group a
+// wave loads the keys it takes itself and no barrier is needed.
+// Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 125 us, 5.0
+// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 69 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 500 us, 0.91
+// PFLOP/s, on zeros 407 us at full clock (1.13), where the vector unit and the matrix cores are busy 50% and 44%. There,
+// measured and not kept: 64 rows a wave with one wave per SIMD (half the LDS reads) 703 us; eight waves in two turns, one four
+// on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three waves per SIMD (168 registers,
+// spilled) 546; two blocks ahead instead of three 519 .. 536.
+constexpr float kLag = 8.f;
 
-template <typename T, int D, int RG, int KG, int NR>
-__global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attention(
+template <typename T, int D, int RG, int KG>
+__global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, PagedBatch bt, PagedPlan plan,
     T* __restrict__ out, float* __restrict__ part, int shift, float scale) {
-  static_assert(RG * KG == 4, "four waves");
+  constexpr int NW = RG * KG;
   constexpr int RB = D * 2;                                  // bytes of a row
   constexpr int PR = RB / 16;                                // its pieces
   constexpr int KL = 64 / PR;                                // keys of a wave-load
   constexpr int BK = 32 * KG;
   constexpr int BB = BK * RB;                                // bytes of a block of K, and of V
-  constexpr int KW = BK / 4;                                 // keys of a block that a wave loads
+  constexpr int KW = BK / NW;                                // keys of a block that a wave loads
   constexpr int NG = (KW + 15) / 16, LG = KW / NG / KL;      // groups of them, wave-loads of a group
   constexpr int NP = NG * LG;                                // wave-loads of a wave and block, for K and for V
-  constexpr int AH = paged_ahead<KG>(), N = AH + 1;          // slots: [N] K blocks, [N] V blocks
+  constexpr int AH = paged_ahead<RG, KG>(), N = AH + 1;          // slots: [N] K blocks, [N] V blocks
   constexpr bool kOwn = RG == 1;                             // a wave loads its own keys
   constexpr int DT = D / 32, KS = D / 16;
-  constexpr int kRows = 32 * NR * RG;
+  constexpr int kRows = 32 * RG;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   args_in_sgprs(q, k_cache, v_cache, bt.table, bt.q_starts, bt.kv_lens, bt.B, bt.T, bt.table_width, bt.page_size, plan.slots,
                 plan.cap, plan.G, plan.by_hkv.m, plan.by_g.m, out, part, shift);
@@ -289,32 +306,25 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
   const int per = un.parts == 1 ? nblk : (int)((uint32_t)(nblk + un.parts - 1) / (uint32_t)un.parts);
   const int b0 = min(nblk, un.pid * per), b1 = min(nblk, b0 + per);
   const int kend = min(keys, b1 * BK);
-  // the rows' last keys, least and most of a row group, and q
-  int pr[NR], wmin[NR];
-  bool live[NR];
-  int64_t qrow[NR];
-  u32x4 qf[NR][KS];
-  const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;      // a negative scale is moved into q (exact)
+  // this lane's row: its last key (the least of the wave's rows: wmin) and q
   const float c2 = fabsf(scale) * 1.44269504088896340736f < FLT_MIN ? FLT_MIN : fabsf(scale) * 1.44269504088896340736f;
+  const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;      // a negative scale is moved into q (exact)
+  const int row = un.tile * kRows + 32 * rgrp + j, row_c = min(row, rows - 1), tok = div(row_c, plan.by_g);
+  const bool live = row < rows;
+  const int pr = live ? min(un.len - un.nq + tok, cap - 1) : -1;
+  int wmin = live ? pr : INT_MAX;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    const int row = un.tile * kRows + 32 * (NR * rgrp + r) + j;
-    live[r] = row < rows;
-    const int c = min(row, rows - 1), tok = div(c, plan.by_g), g = c - tok * G;
-    pr[r] = live[r] ? min(un.len - un.nq + tok, cap - 1) : -1;
-    wmin[r] = live[r] ? pr[r] : INT_MAX;
+  for (int off = 1; off < 32; off <<= 1) wmin = min(wmin, __shfl_xor(wmin, off, 64));
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  const int64_t qrow = ((int64_t)(un.first + tok) * Hq + un.hk * G + (row_c - tok * G)) * D;
+  u32x4 qf[KS];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) wmin[r] = min(wmin[r], __shfl_xor(wmin[r], o, 64));
-    wmin[r] = __builtin_amdgcn_readfirstlane(wmin[r]);
-    qrow[r] = ((int64_t)(un.first + tok) * Hq + un.hk * G + g) * D;
+  for (int s = 0; s < KS; ++s) {
+    qf[s] = load16(q + qrow + 16 * s + 8 * h);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[r][s] = load16(q + qrow[r] + 16 * s + 8 * h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qf[r][s][e] ^= flip;
-    }
+    for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
   }
-  const bool busy = wmin[0] != INT_MAX;                      // a wave whose rows are all past the end only loads
+  const bool busy = wmin != INT_MAX;                         // a wave whose rows are all past the end only loads
 
   // ---- loads ----
   // where the 128 pages from `win` on begin in a cache, lane l holding pages win + l and win + 64 + l: byte offsets of this KV
@@ -396,75 +406,60 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  float ref[NR], lsum[NR];
-  f32x16 o[NR][DT], st[NR];
+  float ref = -INFINITY, lsum[2] = {0.f, 0.f};                // reference (base 2), the lane's share of the weights' sum
   const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  f32x16 o[DT], st = zero;                                    // output, scores of the wave's 32 keys of a block
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    ref[r] = -INFINITY;
-    lsum[r] = 0.f;
-    st[r] = zero;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[r][dt] = zero;
-  }
-  auto scores = [&](uint32_t at, int s0, int s1) {
-#pragma unroll
-    for (int s = s0; s < s1; ++s) {
-      const u32x4 kf = *reinterpret_cast<const u32x4*>(smem + at + (kr ^ (32 * s)));
-#pragma unroll
-      for (int r = 0; r < NR; ++r) st[r] = Mfma<T>::go(kf, qf[r][s], st[r]);
-    }
-  };
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero;
+  auto k_frag = [&](uint32_t at, int s) { return *reinterpret_cast<const u32x4*>(smem + at + (kr ^ (32 * s))); };
+  // One block: the weights of its scores, the weights times V and the next block's scores. Every fragment is read well before
+  // its product (K's and V's first half at the start, V's other half while K's are multiplied)
   auto block = [&](uint32_t kat, uint32_t vat, int kb) {      // kb: the wave's first key
-    f32x16 sc[NR];
-    float sub[NR];
+    u32x4 kf[KS], va[2][DT];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      if (kb + 31 > min(wmin[r], kend - 1)) {                 // some row attends part of these keys only (uniform)
-        const int last = min(pr[r], kend - 1) - kb - 4 * h;   // a key at or below it counts
+    for (int s = 0; s < KS; ++s) kf[s] = k_frag(kat, s);
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (8 * (v >> 2) + (v & 3) > last) st[r][v] = -INFINITY;
-      }
-      float bm = st[r][0];
+    for (int dt = 0; dt < DT; ++dt) va[0][dt] = v_frag(vat + (vr ^ (64 * dt)));
+    __builtin_amdgcn_sched_barrier(0);
+    if (kb + 31 > min(wmin, kend - 1)) {                      // some row attends part of these keys only (uniform)
+      const int last = min(pr, kend - 1) - kb - 4 * h;        // a key at or below it counts
 #pragma unroll
-      for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[r][v]);
-      if (__any(bm * c2 > ref[r] + kLag)) {                   // (uniform; either lane of a row)
-        const float nm = fmaxf(ref[r], fmaxf(bm, __shfl_xor(bm, 32, 64)) * c2);   // -inf while the row has seen no key
-        const float corr = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref[r] - nm);
-        ref[r] = nm;
-        lsum[r] *= corr;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[r][dt] *= corr;
-      }
-      sub[r] = ref[r] == -INFINITY ? 0.f : ref[r] - (15.f - kLag);
-      sc[r] = st[r];
-      st[r] = zero;
+      for (int v = 0; v < 16; ++v)
+        if (8 * (v >> 2) + (v & 3) > last) st[v] = -INFINITY;
     }
+    float bm = st[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
+    if (__any(bm * c2 > ref + kLag)) {                        // (uniform; either lane of a row)
+      const float nm = fmaxf(ref, fmaxf(bm, __shfl_xor(bm, 32, 64)) * c2);   // -inf while the row has seen no key
+      const float corr = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nm);
+      ref = nm;
+      lsum[0] *= corr;
+      lsum[1] *= corr;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
+    }
+    const float sub = ref == -INFINITY ? 0.f : ref - (15.f - kLag);
+    const f32x16 sc = st;
+    st = zero;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {                             // 16 keys
-      u32x4 ph[NR];
+      u32x4 ph;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float ps[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r][8 * s + 2 * i], c2, -sub[r]));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r][8 * s + 2 * i + 1], c2, -sub[r]));
-          ps[0] += p0;
-          ps[1] += p1;
-          ph[r][i] = Mfma<T>::pack(p0, p1);
-        }
-        lsum[r] += ps[0] + ps[1];
+      for (int i = 0; i < 4; ++i) {
+        ph[i] = Mfma<T>::pack(__builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i], c2, -sub)),
+                              __builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i + 1], c2, -sub)));
+        lsum[i & 1] = Mfma<T>::sum2(ph[i], lsum[i & 1]);
       }
-      scores(kat, KS / 2 * s, KS / 2 * s + KS / 2);           // of the next block (past the last one: zeros, not used)
-      u32x4 va[DT];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) va[dt] = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB * s);
+      for (int i = KS / 2 * s; i < KS / 2 * s + KS / 2; ++i)  // the next block's (past the last one: of zeros, not used)
+        st = Mfma<T>::go(kf[i], qf[i], st);
+      if (s == 0) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt) va[1][dt] = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
+      }
 #pragma unroll
-        for (int r = 0; r < NR; ++r) o[r][dt] = Mfma<T>::go(va[dt], ph[r], o[r][dt]);
+      for (int dt = 0; dt < DT; ++dt) o[dt] = Mfma<T>::go(va[s][dt], ph, o[dt]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -485,44 +480,50 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
       load(kbase, at, koff, slot((t + 1) % N));
     }
     sync(std::integral_constant<int, 2 * NP * AH>{});
-    if (busy) scores(slot(0), 0, KS);
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) st = Mfma<T>::go(k_frag(slot(0), i), qf[i], st);
+    }
     sync(std::integral_constant<int, 2 * NP * (AH - 1)>{});
-    int a = 0;                                                // i % N
-    for (int i = b0; i < b1; ++i) {
-      const int a1 = a + 1 == N ? 0 : a + 1, am = a == 0 ? N - 1 : a - 1;
-      load(vbase, at, voff, kV + slot(am));
-      at = rows_of(i + 1 + AH);
-      load(kbase, at, koff, slot(a));
-      if (busy) block(slot(a1), slot(a), i * BK + 32 * kgrp);
-      sync(std::integral_constant<int, 2 * NP * (AH - 1)>{});
-      a = a1;
+    // unrolled over the slots, so that every LDS address is a register and a constant, and over two blocks, so that the
+    // next block's scores need no copy
+    constexpr int U = N % 2 ? 2 * N : N;
+    for (int i = b0; i < b1; i += U) {
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        if (i + t >= b1) break;
+        load(vbase, at, voff, kV + slot((t + AH) % N));
+        at = rows_of(i + t + 1 + AH);
+        load(kbase, at, koff, slot(t % N));
+        if (busy) block(slot((t + 1) % N), slot(t % N), (i + t) * BK + 32 * kgrp);
+        sync(std::integral_constant<int, 2 * NP * (AH - 1)>{});
+      }
     }
     lds_wait_barrier<0>();                                    // nothing is left in flight, and the slots may be reused
   }
-#pragma unroll
-  for (int r = 0; r < NR; ++r) lsum[r] += __shfl_xor(lsum[r], 32, 64);
+  float den = lsum[0] + lsum[1];
+  den += __shfl_xor(den, 32, 64);
   if constexpr (KG > 1) {
     // the key groups' sums meet in LDS as rows, reference and weight sum behind each, and leave 16 bytes of a row a lane
-    static_assert(NR == 1, "one row group a wave");
     constexpr int kPitch = D + 4, kLanes = D / 4;
     float* sums = reinterpret_cast<float*>(smem);
     float* mine = sums + (size_t)(wave * 32 + j) * kPitch;
-    if (live[0]) {
+    if (live) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int v = 0; v < 16; v += 4)
-          *reinterpret_cast<f32x4*>(mine + 32 * dt + 2 * v + 4 * h) = f32x4{o[0][dt][v], o[0][dt][v + 1], o[0][dt][v + 2], o[0][dt][v + 3]};
+          *reinterpret_cast<f32x4*>(mine + 32 * dt + 2 * v + 4 * h) = f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
       if (h == 0) {
-        mine[D] = ref[0];
-        mine[D + 1] = lsum[0];
+        mine[D] = ref;
+        mine[D + 1] = den;
       }
     }
     lds_barrier();
     const int d = 4 * (tid % kLanes);
     for (int r = tid / kLanes; r < min(kRows, rows - un.tile * kRows); r += 256 / kLanes) {
       const float* at = sums + (size_t)((r >> 5) * 32 + (r & 31)) * kPitch;   // row group r / 32: waves r / 32 + RG k
-      float top = -INFINITY, den = 0.f;
+      float top = -INFINITY, all = 0.f;
 #pragma unroll
       for (int k = 0; k < KG; ++k) top = fmaxf(top, at[k * RG * 32 * kPitch + D]);
       f32x4 num = {0.f, 0.f, 0.f, 0.f};
@@ -531,58 +532,58 @@ __global__ __launch_bounds__(256, KG == 4 || NR > 1 ? 1 : 2) void paged_attentio
         const float* theirs = at + k * RG * 32 * kPitch;
         const float m = theirs[D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
         const f32x4 v = *reinterpret_cast<const f32x4*>(theirs + d);
-        den = fmaf(f, theirs[D + 1], den);
+        all = fmaf(f, theirs[D + 1], all);
 #pragma unroll
         for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[e], num[e]);
       }
-      const int row = un.tile * kRows + r, tok = div(row, plan.by_g), g = row - tok * G;
+      const int at_row = un.tile * kRows + r, t = div(at_row, plan.by_g), g = at_row - t * G;
       if (un.parts == 1) {
-        store_row<T>(out + ((int64_t)(un.first + tok) * Hq + un.hk * G + g) * D + d, num, den, un.len - un.nq + tok >= 0);
+        store_row<T>(out + ((int64_t)(un.first + t) * Hq + un.hk * G + g) * D + d, num, all, un.len - un.nq + t >= 0);
       } else {
         float* rec = part + ((size_t)un.rec * kRows + r) * paged_rec<D>();
         if (d == 0) {
           rec[0] = top;
-          rec[1] = den;
+          rec[1] = all;
         }
         *reinterpret_cast<f32x4*>(rec + 4 + d) = num;
       }
     }
     return;
   }
+  if (!live) return;
+  // lane (j, h) holds O^T[32 dt + 8 (v / 4) + 4 h + v % 4][row j]
+  if (un.parts == 1) {
+    T* dst = out + qrow + 4 * h;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    if (!live[r]) continue;
-    // lane (j, h) holds O^T[32 dt + 8 (v / 4) + 4 h + v % 4][row j]
-    if (un.parts == 1) {
-      T* dst = out + qrow[r] + 4 * h;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int v = 0; v < 16; v += 4)
-          store_row<T>(dst + 32 * dt + 2 * v, f32x4{o[r][dt][v], o[r][dt][v + 1], o[r][dt][v + 2], o[r][dt][v + 3]}, lsum[r], pr[r] >= 0);
-    } else {
-      float* rec = part + ((size_t)un.rec * kRows + 32 * (NR * rgrp + r) + j) * paged_rec<D>();
-      if (h == 0) {
-        rec[0] = ref[r];
-        rec[1] = lsum[r];
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int v = 0; v < 16; v += 4)
-          *reinterpret_cast<f32x4*>(rec + 4 + 32 * dt + 2 * v + 4 * h) = f32x4{o[r][dt][v], o[r][dt][v + 1], o[r][dt][v + 2], o[r][dt][v + 3]};
+      for (int v = 0; v < 16; v += 4)
+        store_row<T>(dst + 32 * dt + 2 * v, f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]}, den, pr >= 0);
+  } else {
+    float* rec = part + ((size_t)un.rec * kRows + 32 * rgrp + j) * paged_rec<D>();
+    if (h == 0) {
+      rec[0] = ref;
+      rec[1] = den;
     }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<f32x4*>(rec + 4 + 32 * dt + 2 * v + 4 * h) = f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
   }
 }
 
-// The outputs of the split tiles: a workgroup takes chunks of paged_merge_rows rows, four lane groups a row, each joining
-// every fourth part in order, their weights 2^(reference - largest reference); then the four groups' sums.
-template <int D>
-constexpr int paged_merge_rows() { return 256 / D; }
+// The outputs of the split tiles: a workgroup takes chunks of paged_merge_rows rows, PG lane groups a row, each joining every
+// PG-th part in order, their weights 2^(reference - largest reference); then the groups' sums. Tiles of 32 rows, which few
+// rows on many parts take, have four groups a row, the others one.
+template <int kRows>
+constexpr int paged_merge_groups() { return kRows == 32 ? 4 : 1; }
+template <int D, int kRows>
+constexpr int paged_merge_rows() { return 1024 / D / paged_merge_groups<kRows>(); }
 template <typename T, int D, int kRows, int kBlock>
 __global__ __launch_bounds__(256) void paged_attention_merge(const float* __restrict__ part, PagedBatch bt, PagedPlan plan,
                                                              T* __restrict__ out) {
-  constexpr int kLanes = D / 4, kHere = paged_merge_rows<D>(), kRec = paged_rec<D>();
+  constexpr int kLanes = D / 4, PG = paged_merge_groups<kRows>(), kHere = paged_merge_rows<D, kRows>(), kRec = paged_rec<D>();
   __shared__ f32x4 s_num[256];
   __shared__ float s_top[256 / kLanes], s_den[256 / kLanes];
   args_in_sgprs(part, bt.table, bt.q_starts, bt.kv_lens, bt.B, bt.T, bt.table_width, bt.page_size, plan.slots, plan.cap, plan.G,
@@ -592,25 +593,25 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
   const int share = paged_share<kRows, kBlock>(bt, plan, s0, lane);
   PagedUnit un;
   for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
-    const int r = un.pid * kHere + (grp >> 2), row = un.tile * kRows + r;
+    const int r = un.pid * kHere + grp / PG, row = un.tile * kRows + r;
     const float* rec = part + ((size_t)un.rec * kRows + r) * kRec;
     const size_t step = (size_t)kRows * kRec;
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f, top = -INFINITY;
     if (row < un.nq * plan.G) {
-      for (int p0 = grp & 3; p0 < un.parts; p0 += 32) {       // eight records' loads in flight
+      for (int p0 = grp % PG; p0 < un.parts; p0 += 8 * PG) {       // eight records' loads in flight
         f32x4 v[8];
         float m[8], l[8], nm = top;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float* at = rec + (size_t)min(p0 + 4 * i, un.parts - 1) * step;
+          const float* at = rec + (size_t)min(p0 + PG * i, un.parts - 1) * step;
           m[i] = at[0];
           l[i] = at[1];
           v[i] = *reinterpret_cast<const f32x4*>(at + 4 + 4 * c);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (p0 + 4 * i >= un.parts) m[i] = -INFINITY;
+          if (p0 + PG * i >= un.parts) m[i] = -INFINITY;
           nm = fmaxf(nm, m[i]);
         }
         const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - nm);
@@ -627,29 +628,33 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
         }
       }
     }
-    s_num[threadIdx.x] = num;
-    if (c == 0) {
-      s_top[grp] = top;
-      s_den[grp] = den;
+    if constexpr (PG > 1) {
+      s_num[threadIdx.x] = num;
+      if (c == 0) {
+        s_top[grp] = top;
+        s_den[grp] = den;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    if ((grp & 3) == 0 && row < un.nq * plan.G) {
+    if (grp % PG == 0 && row < un.nq * plan.G) {
+      if constexpr (PG > 1) {
 #pragma unroll
-      for (int i = 1; i < 4; ++i) top = fmaxf(top, s_top[grp + i]);
-      num = f32x4{0.f, 0.f, 0.f, 0.f};
-      den = 0.f;
+        for (int i = 1; i < PG; ++i) top = fmaxf(top, s_top[grp + i]);
+        num = f32x4{0.f, 0.f, 0.f, 0.f};
+        den = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        den = fmaf(f, s_den[grp + i], den);
+        for (int i = 0; i < PG; ++i) {
+          const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          den = fmaf(f, s_den[grp + i], den);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + i * kLanes][e], num[e]);
+          for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + i * kLanes][e], num[e]);
+        }
       }
       const int tok = div(row, plan.by_g), g = row - tok * plan.G;
       store_row<T>(out + ((int64_t)(un.first + tok) * plan.Hq + un.hk * plan.G + g) * D + 4 * c, num, den,
                    un.len - un.nq + tok >= 0);
     }
-    __syncthreads();
+    if constexpr (PG > 1) __syncthreads();
   }
 }
 
@@ -674,39 +679,52 @@ FastDiv fast_div(int d) {
   return {(uint32_t)((((uint64_t)1 << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), l - 1};
 }
 
-template <typename T, int D, int RG, int KG, int NR>
+template <typename T, int D, int RG, int KG>
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   constexpr size_t lds = paged_lds<D, RG, KG>();
-  constexpr int kRows = 32 * NR * RG, kBlock = 32 * KG;
+  constexpr int kRows = 32 * RG, kBlock = 32 * KG;
   const int G = a.Hq / a.Hkv;
-  PagedPlan p{256 * (KG == 4 || NR > 1 ? 1 : 2), std::max(1, kPagedLeast / kBlock), 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
+  PagedPlan p{256 * paged_per_cu<RG, KG>(), std::max(1, kPagedLeast / kBlock), 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
   const int64_t seqs = std::min(a.batch.B, a.batch.T);        // with new tokens
   const int64_t units = (((int64_t)a.batch.T * G + kRows - 1) / kRows + seqs) * a.Hkv;
-  p.most = (int)std::min<size_t>(3 * (size_t)p.slots, a.ws_bytes / ((size_t)kRows * paged_rec<D>() * sizeof(float)));
+  p.most = (int)std::min<size_t>(4 * (size_t)p.slots, a.ws_bytes / ((size_t)kRows * paged_rec<D>() * sizeof(float)));
   if (a.ws && p.most >= 2)
     p.cap = std::min(kPagedParts, (int)((((int64_t)a.max_keys + kBlock - 1) / kBlock + p.least - 1) / p.least));
   const int64_t grid = p.cap == 1 ? units : std::min<int64_t>(units * p.cap, units + p.most / 2 + 1);
   if (lds > 65536) {
     static std::atomic<uint64_t> done{0};
-    if (hipError_t e = allow_lds_once(done, paged_attention<T, D, RG, KG, NR>, lds)) return e;
+    if (hipError_t e = allow_lds_once(done, paged_attention<T, D, RG, KG>, lds)) return e;
   }
   int shift = 0;
   while ((1 << shift) < a.batch.page_size) ++shift;
-  hipError_t e = launch(paged_attention<T, D, RG, KG, NR>, dim3((unsigned)grid), dim3(256), lds, st,
+  hipError_t e = launch(paged_attention<T, D, RG, KG>, dim3((unsigned)grid), dim3(64 * RG * KG), lds, st,
                         static_cast<const T*>(a.q), static_cast<const T*>(a.k_cache), static_cast<const T*>(a.v_cache),
                         a.batch, p, static_cast<T*>(a.out), static_cast<float*>(a.ws), shift, a.scale);
   if (e != hipSuccess || p.cap == 1) return e;
-  constexpr int kHere = paged_merge_rows<D>();
+  constexpr int kHere = paged_merge_rows<D, kRows>();
   const int64_t chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
-  return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 512)), dim3(256), 0, st,
+  return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
                 static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out));
 }
 
+// Which tile serves a call; any serves every call. Sequences of at most 32 rows (decode, few drafted tokens) take four waves
+// on four key groups (RG 1, KG 4), one workgroup a CU; where there are more tiles than those and the keys are few, or very many
+// tiles, one wave, five a CU (28 / 4 heads, us, four waves / one: 100 tokens on 100 keys 12.7 / 8.7, 300 on 100 36 / 21, on 1000
+// 150 / 148, 30 tokens of 32 / 32 heads on up to 2000 63 / 57; but 40 on 500 14.5 / 17.3, 100 on 500 32.0 / 32.9, on 2000 89 /
+// 94, 64 of 32 / 8 heads on 300 .. 8000 125 / 139). More rows take four waves of 128 rows (RG 4), two workgroups a CU, or of 64
+// rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts (us, 128
+// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51; /
+// 2 heads of 64, 22.8 / 20.8; 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
 template <typename T, int D>
 hipError_t pick_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.max_new * (a.Hq / a.Hkv);
-  if (rows <= 32) return launch_paged_attention<T, D, 1, 4, 1>(a, st);
-  return launch_paged_attention<T, D, 4, 1, 1>(a, st);
+  const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T);
+  auto tiles = [&](int rows) { return ((int64_t)a.batch.T * G / rows + seqs) * a.Hkv; };   // at most
+  if (a.max_new * G <= 32) {
+    if (tiles(32) > 256 && (a.max_keys <= 512 || tiles(32) > 768)) return launch_paged_attention<T, D, 1, 1>(a, st);
+    return launch_paged_attention<T, D, 1, 4>(a, st);
+  }
+  if (tiles(64) <= 256 && a.max_keys <= 1024) return launch_paged_attention<T, D, 2, 2>(a, st);
+  return launch_paged_attention<T, D, 4, 1>(a, st);
 }
 
 }  // namespace

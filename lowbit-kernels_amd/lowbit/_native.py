@@ -752,8 +752,7 @@ class NativeExt:
         # graphs share none (LOWBIT_PAGED_WORKSPACE_BYTES(rows, D))
         nbytes = 0
         if split and max_keys > PAGED_SPLIT_KEYS:
-            rows = 32 if max_new * hq <= 32 * hkv else 128
-            nbytes = (768 if rows == 32 else 1536) * rows * (dim + 4) * 4
+            nbytes = (1024 * 32 if max_new * hq <= 32 * hkv else 2048 * 128) * (dim + 4) * 4
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged(
             q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),
