@@ -713,8 +713,8 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
 // 150 / 148, 30 tokens of 32 / 32 heads on up to 2000 63 / 57; but 40 on 500 14.5 / 17.3, 100 on 500 32.0 / 32.9, on 2000 89 /
 // 94, 64 of 32 / 8 heads on 300 .. 8000 125 / 139). More rows take four waves of 128 rows (RG 4), two workgroups a CU, or of 64
 // rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts (us, 128
-// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51; /
-// 2 heads of 64, 22.8 / 20.8; 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
+// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51;
+// 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
 template <typename T, int D>
 hipError_t pick_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T);

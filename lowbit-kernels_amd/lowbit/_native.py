@@ -780,9 +780,13 @@ class NativeExt:
             return sums[0], sums[1], values, ids
         if v == 0:
             raise RuntimeError("token_logprobs needs at least one logit a row")
-        _launch(index, lambda stream, ws, nbytes: self.lib.lowbit_token_logprobs(
+        # few rows are cut into slices, whose sums and alternatives lie here for this call alone
+        nbytes = (1024 + m) * (16 + 8 * top) if m < 512 and v >= 4096 else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_token_logprobs(
             logits.data_ptr(), dtypes[logits.dtype], logits.stride(0) if m > 1 else v, targets.data_ptr(), sums.data_ptr(),
-            sums.data_ptr() + 4 * m, values.data_ptr(), ids.data_ptr(), m, v, int(top), ws, nbytes, stream))
+            sums.data_ptr() + 4 * m, values.data_ptr(), ids.data_ptr(), m, v, int(top), ws.data_ptr() if nbytes else None,
+            nbytes, stream))
         return sums[0], sums[1], values, ids
 
     # ---- bandwidth probes (lowbit_hbm_read, lowbit_hbm_copy) ----
