@@ -53,6 +53,9 @@ __device__ __forceinline__ V block_reduce(V v, V* red, Op op) {
   return t;
 }
 
+// this wave's LDS writes so far come before its later reads (one wave: no barrier is needed)
+__device__ __forceinline__ void lds_wave_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 template <typename T>
 __device__ __forceinline__ float value(const u32x4& v, int i) {
   if constexpr (sizeof(T) == 4) {
@@ -101,10 +104,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                                             int V, int top, int S, Sums* __restrict__ part,
                                                             uint64_t* __restrict__ part_keys) {
   constexpr int kN = 16 / sizeof(T);
-  __shared__ float s_max[kGroups * kThreads];                 // [group][lane]
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  float* s_max = reinterpret_cast<float*>(smem);              // [group][thread]
   __shared__ uint64_t s_list[kList];
-  __shared__ float s_red[8];
-  __shared__ uint64_t s_redk[8];
+  __shared__ Sums s_sums[kThreads / 64];
+  __shared__ uint64_t s_redk[kThreads / 64];
+  __shared__ int s_wave[kThreads / 64];
   __shared__ float s_lane[kThreads];
   __shared__ int s_count;
   __shared__ uint32_t s_bound;
@@ -173,12 +178,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     add(v, r == -INFINITY ? 0.f : r);
     mx = fmaxf(mx, v);
   }
+  // the wave's sums against its maximum, then the workgroup's, added by every thread in order of the waves
   Sums s;
-  s.m = block_reduce(mx, s_red, [](float a, float b) { return fmaxf(a, b); });
+  s.m = wave_max(mx);
   move_sums(r, s.m, z, e);
-  auto plus = [](float a, float b) { return a + b; };
-  s.z = block_reduce(z, s_red, plus);
-  s.e = block_reduce(e, s_red, plus);
+  s.z = wave_sum(z);
+  s.e = wave_sum(e);
+  if (lane == 0) s_sums[tid >> 6] = s;
+  s_lane[tid] = mx;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  s = s_sums[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; ++w) s.m = fmaxf(s.m, s_sums[w].m);
+  s.z = s.e = 0.f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    Sums o = s_sums[w];
+    move_sums(o.m, s.m, o.z, o.e);
+    s.z += o.z;
+    s.e += o.e;
+  }
   if (tid == 0) {
     if (S == 1)
       store_sums(x, V, targets[row], s, logprob + row, entropy + row);
@@ -200,28 +220,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     }
   };
   const int held = (v1 - v0) * kN + (slice == 0 ? head : 0) + (slice == S - 1 ? V - tail0 : 0);   // logits of the slice
-  // the bound: the top-th largest of the lanes' maxima, found bit by bit by the first wave
-  s_lane[tid] = mx;
-  if (tid == 0) s_count = 0;
-  __syncthreads();
+  // the bound: the top-th largest of 64 maxima, each of the threads of one lane number, found bit by bit by the first wave
+  // (of 512 maxima it would be a little higher and leave 20 .. 35 logits, not 24 .. 45, but take 8 compares a bit)
   if (tid < 64) {
-    uint32_t k[kThreads / 64];
+    float m = s_lane[lane];
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) k[i] = order_key(s_lane[64 * i + lane]);
+    for (int i = 1; i < kThreads / 64; ++i) m = fmaxf(m, s_lane[64 * i + lane]);
+    const uint32_t k = order_key(m);
     uint32_t bound = 0;
+#pragma unroll
     for (int bit = 31; bit >= 32 - key_bits<T>(); --bit) {
       const uint32_t trial = bound | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 64; ++i) n += __popcll(__ballot(k[i] >= trial));
-      if (n >= top) bound = trial;
+      if (__popcll(__ballot(k >= trial)) >= top) bound = trial;
     }
     if (key_bits<T>() < 32 && !(bound >> 31)) bound |= (1u << (32 - key_bits<T>())) - 1u;   // (negative: the bits are ones)
     if (lane == 0) s_bound = bound;
   }
   __syncthreads();
-  const uint32_t bound_key = s_bound;
-  const float bound = order_value(bound_key);
+  const float bound = order_value(s_bound);
   auto push = [&](float v, int idx) {
     const int at = atomicAdd(&s_count, 1);
     if (at < kList) s_list[at] = rank_key(v, idx);
@@ -271,7 +287,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
             const int o = __shfl_up(upto, off, 64);
             if (lane >= off) upto += o;
           }
-          int* s_wave = reinterpret_cast<int*>(s_red);
           if (lane == 63) s_wave[tid >> 6] = upto;
           __syncthreads();
           int at = n + upto - c, all = n;
@@ -329,20 +344,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   }
 }
 
-// One wave per row: the slices' sums, and the first of their sorted alternatives `top` times.
+// One workgroup per row, whose first wave joins the slices' sums and alternatives.
 template <typename T>
-__global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride,
+__global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride,
                                                            const int64_t* __restrict__ targets,
                                                            float* __restrict__ logprob, float* __restrict__ entropy,
                                                            float* __restrict__ top_value, int64_t* __restrict__ top_id,
                                                            int V, int top, int S, const Sums* __restrict__ part,
                                                            const uint64_t* __restrict__ part_keys) {
-  __shared__ uint64_t s_keys[kMaxSlices * kMaxTop];
+  __shared__ uint64_t s_keys[kMaxSlices * kMaxTop], s_list[kMaxSlices * kMaxTop];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * stride;
   const uint64_t* keys = part_keys + row * S * top;
-  for (int i = lane; i < S * top; i += 64) s_keys[i] = keys[i];
+  for (int i = threadIdx.x; i < S * top; i += 256) s_keys[i] = keys[i];
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
   Sums s = lane < S ? part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};
   const float m = wave_max(s.m);
   move_sums(s.m, m, s.z, s.e);
@@ -350,44 +367,57 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
   s.z = wave_sum(s.z);
   s.e = wave_sum(s.e);
   if (lane == 0) store_sums(x, V, targets[row], s, logprob + row, entropy + row);
-  __syncthreads();
   const bool none = !(s.m > -INFINITY && s.m < INFINITY) || s.z != s.z;
   const float lz = logf(s.z);
-  int next = 0;
-  uint64_t mine = 0;
-  for (int k = 0; k < top; ++k) {
-    const uint64_t first = lane < S && next < top ? s_keys[lane * top + next] : 0;
-    uint64_t best = first;
+  if (top == 0) return;
+  // the top-th largest of the slices' first alternatives bounds the row's: those of each slice's list down to it are ranked by
+  // counting
+  const uint64_t first = lane < S ? s_keys[lane * top] : 0;
+  int above = 0;
+  for (int l = 0; l < S; ++l) above += s_keys[l * top] > first;
+  const uint64_t at_bound = __ballot(lane < S && above == top - 1);   // (keys are distinct; none where S < top)
+  const uint64_t bound = at_bound ? s_keys[__builtin_ctzll(at_bound) * top] : 0;
+  int mine = 0;
+  if (lane < S)
+    while (mine < top && s_keys[lane * top + mine] >= max(bound, (uint64_t)1)) ++mine;
+  int upto = mine;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const uint64_t o = __shfl_xor(best, off, 64);
-      best = o > best ? o : best;
-    }
-    if (first == best) ++next;                                // (keys are distinct)
-    if (lane == k) mine = best;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += o;
   }
-  if (lane < top) {
-    const int idx = rank_index(mine);
-    top_id[row * top + lane] = idx;
-    top_value[row * top + lane] = none ? NAN : ((float)x[idx] - s.m) - lz;
+  for (int i = 0; i < mine; ++i) s_list[upto - mine + i] = s_keys[lane * top + i];
+  const int n = __shfl(upto, 63, 64);
+  lds_wave_order();
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t key = s_list[i];
+    int rank = 0;
+    for (int k = 0; k < n; ++k) rank += s_list[k] > key;
+    if (rank >= top) continue;
+    const int idx = rank_index(key);
+    top_id[row * top + rank] = idx;
+    top_value[row * top + rank] = none ? NAN : ((float)x[idx] - s.m) - lz;
   }
 }
 
 hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
-  // slices: until about 1024 workgroups, four a CU, of at least 2048 logits
+  // slices: up to 1024 workgroups, four a CU, of at least 2048 logits
   int S = 1;
   if (a.ws && a.M < 512) {
-    S = (int)std::min<int64_t>({(1024 + a.M - 1) / a.M, a.V / 2048, (int64_t)kMaxSlices});
+    S = (int)std::min<int64_t>({1024 / a.M, a.V / 2048, (int64_t)kMaxSlices});
     const size_t per = (size_t)a.M * (sizeof(Sums) + 4 + (size_t)a.top * 8);
     S = (int)std::max<size_t>(1, std::min<size_t>((size_t)std::max(S, 1), a.ws_bytes / per));
   }
+  const int each = a.dtype == 0 ? 4 : 8;                      // logits of a vector
+  const int64_t vectors = (a.V / each + S - 1) / S, steps = (vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  const size_t lds = (size_t)std::max<int64_t>(1, std::min<int64_t>(steps, kGroups)) * kThreads * sizeof(float);
   uint64_t* keys = static_cast<uint64_t*>(a.ws);              // [M][S][top] keys, then [M][S] sums
   Sums* part = reinterpret_cast<Sums*>(keys + (size_t)a.M * S * a.top);
   auto go = [&](auto first, auto second, auto* p) {
-    hipError_t e = launch(first, dim3((unsigned)((int64_t)a.M * S)), dim3(kThreads), 0, st, p, a.stride, a.targets, a.logprob,
+    hipError_t e = launch(first, dim3((unsigned)((int64_t)a.M * S)), dim3(kThreads), lds, st, p, a.stride, a.targets, a.logprob,
                           a.entropy, a.top_value, a.top_id, a.V, a.top, S, part, keys);
     if (e != hipSuccess || S == 1) return e;
-    return launch(second, dim3((unsigned)a.M), dim3(64), 0, st, p, a.stride, a.targets, a.logprob, a.entropy, a.top_value,
+    return launch(second, dim3((unsigned)a.M), dim3(256), 0, st, p, a.stride, a.targets, a.logprob, a.entropy, a.top_value,
                   a.top_id, a.V, a.top, S, part, keys);
   };
   if (a.dtype == 0) return go(logprobs_kernel<float>, logprobs_join_kernel<float>, static_cast<const float*>(a.logits));
