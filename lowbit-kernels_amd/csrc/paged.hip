@@ -41,8 +41,10 @@ __device__ __forceinline__ void turn_cos_sin(int64_t p, float inv_f, float& c, f
 // A workgroup takes kTokens tokens: their cos and sin, one pair a thread, go to LDS while the first heads are loaded; then D /
 // 16 lanes a head, lane t the dims 8 t .. 8 t + 7 and their partners D / 2 + 8 t .. in two 16-byte pieces, so that the rotation
 // stays in a lane and the norm's sum takes three (D = 128) or two lane exchanges. y = x / sqrt(mean(x^2) + eps) * w and the
-// rotation in 32 bits, rounded once. Bound: memory (8192 tokens of 28 / 4 heads of 128 in fp16, 151 MB, XXX), one token's
-// launch. Four tokens a workgroup from kManyTokens on, else one: YYY.
+// rotation in 32 bits, rounded once. Bound: memory (8192 tokens of 28 / 4 heads of 128 in fp16, 151 MB, 28 us, 5.3 TB/s), of few
+// tokens the launch. Four tokens a workgroup, whose pairs keep all its threads busy, from kManyTokens on, else one (28 / 4
+// heads, us, one / four: 67 tokens 3.4 / 5.7, 512 4.3 / 6.2, 1024 6.6 / 7.0, 2048 10.4 / 10.1, 8192 31 / 28; 16 / 2 heads 1024
+// 5.4 / 4.9; 14 / 2 heads of 64 8192 20 / 12).
 constexpr int kHeadsAhead = 3;           // heads of a lane group in flight
 constexpr int kManyTokens = 1024;
 

@@ -221,6 +221,12 @@ def _need(t, name, dtype, shape, device):
         raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device}, got {got}")
 
 
+def _need_fast(t, name, dtype, shape, index, device):
+    """_need for calls whose host time counts: one pass over t's properties by GPU index, the message from _need."""
+    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        _need(t, name, dtype, shape, device)
+
+
 def _check_norm(norm, k, device):
     """The fused input norm's weight: fp16 [K], contiguous, on x's GPU."""
     import torch
@@ -689,11 +695,11 @@ class NativeExt:
 
     def _check_pages(self, k_cache, v_cache, like, hkv, dim):
         """Both caches [pages, hkv, page_size, dim] beside `like`; returns (pages, page_size)."""
-        shape = k_cache.shape
+        shape, dtype, index = k_cache.shape, like.dtype, like.get_device()
         if len(shape) != 4 or v_cache.shape != shape or shape[1] != hkv or shape[3] != dim:
             raise RuntimeError(f"the caches must be [pages, {hkv}, page_size, {dim}], got {list(shape)} and {list(v_cache.shape)}")
         for t in (k_cache, v_cache):
-            if t.dtype is not like.dtype or not t.is_contiguous() or t.get_device() != like.get_device():
+            if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != index:
                 raise RuntimeError(f"the caches must be contiguous {like.dtype} tensors on the same GPU")
         return shape[0], shape[2]
 
@@ -709,15 +715,15 @@ class NativeExt:
         if qkv.shape[1] != (hq + 2 * hkv) * dim or qkv.stride(1) != 1:
             raise RuntimeError(f"rows of qkv must hold (Hq + 2 Hkv) * D = {(hq + 2 * hkv) * dim} values side by side")
         device = qkv.device
-        _need(q_out, "q_out", qkv.dtype, (m, hq, dim), device)
+        _need_fast(q_out, "q_out", qkv.dtype, (m, hq, dim), index, device)
         if (q_weight is None) != (k_weight is None):
             raise RuntimeError("q_weight goes with k_weight")
         if q_weight is not None:
-            _need(q_weight, "q_weight", qkv.dtype, (dim,), device)
-            _need(k_weight, "k_weight", qkv.dtype, (dim,), device)
-        _need(positions, "positions", torch.int64, (m,), device)
-        _need(slots, "slots", torch.int64, (m,), device)
-        _need(inv_freq, "inv_freq", torch.float32, (dim // 2,), device)
+            _need_fast(q_weight, "q_weight", qkv.dtype, (dim,), index, device)
+            _need_fast(k_weight, "k_weight", qkv.dtype, (dim,), index, device)
+        _need_fast(positions, "positions", torch.int64, (m,), index, device)
+        _need_fast(slots, "slots", torch.int64, (m,), index, device)
+        _need_fast(inv_freq, "inv_freq", torch.float32, (dim // 2,), index, device)
         pages, page_size = self._check_pages(k_cache, v_cache, qkv, hkv, dim)
         if m == 0:
             return
@@ -740,11 +746,11 @@ class NativeExt:
         batch, width = page_table.shape
         hkv = k_cache.shape[1]
         device = q.device
-        _need(q, "q", q.dtype, (t, hq, dim), device)
-        _need(out, "out", q.dtype, (t, hq, dim), device)
-        _need(page_table, "page_table", torch.int32, (batch, width), device)
-        _need(q_starts, "q_starts", torch.int32, (batch + 1,), device)
-        _need(kv_lens, "kv_lens", torch.int32, (batch,), device)
+        _need_fast(q, "q", q.dtype, (t, hq, dim), index, device)
+        _need_fast(out, "out", q.dtype, (t, hq, dim), index, device)
+        _need_fast(page_table, "page_table", torch.int32, (batch, width), index, device)
+        _need_fast(q_starts, "q_starts", torch.int32, (batch + 1,), index, device)
+        _need_fast(kv_lens, "kv_lens", torch.int32, (batch,), index, device)
         pages, page_size = self._check_pages(k_cache, v_cache, q, hkv, dim)
         if t == 0 or batch == 0:
             return
@@ -763,31 +769,32 @@ class NativeExt:
         """Of logits [M, V] (float32, float16 or bfloat16; rows may lie apart): (log probability of targets [M] (int64;
         negative: 0), entropy, log probabilities and ids of the `top` <= 32 most likely tokens): float32 [M], float32 [M],
         float32 [M, top], int64 [M, top]. Equal logits rank by index."""
-        dtypes = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-        if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in dtypes:
+        dtype = DTYPE_F32 if logits.dtype is torch.float32 else DTYPE_F16 if logits.dtype is torch.float16 else DTYPE_BF16
+        if not logits.is_cuda or logits.dim() != 2 or (dtype == DTYPE_BF16 and logits.dtype is not torch.bfloat16):
             raise RuntimeError("logits must be a 2-D float32, float16 or bfloat16 CUDA tensor [M, V]")
         m, v = logits.shape
         if v > 1 and logits.stride(1) != 1:
             raise RuntimeError("a row of logits must lie side by side")
         index, device = logits.get_device(), logits.device
-        _need(targets, "targets", torch.int64, (m,), device)
+        _need_fast(targets, "targets", torch.int64, (m,), index, device)
         if top < 0 or top > min(v, 32):
             raise RuntimeError(f"top must be 0..32 and at most V = {v}, got {top}")
-        sums = torch.empty((2, m), dtype=torch.float32, device=device)
+        logprob = torch.empty(m, dtype=torch.float32, device=device)
+        entropy = torch.empty(m, dtype=torch.float32, device=device)
         values = torch.empty((m, top), dtype=torch.float32, device=device)
         ids = torch.empty((m, top), dtype=torch.int64, device=device)
         if m == 0:
-            return sums[0], sums[1], values, ids
+            return logprob, entropy, values, ids
         if v == 0:
             raise RuntimeError("token_logprobs needs at least one logit a row")
         # few rows are cut into slices, whose sums and alternatives lie here for this call alone
         nbytes = (1024 + m) * (16 + 8 * top) if m < 512 and v >= 4096 else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_token_logprobs(
-            logits.data_ptr(), dtypes[logits.dtype], logits.stride(0) if m > 1 else v, targets.data_ptr(), sums.data_ptr(),
-            sums.data_ptr() + 4 * m, values.data_ptr(), ids.data_ptr(), m, v, int(top), ws.data_ptr() if nbytes else None,
+            logits.data_ptr(), dtype, logits.stride(0) if m > 1 else v, targets.data_ptr(), logprob.data_ptr(),
+            entropy.data_ptr(), values.data_ptr(), ids.data_ptr(), m, v, int(top), ws.data_ptr() if nbytes else None,
             nbytes, stream))
-        return sums[0], sums[1], values, ids
+        return logprob, entropy, values, ids
 
     # ---- bandwidth probes (lowbit_hbm_read, lowbit_hbm_copy) ----
     def hbm_read(self, buf, sink, blocks):

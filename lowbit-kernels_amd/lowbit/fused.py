@@ -283,6 +283,49 @@ class FusedQwen2:
 
     __call__ = forward
 
+    @torch.inference_mode()
+    def score(self, tokens, top=0):
+        """The log probability of each of tokens [M] (int64, M >= 2) after the first, given the ones before it: (log
+        probabilities [M - 1], entropies of the distributions [M - 1], and the `top` <= 32 likeliest tokens' log
+        probabilities and ids [M - 1, top]), float32 and int64, from one forward (cache rows 0 .. M - 1 are written)."""
+        logits = self.forward(tokens, torch.arange(tokens.shape[0], device=tokens.device))
+        return ops.ext().token_logprobs(logits[:-1], tokens[1:].contiguous(), top)
+
+    def paged_caches(self, pages, page_size=64):
+        """(k, v) [layers, pages, Hkv, page_size, head_dim] for forward_paged, whose pages the caller hands out."""
+        k = torch.zeros(len(self.layers), pages, self.hkv, page_size, self.head_dim, dtype=torch.float16,
+                        device=self.embed.device)
+        return k, torch.zeros_like(k)
+
+    @torch.inference_mode()
+    def forward_paged(self, tokens, positions, slots, page_table, q_starts, kv_lens, caches, max_new, max_keys, rows=None):
+        """One step of a batch of sequences over paged caches: tokens, positions and slots (int64 [T]) hold the sequences' new
+        tokens one after another (prompts or pieces of them, decode tokens, drafts), sequence b's in q_starts[b] ..
+        q_starts[b + 1] (int32 [B + 1]); its keys, the new tokens' included, are the first kv_lens[b] (int32 [B]) in the pages
+        page_table[b] (int32 [B, width]), and token t's k and v go to slot slots[t] = page * page_size + row (negative: a
+        padded token's, nowhere). max_new, max_keys: bounds on a sequence's new tokens and keys. Returns the logits of `rows`
+        (int64, indices into the T tokens; None: of all)."""
+        ext = ops.ext()
+        t = tokens.shape[0]
+        h = self._embedding(tokens)
+        xn = torch.empty_like(h)
+        q = torch.empty(t, self.hq, self.head_dim, dtype=torch.float16, device=h.device)
+        attn = torch.zeros_like(q)                          # (rows of no sequence are left alone: zeros)
+        for i, lay in enumerate(self.layers):
+            k_cache, v_cache = caches[0][i], caches[1][i]
+            qkv = lay["qkv"](h, EPI_BIAS, lay["qkv"].bias, norm=(lay["in_norm"], self.eps))
+            ext.norm_rope_paged(qkv, None, None, self.eps, positions, self.inv_freq, slots, q, k_cache, v_cache, self.hq,
+                                self.hkv, permuted=self.quant in ("int4", "fp16_gemv"))
+            ext.attention_paged(q, k_cache, v_cache, page_table, q_starts, kv_lens, attn, max_new, max_keys, self.scale)
+            lay["o"](attn.view(t, -1), EPI_RESIDUAL, h, out=h)
+            act = lay["gu"](h, EPI_SILU_MUL, norm=(lay["post_norm"], self.eps))
+            lay["down"](act, EPI_RESIDUAL, h, out=h)
+        if rows is not None:
+            h = h[rows]
+            xn = torch.empty_like(h)
+        ext.rmsnorm(h, self.final_norm, self.eps, out=xn)
+        return self.logits(xn)
+
 
 class FusedDecoder:
     """GraphDecoder's interface (prefill / capture / step / greedy) over a FusedQwen2."""
