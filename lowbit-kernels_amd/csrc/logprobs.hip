@@ -1,9 +1,10 @@
 // Log probabilities of given tokens with the entropy and the most likely alternatives of each row of logits.
 //
-// A row is read once from memory. Every lane keeps, against a reference r that follows its largest logit only when one passes
-// it by more than kLag, z = sum exp(x - r) and e = sum exp(x - r) (x - r); when all is read, the sums are moved to the row's
-// maximum m: log p(t) = (x_t - m) - log z, H = log z - e / z. Differences from a logit, not products with log2(e), are what
-// is rounded, so rows far from zero (or at the type's lowest value throughout) lose nothing.
+// A row is read once from memory. Every lane keeps, against its largest logit so far r, z = sum exp(x - r) and e = sum exp(x -
+// r) (x - r); when all is read, the sums are moved to the row's maximum m: log p(t) = (x_t - m) - log z, H = log z - e / z.
+// Every term of e, and what a move to a larger reference adds, is 0 or below, so nothing cancels (a reference that lags 16
+// behind the maximum saves instructions and cost entropies up to 4e-5). Differences from a logit, not products with log2(e),
+// are what is rounded, so rows far from zero (or at the type's lowest value throughout) lose nothing.
 // The alternatives: the `top`-th largest of the lanes' maxima is a bound that `top` logits at least reach, and almost no other
 // does; the maxima of the groups of vectors that each lane has read (kept in LDS) say which groups hold such logits, and only
 // those are read again (from L2). What reaches the bound is ranked by counting.
@@ -24,7 +25,6 @@ constexpr int kUnroll = 4;               // 16-byte vectors of a lane in flight
 constexpr int kGroups = 16;              // groups of vectors a lane keeps the maxima of
 constexpr int kList = 1024;              // logits that may reach the bound on the fast path
 constexpr int kMaxSlices = 64;
-constexpr float kLag = 16.f;             // exp(16) more than the reference's weight of 1 is far from fp32's end
 
 // (value, index) as one number, larger = earlier among the alternatives: the larger value (-0 equal to +0, a NaN above
 // every number, as torch orders them), then the smaller index. Zero is below every key.
@@ -95,7 +95,7 @@ __device__ __forceinline__ void store_sums(const T* x, int V, int64_t t, const S
 }
 
 // Workgroup (row, slice): see the top of the file. part (S > 1): [row][slice] Sums, then keys [row][slice][top].
-// Bound: memory, 2047 rows of 151665 in fp16 (621 MB) 123 us, 5.0 TB/s; of few rows the chain of load, sums, bound, reread and
+// Bound: memory, 2047 rows of 151665 in fp16 (621 MB) 126 us, 4.9 TB/s; of few rows the chain of load, sums, bound, reread and
 // join: 48 rows of 151936 in fp32 18 us, one in fp16 13.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ logits, int64_t stride,
@@ -126,13 +126,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   const int steps = (v1 - v0 + kThreads * kUnroll - 1) / (kThreads * kUnroll), every = (steps + kGroups - 1) / kGroups;
   const int single = slice == 0 && tid < head ? tid : slice == S - 1 && tail0 + (int)tid - 16 < V && tid >= 16 ? tail0 + tid - 16 : -1;
 
-  float r = -INFINITY, z = 0.f, e = 0.f, mx = -INFINITY;
-  auto raise = [&](float vm) {                                // the lane's reference, where a logit passes it
-    if (__any(vm > r + kLag)) {
-      if (vm > r) {
-        move_sums(r, vm, z, e);
-        r = vm;
-      }
+  float r = -INFINITY, z = 0.f, e = 0.f;
+  auto raise = [&](float v) {                                 // the lane's reference, to v where that is larger
+    if (v > r) {
+      move_sums(r, v, z, e);
+      r = v;
     }
   };
   auto add = [&](float v, float ref) {                        // (p d with d held above -inf: 0 log 0 = 0)
@@ -168,25 +166,20 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       }
     gm = step % every == 0 ? sm : fmaxf(gm, sm);
     s_max[step / every * kThreads + tid] = gm;
-    mx = fmaxf(mx, sm);
   }
   if (single >= 0) {
     const float v = (float)x[single];
-    if (v > r) {
-      move_sums(r, v, z, e);
-      r = v;
-    }
+    raise(v);
     add(v, r == -INFINITY ? 0.f : r);
-    mx = fmaxf(mx, v);
   }
   // the wave's sums against its maximum, then the workgroup's, added by every thread in order of the waves
   Sums s;
-  s.m = wave_max(mx);
+  s.m = wave_max(r);
   move_sums(r, s.m, z, e);
   s.z = wave_sum(z);
   s.e = wave_sum(e);
   if (lane == 0) s_sums[tid >> 6] = s;
-  s_lane[tid] = mx;
+  s_lane[tid] = r;
   if (tid == 0) s_count = 0;
   __syncthreads();
   s = s_sums[0];
