@@ -319,7 +319,7 @@ int lowbit_f16_gemv_pick(const void* x, const void* w, void* y, int64_t N, int64
  * rotate-half position rotation of the pairs (i, i + D / 2) by positions[m] * inv_freq[i] (the angle in 64 bits), all in 32
  * bits and rounded once; q -> q_out [M][Hq][D], k and the v heads as they are -> the caches' slot slots[m]. A slot outside
  * the cache (a padded row's, e.g. -1) leaves the caches as they are; of several rows with one slot any one's values may
- * stay in any of its heads. permuted != 0: each head's D values lie in the RoPE-permuted order of lowbit_rope_kv (16-row
+ * stay in any of its heads (the callers' tokens have slots of their own). M * (Hq + 2 Hkv) at most 2^25. permuted != 0: each head's D values lie in the RoPE-permuted order of lowbit_rope_kv (16-row
  * tiles: dims 8 t .. 8 t + 7, then D / 2 + 8 t ..). Outputs must not overlap inputs. */
 int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const void* q_weight, const void* k_weight,
                            float eps, const int64_t* positions, const float* inv_freq, const int64_t* slots,
@@ -335,14 +335,15 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
  * them may hold anything. max_new and max_keys: bounds on a sequence's new tokens and keys that size the launch (a captured
  * graph keeps them); results do not depend on them beyond the order of sums. workspace (optional, 16-byte aligned, no
  * initial contents): lets few rows split their keys over the GPU; calls that overlap must
- * not share one. The same bits on every call for given lengths and bounds. */
+ * not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22, table_width *
+ * page_size 2^30. */
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
                            int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
                            void* stream);
 
-/* For M rows of logits [V] (float32, float16 or bfloat16; row m at logits + m * row_stride values, any alignment of the
+/* For M <= 2^22 rows of logits [V] (float32, float16 or bfloat16; row m at logits + m * row_stride values, any alignment of the
  * type): logprob[m] = log_softmax(logits[m])[targets[m]] (0 where the target is negative: none asked; NaN where it is V or
  * more), entropy[m] = - sum p log p (0 log 0 = 0), and the `top` <= 32 largest logits of the row in falling order, equal
  * ones by index (-0 equal to +0, a NaN above every number): top_ids [M][top] and their log probabilities top_values

@@ -708,8 +708,8 @@ int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, con
   if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_values || !top_ids)))
     return fail(LOWBIT_ERR_ARG, "null pointer argument");
   if (dtype < LOWBIT_DTYPE_F32 || dtype > LOWBIT_DTYPE_BF16) return fail(LOWBIT_ERR_ARG, "token_logprobs: dtype is F32, F16 or BF16");
-  if (M < 1 || V < 1 || !fits_int(M) || !fits_int(V + 65536) || row_stride < 0 || row_stride > ((int64_t)1 << 40))
-    return fail(LOWBIT_ERR_SHAPE, "token_logprobs: M and V must be positive, the row stride not negative");
+  if (M < 1 || V < 1 || M > (1 << 22) || !fits_int(V) || !fits_int(V + 65536) || row_stride < 0 || row_stride > ((int64_t)1 << 40))
+    return fail(LOWBIT_ERR_SHAPE, "token_logprobs: M and V must be positive, M at most 2^22, the row stride not negative");
   if (top < 0 || top > kMaxTop || top > V) return fail(LOWBIT_ERR_SHAPE, "token_logprobs: top must be 0..%d and at most V", kMaxTop);
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LOWBIT_DTYPE_F32 ? 3 : 1)) ||
       ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(top_ids)) & 7) ||

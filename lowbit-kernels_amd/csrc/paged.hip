@@ -244,7 +244,8 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
         u.pid = rest % (kRows / kMerge);
       }
       u.rec = p.cap == 1 ? 0 : recs + pick(recs_upto - split) + (u.tile * p.Hkv + u.hk) * u.parts + (kMerge == 0 ? u.pid : 0);
-      return true;
+      // (starts that fall, which the caller rules out, could number more work than 32 bits hold: never past the buffers)
+      return at >= 0 && (uint32_t)u.tile < (uint32_t)u.tiles && (p.cap == 1 || (uint32_t)u.rec < (uint32_t)p.most);
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     if (p.cap > 1) recs += __builtin_amdgcn_readlane(recs_upto, 63);

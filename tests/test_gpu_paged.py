@@ -240,6 +240,70 @@ def test_attention_paged(cuda, hq, hkv, d, dt):
         check_attend(x, lens, d ** -0.5, max_new=1 << 40, max_keys=1 << 40)
 
 
+def widened(x, keys):
+    """The batch with a table of room for `keys` keys (its own pages first), so that bounds are not held to its length."""
+    page = x[1].shape[2]
+    table = torch.full((x[3].shape[0], -(-keys // page)), -1, dtype=torch.int32, device="cuda")
+    table[:, :x[3].shape[1]] = x[3][:, :table.shape[1]]
+    return x[:3] + (table,) + x[4:]
+
+
+# the bounds choose the tile (at most 32 rows and few keys: one wave where the batch is large, else four; 64 rows and 1024 keys;
+# 128 rows) and whether keys are split: every batch under every choice
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (8, 8, 64), (9, 1, 128)])
+def test_attention_paged_under_every_bound(cuda, hq, hkv, d, dt):
+    for i, lens in enumerate(([(1, 700), (2, 3), (0, 9), (1, 1)], [(70, 700), (1, 513), (5, 1300)], [(333, 333), (1, 2100)])):
+        x = widened(batch(lens, hq, hkv, d, (16, 64, 32)[i], dt, 7 * i + hq), 1 << 16)
+        for max_new, max_keys in ((1, 100), (1, 512), (1, 60000), (64, 300), (64, 1024), (64, 60000), (500, 60000)):
+            print(lens, max_new, max_keys, flush=True)
+            check_attend(x, lens, d ** -0.5, max_new, max_keys)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,n", [(28, 4, 128, 130), (16, 8, 64, 200), (4, 4, 128, 333)])
+def test_attention_paged_of_many_sequences(cuda, hq, hkv, d, n, dt):
+    """More sequences than a wave has lanes, among them some without new tokens and some without keys; short keys, then a few
+    long ones among them, which are split while the others are not."""
+    short = [(0 if i % 17 == 5 else 1 + (i % 23 == 3), 0 if i % 29 == 7 else 1 + (i * 37) % 300) for i in range(n)]
+    short = [(a, max(a, b) if b else 0) for a, b in short]
+    check_attend(batch(short, hq, hkv, d, 16, dt, n), short, d ** -0.5)
+    long = list(short)
+    for i, keys in ((2, 9000), (70, 5000), (n - 1, 20011)):
+        long[i] = (1, keys)
+    x = batch(long, hq, hkv, d, 32, dt, n + 1)
+    one = check_attend(x, long, d ** -0.5)
+    assert torch.equal(one, check_attend(x, long, d ** -0.5))
+    long[n // 2] = (150, 4000)                               # and a piece of a prompt
+    check_attend(batch(long, hq, hkv, d, 64, dt, n + 2), long, d ** -0.5)
+
+
+def test_attention_paged_of_shared_pages(cuda):
+    """Two sequences that begin with the same pages (a shared prefix), and one page twice in a sequence."""
+    lens = [(3, 200), (1, 150), (40, 300)]
+    x = list(batch(lens, 16, 2, 128, 16, torch.float16, 3))
+    x[3][1, :8] = x[3][0, :8]
+    x[3][2, 5] = x[3][2, 2]
+    k1, v1 = x[6][1]
+    k1[:128], v1[:128] = x[6][0][0][:128], x[6][0][1][:128]
+    k2, v2 = x[6][2]
+    k2[80:96], v2[80:96] = k2[32:48].clone(), v2[32:48].clone()
+    check_attend(x, lens, 128 ** -0.5)
+
+
+def test_attention_paged_with_starts_that_do_not_hold(cuda):
+    """Starts past q's rows or below zero are held to them, and nothing outside out is written."""
+    lens = [(4, 50), (3, 40)]
+    x = list(batch(lens, 16, 2, 128, 16, torch.float16, 3))
+    room = torch.full((7 + 8, 16, 128), 777.0, dtype=torch.float16, device="cuda")
+    for starts in ([-5, 4, 1000], [0, 4, 7], [7, 7, 7], [900, 900, 900], [-3, -2, -1]):
+        x[4] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        room.fill_(777.0)
+        ops.ext().attention_paged(*x[:6], room[4:11], 4, 50, 0.1)
+        torch.cuda.synchronize()
+        assert bool((room[:4] == 777.0).all()) and bool((room[11:] == 777.0).all())
+
+
 def test_attention_paged_rows_without_keys_and_of_no_sequence(cuda):
     """New tokens before a sequence's first key get zeros; rows in front of, between and behind the sequences stay."""
     for dt, lens in ((torch.float16, [(4, 0), (6, 2), (1, 0), (70, 3), (2, 9)]), (torch.bfloat16, [(1, 0)]),

@@ -64,6 +64,7 @@ PAGED = [(dict(dtype=F32), 1, "F16 or BF16"), (dict(dtype=7), 1, "F16 or BF16"),
     (logprobs, dict(ent=None), 1, "null"), (logprobs, dict(tv=None), 1, "null"), (logprobs, dict(ti=None), 1, "null"),
     (logprobs, dict(dtype=3), 1, "dtype"), (logprobs, dict(m=0), 3, "M and V"), (logprobs, dict(v=0), 3, "M and V"),
     (logprobs, dict(v=(1 << 31) - 5), 3, "M and V"), (logprobs, dict(stride=-1), 3, "stride"),
+    (logprobs, dict(m=(1 << 22) + 1), 3, "2^22"), (attend, dict(b=1 << 22), 3, "2^22"), (norm_rope, dict(m=1 << 21), 3, "2^25"),
     (logprobs, dict(top=33), 3, "top must"), (logprobs, dict(top=-1), 3, "top must"), (logprobs, dict(v=2), 3, "top must"),
     (logprobs, dict(x=ctypes.c_void_p(4097)), 4, "naturally"), (logprobs, dict(x=ODD2, dtype=F32), 4, "naturally"),
     (logprobs, dict(t=ODD4), 4, "naturally"), (logprobs, dict(ti=ODD4), 4, "naturally"), (logprobs, dict(tv=ODD2), 4, "naturally"),
