@@ -745,6 +745,7 @@ hipError_t pick_norm_rope(const NormRopeArgs& a, hipStream_t st) {
 
 constexpr int kPagedParts = 256;                             // of a tile at most
 constexpr int kPagedLeast = 256;                             // keys of a part at least
+constexpr int kPagedWhole = 768;                             // keys up to which decode tiles are not split
 
 template <typename T, int D, int RG, int KG>
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
@@ -755,7 +756,12 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   const int64_t seqs = std::min(a.batch.B, a.batch.T);        // with new tokens
   const int64_t units = (((int64_t)a.batch.T * G + kRows - 1) / kRows + seqs) * a.Hkv;
   p.most = (int)std::min<size_t>(4 * (size_t)p.slots, a.ws_bytes / ((size_t)kRows * paged_rec<D>() * sizeof(float)));
-  if (a.ws && p.most >= 2)
+  // no split, and no launch of the merge, where it does not pay: decode tiles of few keys, other tiles of not many that fill
+  // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.7 / 11.9, one launch less for
+  // the host; 40 on 800 18.8, on 760 whole 15.3; a prompt of 500 29.5 / 16.3; six prompts of 171 .. 794, 14 / 2 heads of 64,
+  // 23.6 / 20.3)
+  const bool whole = RG == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * units >= p.slots;
+  if (a.ws && p.most >= 2 && !whole)
     p.cap = std::min(kPagedParts, (int)((((int64_t)a.max_keys + kBlock - 1) / kBlock + p.least - 1) / p.least));
   const int64_t grid = p.cap == 1 ? units : std::min<int64_t>(units * p.cap, units + p.most / 2 + 1);
   if (lds > 65536) {

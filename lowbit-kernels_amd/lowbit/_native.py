@@ -163,7 +163,8 @@ WORKSPACE_COUNTER_BYTES = 16384
 WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (16 << 20)     # LOWBIT_WORKSPACE_BYTES
 PREFILL_WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (64 << 20)
 ATTENTION_WORKSPACE_BYTES = 4 << 20
-PAGED_SPLIT_KEYS = 256                  # attention_paged cuts longer sequences into parts of at least as many keys
+PAGED_SPLIT_KEYS = 256                  # attention_paged cuts longer sequences into parts of at least as many keys,
+PAGED_WHOLE_KEYS = 768                  # those of at most 32 query rows a KV head from more keys on
 PICK_WORKSPACE_BYTES = 1 << 20          # the greedy pick's keys: 8 bytes per 8 head rows
 _WORKSPACES = {}
 _CAPTURE_STREAMS = {}
@@ -757,7 +758,7 @@ class NativeExt:
         # the split tiles' records, from the caching allocator for this call alone: calls on several streams and captured
         # graphs share none (LOWBIT_PAGED_WORKSPACE_BYTES(rows, D))
         nbytes = 0
-        if split and max_keys > PAGED_SPLIT_KEYS:
+        if split and max_keys > (PAGED_WHOLE_KEYS if max_new * hq <= 32 * hkv else PAGED_SPLIT_KEYS):
             nbytes = (1024 * 32 if max_new * hq <= 32 * hkv else 2048 * 128) * (dim + 4) * 4
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged(
