@@ -331,12 +331,12 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
  * 0 .. kv_lens[b] - 1, the last of them the new tokens' own, key j in row j % page_size of page page_table[b][j / page_size]
  * (page_table [B][table_width]; keys past the table are not attended, a page outside 0 .. pages - 1 reads as zeros). New
  * token i attends the keys up to kv_lens[b] - new + i; one that is left none (kv_lens[b] < new) gets zeros. Scores scaled by
- * `scale`; softmax, its sums and the output's sums in 32 bits. Keys up to kv_lens[b] - 1 must hold finite values; rows past
- * them may hold anything. max_new and max_keys: bounds on a sequence's new tokens and keys that size the launch (a captured
- * graph keeps them); results do not depend on them beyond the order of sums. workspace (optional, 16-byte aligned, no
- * initial contents): lets few rows split their keys over the GPU; calls that overlap must
- * not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22, table_width *
- * page_size 2^30. */
+ * `scale`; softmax, its sums and the output's sums in 32 bits. Rows past a sequence's keys may hold anything, and an
+ * infinity or a NaN in a key's k or v reaches only the rows that attend the key. max_new and max_keys: bounds on a sequence's
+ * new tokens and keys that size the launch (a captured graph keeps them); results do not depend on them beyond the order of
+ * sums. workspace (optional, 16-byte aligned, no initial contents): lets few rows split their keys over the GPU; calls that
+ * overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22,
+ * table_width * page_size 2^30. */
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,

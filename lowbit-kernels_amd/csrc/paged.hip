@@ -271,6 +271,8 @@ struct Mfma<f16> {
   static __device__ __forceinline__ float sum2(uint32_t p, float c) {   // c + the two values
     return dot2(as_f16x2(p), f16x2{(f16)1.f, (f16)1.f}, c);
   }
+  static constexpr uint32_t kExponent = 0x7C00u;              // all ones: an infinity or a NaN
+  static __device__ __forceinline__ float half_of(uint32_t w, int i) { return (float)as_f16x2(w)[i]; }
 };
 template <>
 struct Mfma<bf16> {
@@ -285,7 +287,18 @@ struct Mfma<bf16> {
   static __device__ __forceinline__ float sum2(uint32_t p, float c) {
     return c + (__builtin_bit_cast(float, p << 16) + __builtin_bit_cast(float, p & 0xFFFF0000u));
   }
+  static constexpr uint32_t kExponent = 0x7F80u;
+  static __device__ __forceinline__ float half_of(uint32_t w, int i) {
+    return __builtin_bit_cast(float, i ? w & 0xFFFF0000u : w << 16);
+  }
 };
+
+// a pair's finite values, zeros for the others
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t e = Mfma<T>::kExponent;
+  return ((w & e) == e ? 0u : w & 0xFFFFu) | ((w & (e << 16)) == e << 16 ? 0u : w & 0xFFFF0000u);
+}
 
 // four values of a row's output; a row without a key gets zeros
 template <typename T>
@@ -326,9 +339,9 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // transposing read do (no conflict is counted). K is requested paged_ahead + 1 blocks before its scores' weights, V
 // paged_ahead, and a block's scores are multiplied while the vector unit evaluates the block before. With one row group a
 // wave loads the keys it takes itself and no barrier is needed.
-// Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 125 us, 5.0
-// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 69 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 500 us, 0.91
-// PFLOP/s, on zeros 407 us at full clock (1.13), where the vector unit and the matrix cores are busy 50% and 44%. There,
+// Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 132 us, 4.7
+// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 69 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 521 us, 0.88
+// PFLOP/s (500 and on zeros 407 us, at full clock 1.13, before odd values were kept to their rows), where the vector unit and the matrix cores are busy 50% and 44%. There,
 // measured and not kept: 64 rows a wave with one wave per SIMD (half the LDS reads) 703 us; eight waves in two turns, one four
 // on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three waves per SIMD (168 registers,
 // spilled) 546; two blocks ahead instead of three 519 .. 536.
@@ -503,6 +516,37 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
     }
+    // Where a row leaves out a key that exists, its weight 0 may meet an infinity or a NaN of that key's V: those are taken out
+    // of the product, and the rows that do attend the key add them themselves (uniform; rare; without this the blocks on the
+    // diagonal would carry a token's NaN to tokens before it. It costs 4% of a prompt of 8000 tokens, 5% of a mixed step)
+    bool odd = false;
+    if (wmin < min(kb + 31, kend - 1)) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u32x4 second = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          odd |= finite2<T>(va[0][dt][e]) != va[0][dt][e] || finite2<T>(second[e]) != second[e];
+      }
+      odd = __any(odd);
+      if (odd) {
+        const int last = min(pr, kend - 1) - kb;
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key)
+          if (key <= last) {
+            const uint32_t at = vat + kV + (32 * kgrp + key) * RB + 8 * h;
+#pragma unroll
+            for (int v = 0; v < D / 8; ++v) {
+              const uint2 p = *reinterpret_cast<const uint2*>(smem + at + 16 * (v ^ vswz(key)));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t w = i < 2 ? p.x : p.y;
+                if (((w >> (16 * (i & 1))) & Mfma<T>::kExponent) == Mfma<T>::kExponent) o[v >> 2][4 * (v & 3) + i] += Mfma<T>::half_of(w, i & 1);
+              }
+            }
+          }
+      }
+    }
     const float sub = ref == -INFINITY ? 0.f : ref - (15.f - kLag);
     const f32x16 sc = st;
     st = zero;
@@ -521,6 +565,12 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       if (s == 0) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) va[1][dt] = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
+      }
+      if (odd) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) va[s][dt][e] = finite2<T>(va[s][dt][e]);
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] = Mfma<T>::go(va[s][dt], ph, o[dt]);

@@ -470,6 +470,34 @@ def test_paged_calls_on_two_streams_and_two_graphs_at_once(cuda):
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (14, 2, 64)])
+def test_attention_paged_of_keys_that_are_not_finite(cuda, hq, hkv, d, dt):
+    """An infinity or a NaN in a token's k or v reaches the rows that attend it and no other: those before it have the bits
+    that they have without it, in tiles of every kind, split and not."""
+    for lens, at in (([(5, 300)], 297), ([(60, 60)], 31), ([(300, 300), (1, 40)], 150), ([(200, 1500)], 1400), ([(9, 2000)], 1995)):
+        for which, bad in ((1, float("nan")), (2, float("nan")), (2, float("inf")), (2, -float("inf"))):
+            x = list(batch(lens, hq, hkv, d, 16, dt, at))
+            clean = torch.empty_like(x[0])
+            new, keys = lens[0]
+            args = (max(n for n, _ in lens), max(k for _, k in lens), d ** -0.5)
+            ops.ext().attention_paged(*x[:6], clean, *args)
+            x[which][x[3][0, at // 16], 0, at % 16, 5] = bad   # of the first KV head
+            out = torch.empty_like(clean)
+            ops.ext().attention_paged(*x[:6], out, *args)
+            first, g = at - (keys - new), hq // hkv          # the first row that attends it
+            hit = out[first:new, :g, 5] if which == 2 else out[first:new, :g]
+            if bad != bad:
+                assert bool(hit.isnan().all()), (lens, which)
+            else:
+                assert bool((hit == bad).all()), (lens, which, bad)
+            if which == 2:
+                out[first:new, :g, 5] = clean[first:new, :g, 5]
+            else:
+                out[first:new, :g] = clean[first:new, :g]
+            assert torch.equal(out, clean), (lens, which, bad)
+
+
 # ---- refusals ----
 
 def test_paged_refusals_of_tensors(cuda):
