@@ -159,7 +159,7 @@ struct PagedPlan {
   FastDiv by_hkv, by_g;
 };
 struct PagedUnit {
-  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec;   // first: the sequence's first row of q; rec: the part's records
+  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec;   // first: the sequence's first row of q; rec: the part's record (parts > 1)
 };
 
 // sum of the lanes up to and including this one
@@ -244,8 +244,10 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
         u.pid = rest % (kRows / kMerge);
       }
       u.rec = p.cap == 1 ? 0 : recs + pick(recs_upto - split) + (u.tile * p.Hkv + u.hk) * u.parts + (kMerge == 0 ? u.pid : 0);
-      // (starts that fall, which the caller rules out, could number more work than 32 bits hold: never past the buffers)
-      return at >= 0 && (uint32_t)u.tile < (uint32_t)u.tiles && (p.cap == 1 || (uint32_t)u.rec < (uint32_t)p.most);
+      // (starts that fall, which the caller rules out, could number more work than 32 bits hold: never past the buffers. A
+      // tile of one part has no record, whatever its number)
+      return at >= 0 && (uint32_t)u.tile < (uint32_t)u.tiles &&
+             (u.parts == 1 || (u.rec >= 0 && u.rec <= p.most - (kMerge == 0 ? 1 : u.parts)));
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     if (p.cap > 1) recs += __builtin_amdgcn_readlane(recs_upto, 63);
