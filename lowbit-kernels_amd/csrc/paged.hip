@@ -522,7 +522,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     // of the product, and the rows that do attend the key add them themselves (uniform; rare; without this the blocks on the
     // diagonal would carry a token's NaN to tokens before it. It costs 4% of a prompt of 8000 tokens, 5% of a mixed step)
     bool odd = false;
-    if (wmin < min(kb + 31, kend - 1)) {
+    if (wmin < min(kb + 31, len - 1)) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4 second = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
