@@ -295,11 +295,17 @@ struct Mfma<bf16> {
   }
 };
 
+// the sign bits of a pair's values that are infinities or NaN (the exponent's ones carry into them, none past them)
+template <typename T>
+__device__ __forceinline__ uint32_t odd2(uint32_t w) {
+  constexpr uint32_t one = Mfma<T>::kExponent & -Mfma<T>::kExponent;   // the exponent's last bit
+  return ((w & 0x7FFF7FFFu) + (one | one << 16)) & 0x80008000u;
+}
 // a pair's finite values, zeros for the others
 template <typename T>
 __device__ __forceinline__ uint32_t finite2(uint32_t w) {
-  constexpr uint32_t e = Mfma<T>::kExponent;
-  return ((w & e) == e ? 0u : w & 0xFFFFu) | ((w & (e << 16)) == e << 16 ? 0u : w & 0xFFFF0000u);
+  const uint32_t m = odd2<T>(w);
+  return w & ~(m | (m - (m >> 15)));
 }
 
 // four values of a row's output; a row without a key gets zeros
@@ -341,9 +347,9 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // transposing read do (no conflict is counted). K is requested paged_ahead + 1 blocks before its scores' weights, V
 // paged_ahead, and a block's scores are multiplied while the vector unit evaluates the block before. With one row group a
 // wave loads the keys it takes itself and no barrier is needed.
-// Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 132 us, 4.7
-// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 69 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 521 us, 0.88
-// PFLOP/s (500 and on zeros 407 us, at full clock 1.13, before odd values were kept to their rows), where the vector unit and the matrix cores are busy 50% and 44%. There,
+// Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 130 us, 4.8
+// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 70 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 514 us in fp16,
+// 0.90 PFLOP/s, 501 in bf16; the vector unit and the matrix cores are busy 50% and 44%. There,
 // measured and not kept: 64 rows a wave with one wave per SIMD (half the LDS reads) 703 us; eight waves in two turns, one four
 // on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three waves per SIMD (168 registers,
 // spilled) 546; two blocks ahead instead of three 519 .. 536.
@@ -491,6 +497,10 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = zero;
   auto k_frag = [&](uint32_t at, int s) { return *reinterpret_cast<const u32x4*>(smem + at + (kr ^ (32 * s))); };
+  // some row leaves out a key of the 32 from kb on that is there (keys past the tile's last row may be, up to the sequence's
+  // last)
+  auto guarded = [&](int kb) { return wmin < min(kb + 31, len - 1); };
+  bool some_odd = false;
   // One block: the weights of its scores, the weights times V and the next block's scores. Every fragment is read well before
   // its product (K's and V's first half at the start, V's other half while K's are multiplied)
   auto block = [&](uint32_t kat, uint32_t vat, int kb) {      // kb: the wave's first key
@@ -518,36 +528,19 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
     }
-    // Where a row leaves out a key that exists, its weight 0 may meet an infinity or a NaN of that key's V: those are taken out
-    // of the product, and the rows that do attend the key add them themselves (uniform; rare; without this the blocks on the
-    // diagonal would carry a token's NaN to tokens before it. It costs 4% of a prompt of 8000 tokens, 5% of a mixed step)
+    // Where a row leaves out a key that the block holds, its weight 0 may meet an infinity or a NaN of that key's V: those are
+    // taken out of the product, and the rows that do attend the key get them after the walk (uniform; rare)
     bool odd = false;
-    if (wmin < min(kb + 31, len - 1)) {
+    if (guarded(kb)) {
+      uint32_t any = 0;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4 second = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          odd |= finite2<T>(va[0][dt][e]) != va[0][dt][e] || finite2<T>(second[e]) != second[e];
+        for (int e = 0; e < 4; ++e) any |= odd2<T>(va[0][dt][e]) | odd2<T>(second[e]);
       }
-      odd = __any(odd);
-      if (odd) {
-        const int last = min(pr, kend - 1) - kb;
-#pragma unroll 1
-        for (int key = 0; key < 32; ++key)
-          if (key <= last) {
-            const uint32_t at = vat + kV + (32 * kgrp + key) * RB + 8 * h;
-#pragma unroll
-            for (int v = 0; v < D / 8; ++v) {
-              const uint2 p = *reinterpret_cast<const uint2*>(smem + at + 16 * (v ^ vswz(key)));
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t w = i < 2 ? p.x : p.y;
-                if (((w >> (16 * (i & 1))) & Mfma<T>::kExponent) == Mfma<T>::kExponent) o[v >> 2][4 * (v & 3) + i] += Mfma<T>::half_of(w, i & 1);
-              }
-            }
-          }
-      }
+      odd = __any(any != 0);
+      some_odd |= odd;
     }
     const float sub = ref == -INFINITY ? 0.f : ref - (15.f - kLag);
     const f32x16 sc = st;
@@ -616,6 +609,28 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       }
     }
     lds_wait_barrier<0>();                                    // nothing is left in flight, and the slots may be reused
+    if (some_odd) {                                           // the values that the guarded blocks left out, from the pages again
+#pragma unroll 1
+      for (int i = b0; i < b1; ++i) {
+        const int kb = i * BK + 32 * kgrp;
+        if (!guarded(kb)) continue;
+#pragma unroll 1
+        for (int key = kb; key < min(kb + 32, kend); ++key) {
+          const int id = table[key >> shift];
+          if (id < 0 || id >= bt.pages) continue;             // (zeros)
+          const T* from = v_cache + (((int64_t)id * Hkv + un.hk) * bt.page_size + (key & (bt.page_size - 1))) * D + 4 * h;
+#pragma unroll
+          for (int v = 0; v < D / 8; ++v) {
+            const uint2 p = *reinterpret_cast<const uint2*>(from + 8 * v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t w = e < 2 ? p.x : p.y;
+              if (key <= pr && (odd2<T>(w) >> (16 * (e & 1)) & 0x8000u)) o[v >> 2][4 * (v & 3) + e] += Mfma<T>::half_of(w, e & 1);
+            }
+          }
+        }
+      }
+    }
   }
   float den = lsum[0] + lsum[1];
   den += __shfl_xor(den, 32, 64);
