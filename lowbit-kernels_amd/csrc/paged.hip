@@ -751,8 +751,9 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
         top = nm;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (m[i] == -INFINITY) continue;                    // (a part that saw no key)
-          const float f = __builtin_amdgcn_exp2f(m[i] - top);
+          if (p0 + PG * i >= un.parts) continue;
+          // (no score of a part's keys above -inf: its sums are zeros, or NaN where a score was, which factor 0 keeps)
+          const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - top);
           den = fmaf(f, l[i], den);
 #pragma unroll
           for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[i][e], num[e]);
