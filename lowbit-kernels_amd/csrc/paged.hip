@@ -334,8 +334,10 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // taking the block's 32 keys of key group kg for its rows. Per 32 keys (32x32x16 MFMA, lane l: j = l % 32, h = l / 32):
 //   S^T = K Q^T: A = 32 keys x 16 dims from LDS, B = 32 rows (registers); lane (j, h) holds row j's scores of keys 8 (v / 4) +
 //   4 h + v % 4, v < 16.
-//   Softmax in base 2 against a reference that follows the running maximum only when a score passes it by more than kLag, so
-//   that the output's registers are rescaled in the first blocks only. Weights are 2^(score - reference + 15 - kLag), the
+//   Softmax in base 2 (c2 = |scale| log2 e) against a reference that follows the row's running maximum only when a score passes
+//   it by more than kLag / c2, so that the output's registers are rescaled in the first blocks only. The products start at
+//   minus the reference, so that a difference is scaled and rounded, never the score itself: above 2^24 / c2, scaled scores have
+//   steps of 1 and more, and weights 2^(step / 2) too large leave fp16. Weights are 2^((score - reference) c2 + 15 - kLag), the
 //   largest between 2^(15 - kLag) and 2^15, rounded to T for the second product: half a step of T for each weight, the same
 //   relative step as the output's own rounding; in fp16 those below 2^-14 are off by 2^-25, i.e. 2^-32 of the largest. Their
 //   sum, in 32 bits, is of the rounded weights, as the output's is.
@@ -354,6 +356,9 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three waves per SIMD (168 registers,
 // spilled) 546; two blocks ahead instead of three 519 .. 536.
 constexpr float kLag = 8.f;
+
+// of scores to powers of 2; a negative scale's sign goes into q
+__device__ __forceinline__ float score_scale(float scale) { return fmaxf(fabsf(scale) * 1.44269504088896340736f, FLT_MIN); }
 
 template <typename T, int D, int RG, int KG>
 __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
   const int b0 = min(nblk, un.pid * per), b1 = min(nblk, b0 + per);
   const int kend = min(keys, b1 * BK);
   // this lane's row: its last key (the least of the wave's rows: wmin) and q
-  const float c2 = fabsf(scale) * 1.44269504088896340736f < FLT_MIN ? FLT_MIN : fabsf(scale) * 1.44269504088896340736f;
+  const float c2 = score_scale(scale), lag = fminf(kLag / c2, FLT_MAX);
   const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;      // a negative scale is moved into q (exact)
   const int row = un.tile * kRows + 32 * rgrp + j, row_c = min(row, rows - 1), tok = div(row_c, plan.by_g);
   const bool live = row < rows;
@@ -491,9 +496,10 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  float ref = -INFINITY, lsum[2] = {0.f, 0.f};                // reference (base 2), the lane's share of the weights' sum
+  float lsum[2] = {0.f, 0.f};                                 // the lane's share of the weights' sum
   const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  f32x16 o[DT], st = zero;                                    // output, scores of the wave's 32 keys of a block
+  f32x16 o[DT], st = zero, neg = zero;                        // output, scores of the wave's 32 keys of a block less the row's
+  float pass = -INFINITY;                                     // reference, minus that; what a score passes to move it (-inf: none yet)
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = zero;
   auto k_frag = [&](uint32_t at, int s) { return *reinterpret_cast<const u32x4*>(smem + at + (kr ^ (32 * s))); };
@@ -519,12 +525,19 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     float bm = st[0];
 #pragma unroll
     for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
-    if (__any(bm * c2 > ref + kLag)) {                        // (uniform; either lane of a row)
-      const float nm = fmaxf(ref, fmaxf(bm, __shfl_xor(bm, 32, 64)) * c2);   // -inf while the row has seen no key
-      const float corr = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - nm);
-      ref = nm;
+    if (__any(bm > pass)) {                                   // (uniform; either lane of a row)
+      const bool fresh = pass == -INFINITY;                   // (the row has seen no key: its reference counts as 0)
+      const float top = fmaxf(bm, __shfl_xor(bm, 32, 64)), up = fresh ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
+      const float ref = up - neg[0], d = ref + neg[0];        // (d: what the rounded reference moves by)
+      const float corr = fresh ? 1.f : __builtin_amdgcn_exp2f(-d * c2);
+      pass = top == -INFINITY ? pass : lag;
       lsum[0] *= corr;
       lsum[1] *= corr;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        st[v] -= d;
+        neg[v] = -ref;
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
     }
@@ -537,21 +550,24 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       for (int dt = 0; dt < DT; ++dt) {
         const u32x4 second = v_frag(vat + (vr ^ (64 * dt)) + 16 * RB);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) any |= odd2<T>(va[0][dt][e]) | odd2<T>(second[e]);
+        for (int e = 0; e < 4; ++e) {
+          uint32_t first = va[0][dt][e];
+          asm("" : "+v"(first));                              // (else every block takes the steps shared with finite2 below)
+          any |= odd2<T>(first) | odd2<T>(second[e]);
+        }
       }
       odd = __any(any != 0);
       some_odd |= odd;
     }
-    const float sub = ref == -INFINITY ? 0.f : ref - (15.f - kLag);
     const f32x16 sc = st;
-    st = zero;
+    st = neg;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {                             // 16 keys
       u32x4 ph;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ph[i] = Mfma<T>::pack(__builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i], c2, -sub)),
-                              __builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i + 1], c2, -sub)));
+        ph[i] = Mfma<T>::pack(__builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i], c2, 15.f - kLag)),
+                              __builtin_amdgcn_exp2f(fmaf(sc[8 * s + 2 * i + 1], c2, 15.f - kLag)));
         lsum[i & 1] = Mfma<T>::sum2(ph[i], lsum[i & 1]);
       }
 #pragma unroll
@@ -632,6 +648,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       }
     }
   }
+  const float ref = pass == -INFINITY ? -INFINITY : -neg[0];
   float den = lsum[0] + lsum[1];
   den += __shfl_xor(den, 32, 64);
   if constexpr (KG > 1) {
@@ -661,7 +678,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
       for (int k = 0; k < KG; ++k) {
         const float* theirs = at + k * RG * 32 * kPitch;
-        const float m = theirs[D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        const float m = theirs[D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c2);
         const f32x4 v = *reinterpret_cast<const f32x4*>(theirs + d);
         all = fmaf(f, theirs[D + 1], all);
 #pragma unroll
@@ -705,7 +722,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 }
 
 // The outputs of the split tiles: a workgroup takes chunks of paged_merge_rows rows, PG lane groups a row, each joining every
-// PG-th part in order, their weights 2^(reference - largest reference); then the groups' sums. Tiles of 32 rows, which few
+// PG-th part in order, their weights 2^((reference - largest reference) c2); then the groups' sums. Tiles of 32 rows, which few
 // rows on many parts take, have four groups a row, the others one.
 template <int kRows>
 constexpr int paged_merge_groups() { return kRows == 32 ? 4 : 1; }
@@ -713,13 +730,14 @@ template <int D, int kRows>
 constexpr int paged_merge_rows() { return 1024 / D / paged_merge_groups<kRows>(); }
 template <typename T, int D, int kRows, int kBlock>
 __global__ __launch_bounds__(256) void paged_attention_merge(const float* __restrict__ part, PagedBatch bt, PagedPlan plan,
-                                                             T* __restrict__ out) {
+                                                             T* __restrict__ out, float scale) {
   constexpr int kLanes = D / 4, PG = paged_merge_groups<kRows>(), kHere = paged_merge_rows<D, kRows>(), kRec = paged_rec<D>();
   __shared__ f32x4 s_num[256];
   __shared__ float s_top[256 / kLanes], s_den[256 / kLanes];
   args_in_sgprs(part, bt.table, bt.q_starts, bt.kv_lens, bt.B, bt.T, bt.table_width, bt.page_size, plan.slots, plan.cap, plan.G,
                 plan.by_hkv.m, plan.by_g.m, out);
   const int lane = threadIdx.x & 63, grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  const float c2 = score_scale(scale);
   const PagedSeq s0 = paged_seq<kRows, kBlock>(bt, plan.G, lane);
   const int share = paged_share<kRows, kBlock>(bt, plan, s0, lane);
   PagedUnit un;
@@ -745,7 +763,7 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
           if (p0 + PG * i >= un.parts) m[i] = -INFINITY;
           nm = fmaxf(nm, m[i]);
         }
-        const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - nm);
+        const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - nm) * c2);
         den *= f0;
         num *= f0;
         top = nm;
@@ -753,7 +771,7 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
         for (int i = 0; i < 8; ++i) {
           if (p0 + PG * i >= un.parts) continue;
           // (no score of a part's keys above -inf: its sums are zeros, or NaN where a score was, which factor 0 keeps)
-          const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - top);
+          const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - top) * c2);
           den = fmaf(f, l[i], den);
 #pragma unroll
           for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[i][e], num[e]);
@@ -776,7 +794,7 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
         den = 0.f;
 #pragma unroll
         for (int i = 0; i < PG; ++i) {
-          const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c2);
           den = fmaf(f, s_den[grp + i], den);
 #pragma unroll
           for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + i * kLanes][e], num[e]);
@@ -844,7 +862,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   constexpr int kHere = paged_merge_rows<D, kRows>();
   const int64_t chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
   return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
-                static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out));
+                static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.scale);
 }
 
 // Which tile serves a call; any serves every call. Sequences of at most 32 rows (decode, few drafted tokens) take four waves
