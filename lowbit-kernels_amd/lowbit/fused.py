@@ -287,8 +287,12 @@ class FusedQwen2:
     def score(self, tokens, top=0):
         """The log probability of each of tokens [M] (int64, M >= 2) after the first, given the ones before it: (log
         probabilities [M - 1], entropies of the distributions [M - 1], and the `top` <= 32 likeliest tokens' log
-        probabilities and ids [M - 1, top]), float32 and int64, from one forward (cache rows 0 .. M - 1 are written)."""
-        logits = self.forward(tokens, torch.arange(tokens.shape[0], device=tokens.device))
+        probabilities and ids [M - 1, top]), float32 and int64, from one forward (cache rows 0 .. M - 1 are written; a text
+        of more than max_len tokens is refused)."""
+        m = tokens.shape[0]
+        if m > self.max_len:
+            raise ValueError(f"a {m}-token text does not fit a {self.max_len}-token cache")
+        logits = self.forward(tokens, torch.arange(m, device=tokens.device))
         return ops.ext().token_logprobs(logits[:-1], tokens[1:].contiguous(), top)
 
     def paged_caches(self, pages, page_size=64):
