@@ -308,14 +308,13 @@ class FusedQwen2:
         q_starts[b + 1] (int32 [B + 1]); its keys, the new tokens' included, are the first kv_lens[b] (int32 [B]) in the pages
         page_table[b] (int32 [B, width]), and token t's k and v go to slot slots[t] = page * page_size + row (negative: a
         padded token's, nowhere). max_new, max_keys: bounds on a sequence's new tokens and keys. Returns the logits of `rows`
-        (int64, indices into the T tokens; None: of all)."""
+        (int64, indices into the T tokens; None: of all; may be empty, as T may be 0)."""
         ext = ops.ext()
         t = tokens.shape[0]
         h = self._embedding(tokens)
-        xn = torch.empty_like(h)
         q = torch.empty(t, self.hq, self.head_dim, dtype=torch.float16, device=h.device)
         attn = torch.zeros_like(q)                          # (rows of no sequence are left alone: zeros)
-        for i, lay in enumerate(self.layers):
+        for i, lay in enumerate(self.layers if t else ()):
             k_cache, v_cache = caches[0][i], caches[1][i]
             qkv = lay["qkv"](h, EPI_BIAS, lay["qkv"].bias, norm=(lay["in_norm"], self.eps))
             ext.norm_rope_paged(qkv, None, None, self.eps, positions, self.inv_freq, slots, q, k_cache, v_cache, self.hq,
@@ -326,9 +325,9 @@ class FusedQwen2:
             lay["down"](act, EPI_RESIDUAL, h, out=h)
         if rows is not None:
             h = h[rows]
-            xn = torch.empty_like(h)
-        ext.rmsnorm(h, self.final_norm, self.eps, out=xn)
-        return self.logits(xn)
+        if h.shape[0] == 0:                                 # (a step of prompt pieces alone asks for no logits)
+            return h.new_empty(0, self.head.shape[0])
+        return self.logits(ext.rmsnorm(h, self.final_norm, self.eps))
 
 
 class FusedDecoder:
