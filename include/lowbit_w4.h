@@ -334,8 +334,8 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
  * `scale`; softmax, its sums and the output's sums in 32 bits. Rows past a sequence's keys may hold anything, and an
  * infinity or a NaN in a key's k or v reaches only the rows that attend the key. max_new and max_keys: bounds on a sequence's
  * new tokens and keys that size the launch (a captured graph keeps them); results do not depend on them beyond the order of
- * sums. workspace (optional, 16-byte aligned, no initial contents): lets few rows split their keys over the GPU; calls that
- * overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22,
+ * sums. workspace (optional, 16-byte aligned, no initial contents): lets few rows split their keys over the GPU, as far as its
+ * size goes (lowbit_attention_paged_workspace: what the call has use for); calls that overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22,
  * table_width * page_size 2^30. */
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
@@ -343,13 +343,19 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
                            int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* Bytes of workspace that lowbit_attention_paged has use for with these sizes and bounds (0: it splits nothing, or refuses
+ * them). */
+size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                                        int64_t page_size, int64_t max_new, int64_t max_keys);
+
 /* For M <= 2^22 rows of logits [V] (float32, float16 or bfloat16; row m at logits + m * row_stride values, any alignment of the
  * type): logprob[m] = log_softmax(logits[m])[targets[m]] (0 where the target is negative: none asked; NaN where it is V or
  * more), entropy[m] = - sum p log p (0 log 0 = 0), and the `top` <= 32 largest logits of the row in falling order, equal
  * ones by index (-0 equal to +0, a NaN above every number): top_ids [M][top] and their log probabilities top_values
  * [M][top]. Sums in 32 bits. A row with a NaN, a +inf, or nothing above -inf has NaN results, its top_ids by the same
- * order. workspace (optional, 16-byte aligned, no initial contents): lets few rows split over the GPU; calls that overlap
- * must not share one. */
+ * order. workspace (optional, 16-byte aligned, no initial contents): lets few rows split over the GPU, as far as its size goes
+ * ((1024 + M) * (16 + 8 * top) bytes serve every split, none is made from 512 rows on); calls that overlap must not share
+ * one. */
 int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* targets, float* logprob,
                           float* entropy, float* top_values, int64_t* top_ids, int64_t M, int64_t V, int top,
                           void* workspace, size_t workspace_bytes, void* stream);

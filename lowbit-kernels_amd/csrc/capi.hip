@@ -675,6 +675,39 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
   return hip_status(norm_rope_paged_launch(a, static_cast<hipStream_t>(stream)), "norm_rope_paged");
 }
 
+static int check_paged_batch(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t table_width, int64_t page_size,
+                             int64_t max_new, int64_t max_keys) {
+  // (the launch's workgroups and the keys' numbers stay within 32 bits)
+  if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > (1 << 22) / Hkv || table_width > (1 << 30) / page_size)
+    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B * Hkv "
+                "2^22 and the table's keys 2^30");
+  if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
+  return LOWBIT_OK;
+}
+
+static PagedAttentionArgs paged_sizes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                                      int64_t page_size, int64_t max_new, int64_t max_keys) {
+  PagedAttentionArgs a{};
+  a.batch.T = (int)T;
+  a.batch.B = (int)B;
+  a.batch.table_width = (int)table_width;
+  a.batch.page_size = (int)page_size;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.max_new = (int)std::min(max_new, T);
+  a.max_keys = (int)std::min(max_keys, table_width * page_size);
+  return a;
+}
+
+size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                                        int64_t page_size, int64_t max_new, int64_t max_keys) {
+  if (check_paged("attention_paged", LOWBIT_DTYPE_F16, Hq, Hkv, D, 1, page_size) ||
+      check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
+    return 0;
+  return attention_paged_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
+}
+
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
@@ -683,11 +716,7 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
   if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
     return fail(LOWBIT_ERR_ARG, "null pointer argument");
   if (int rc = check_paged("attention_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
-  // (the launch's workgroups and the keys' numbers stay within 32 bits)
-  if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > (1 << 22) / Hkv || table_width > (1 << 30) / page_size)
-    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B * Hkv "
-                "2^22 and the table's keys 2^30");
-  if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
+  if (int rc = check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys)) return rc;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return fail(LOWBIT_ERR_ALIGN, "attention_paged needs 16-byte aligned q, caches and out");
   if ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(q_starts) |
@@ -695,10 +724,19 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
     return fail(LOWBIT_ERR_ALIGN, "attention_paged needs naturally aligned page_table, q_starts and kv_lens");
   if (workspace && !aligned16(workspace)) return fail(LOWBIT_ERR_ARG, "attention_paged: the workspace must be 16-byte aligned");
   if (int rc = check_device()) return rc;
-  const PagedAttentionArgs a{q, k_cache, v_cache, out,
-                             PagedBatch{page_table, q_starts, kv_lens, (int)T, (int)B, (int)table_width, (int)page_size, pages},
-                             dtype == LOWBIT_DTYPE_BF16, (int)Hq, (int)Hkv, (int)D, (int)std::min(max_new, T),
-                             (int)std::min(max_keys, table_width * page_size), scale, workspace, workspace ? workspace_bytes : 0};
+  PagedAttentionArgs a = paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys);
+  a.q = q;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.out = out;
+  a.batch.table = page_table;
+  a.batch.q_starts = q_starts;
+  a.batch.kv_lens = kv_lens;
+  a.batch.pages = pages;
+  a.bf16 = dtype == LOWBIT_DTYPE_BF16;
+  a.scale = scale;
+  a.ws = workspace;
+  a.ws_bytes = workspace ? workspace_bytes : 0;
   return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
 }
 

@@ -397,6 +397,7 @@ struct PagedAttentionArgs {
   size_t ws_bytes;
 };
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st);
+size_t attention_paged_workspace(const PagedAttentionArgs& a);   // bytes that the launch has use for; reads sizes and bounds only
 
 // ---- log probabilities (logprobs.hip) ----
 constexpr int kMaxTop = 32;

@@ -325,8 +325,7 @@ constexpr size_t paged_lds() {
   const size_t merge = KG > 1 ? (size_t)4 * 32 * (D + 4) * 4 : 0;
   return ring > merge ? ring : merge;
 }
-template <int RG, int KG>
-constexpr int paged_per_cu() { return KG > 1 ? 1 : RG == 1 ? 5 : 2; }   // workgroups, by their LDS at D = 128
+constexpr int paged_per_cu(int rg, int kg) { return kg > 1 ? 1 : rg == 1 ? 5 : 2; }   // workgroups, by their LDS at D = 128
 template <int D>
 constexpr int paged_rec() { return D + 4; }                  // floats of a row's record: reference, weight sum, -, -, output
 
@@ -833,23 +832,62 @@ constexpr int kPagedParts = 256;                             // of a tile at mos
 constexpr int kPagedLeast = 256;                             // keys of a part at least
 constexpr int kPagedWhole = 768;                             // keys up to which decode tiles are not split
 
-template <typename T, int D, int RG, int KG>
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
-  constexpr size_t lds = paged_lds<D, RG, KG>();
-  constexpr int kRows = 32 * RG, kBlock = 32 * KG;
-  const int G = a.Hq / a.Hkv;
-  PagedPlan p{256 * paged_per_cu<RG, KG>(), std::max(1, kPagedLeast / kBlock), 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
-  const int64_t seqs = std::min(a.batch.B, a.batch.T);        // with new tokens
-  const int64_t units = (((int64_t)a.batch.T * G + kRows - 1) / kRows + seqs) * a.Hkv;
-  p.most = (int)std::min<size_t>(4 * (size_t)p.slots, a.ws_bytes / ((size_t)kRows * paged_rec<D>() * sizeof(float)));
+// How a call is launched, from its sizes and bounds alone.
+struct PagedLaunch {
+  int rg, kg;                                                // the tile, as rows and keys of 32
+  int slots;                                                 // workgroups that the GPU holds at once
+  int64_t units;                                             // tiles times KV heads at most
+  int least, cap;                                            // blocks of a part at least, parts of a tile at most (1: no split)
+  int records;                                               // of split tiles that the workspace has use for
+};
+
+// Which tile serves a call; any serves every call. Sequences of at most 32 rows (decode, few drafted tokens) take four waves
+// on four key groups (RG 1, KG 4), one workgroup a CU; where there are more tiles than those and the keys are few, or very many
+// tiles, one wave, five a CU (28 / 4 heads, us, four waves / one: 100 tokens on 100 keys 12.7 / 8.7, 300 on 100 36 / 21, on 1000
+// 150 / 148, 30 tokens of 32 / 32 heads on up to 2000 63 / 57; but 40 on 500 14.5 / 17.3, 100 on 500 32.0 / 32.9, on 2000 89 /
+// 94, 64 of 32 / 8 heads on 300 .. 8000 125 / 139). More rows take four waves of 128 rows (RG 4), two workgroups a CU, or of 64
+// rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts (us, 128
+// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51;
+// 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
+PagedLaunch paged_launch(const PagedAttentionArgs& a) {
+  const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T);   // with new tokens
+  auto tiles = [&](int rows) { return ((int64_t)a.batch.T * G / rows + seqs) * a.Hkv; };   // at most
+  PagedLaunch p{};
+  if (a.max_new * G <= 32) {
+    p.rg = 1;
+    p.kg = tiles(32) > 256 && (a.max_keys <= 512 || tiles(32) > 768) ? 1 : 4;
+  } else if (tiles(64) <= 256 && a.max_keys <= 1024) {
+    p.rg = p.kg = 2;
+  } else {
+    p.rg = 4;
+    p.kg = 1;
+  }
+  const int rows = 32 * p.rg, block = 32 * p.kg;
+  p.slots = 256 * paged_per_cu(p.rg, p.kg);
+  p.units = (((int64_t)a.batch.T * G + rows - 1) / rows + seqs) * a.Hkv;
+  p.least = std::max(1, kPagedLeast / block);
   // no split, and no launch of the merge, where it does not pay: decode tiles of few keys, other tiles of not many that fill
   // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.7 / 11.9, one launch less for
   // the host; 40 on 800 18.8, on 760 whole 15.3; a prompt of 500 29.5 / 16.3; six prompts of 171 .. 794, 14 / 2 heads of 64,
   // 23.6 / 20.3)
-  const bool whole = RG == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * units >= p.slots;
-  if (a.ws && p.most >= 2 && !whole)
-    p.cap = std::min(kPagedParts, (int)((((int64_t)a.max_keys + kBlock - 1) / kBlock + p.least - 1) / p.least));
-  const int64_t grid = p.cap == 1 ? units : std::min<int64_t>(units * p.cap, units + p.most / 2 + 1);
+  const bool whole = p.rg == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * p.units >= p.slots;
+  p.cap = whole ? 1 : std::min(kPagedParts, (int)((((int64_t)a.max_keys + block - 1) / block + p.least - 1) / p.least));
+  // twice the free slots that paged_share gives parts at most, and twice what the tiles can be cut into
+  p.records = p.cap == 1 ? 0 : (int)std::min<int64_t>(p.rg == 4 ? 2048 : 1024, 2 * p.units * p.cap);
+  return p;
+}
+
+size_t paged_record_bytes(int rg, int D) { return (size_t)32 * rg * (D == 64 ? paged_rec<64>() : paged_rec<128>()) * sizeof(float); }
+
+template <typename T, int D, int RG, int KG>
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch& l, hipStream_t st) {
+  constexpr size_t lds = paged_lds<D, RG, KG>();
+  constexpr int kRows = 32 * RG, kBlock = 32 * KG;
+  const int G = a.Hq / a.Hkv;
+  PagedPlan p{l.slots, l.least, 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
+  p.most = a.ws ? (int)std::min<size_t>((size_t)l.records, a.ws_bytes / paged_record_bytes(RG, D)) : 0;
+  if (p.most >= 2) p.cap = l.cap;
+  const int64_t grid = p.cap == 1 ? l.units : std::min<int64_t>(l.units * p.cap, l.units + p.most / 2 + 1);
   if (lds > 65536) {
     static std::atomic<uint64_t> done{0};
     if (hipError_t e = allow_lds_once(done, paged_attention<T, D, RG, KG>, lds)) return e;
@@ -860,29 +898,17 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
                         a.batch, p, static_cast<T*>(a.out), static_cast<float*>(a.ws), shift, a.scale);
   if (e != hipSuccess || p.cap == 1) return e;
   constexpr int kHere = paged_merge_rows<D, kRows>();
-  const int64_t chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
+  const int64_t seqs = std::min(a.batch.B, a.batch.T), chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
   return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
                 static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.scale);
 }
 
-// Which tile serves a call; any serves every call. Sequences of at most 32 rows (decode, few drafted tokens) take four waves
-// on four key groups (RG 1, KG 4), one workgroup a CU; where there are more tiles than those and the keys are few, or very many
-// tiles, one wave, five a CU (28 / 4 heads, us, four waves / one: 100 tokens on 100 keys 12.7 / 8.7, 300 on 100 36 / 21, on 1000
-// 150 / 148, 30 tokens of 32 / 32 heads on up to 2000 63 / 57; but 40 on 500 14.5 / 17.3, 100 on 500 32.0 / 32.9, on 2000 89 /
-// 94, 64 of 32 / 8 heads on 300 .. 8000 125 / 139). More rows take four waves of 128 rows (RG 4), two workgroups a CU, or of 64
-// rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts (us, 128
-// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51;
-// 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
 template <typename T, int D>
 hipError_t pick_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
-  const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T);
-  auto tiles = [&](int rows) { return ((int64_t)a.batch.T * G / rows + seqs) * a.Hkv; };   // at most
-  if (a.max_new * G <= 32) {
-    if (tiles(32) > 256 && (a.max_keys <= 512 || tiles(32) > 768)) return launch_paged_attention<T, D, 1, 1>(a, st);
-    return launch_paged_attention<T, D, 1, 4>(a, st);
-  }
-  if (tiles(64) <= 256 && a.max_keys <= 1024) return launch_paged_attention<T, D, 2, 2>(a, st);
-  return launch_paged_attention<T, D, 4, 1>(a, st);
+  const PagedLaunch l = paged_launch(a);
+  if (l.rg == 4) return launch_paged_attention<T, D, 4, 1>(a, l, st);
+  if (l.rg == 2) return launch_paged_attention<T, D, 2, 2>(a, l, st);
+  return l.kg == 4 ? launch_paged_attention<T, D, 1, 4>(a, l, st) : launch_paged_attention<T, D, 1, 1>(a, l, st);
 }
 
 }  // namespace
@@ -890,6 +916,11 @@ hipError_t pick_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
 hipError_t norm_rope_paged_launch(const NormRopeArgs& a, hipStream_t st) {
   if (a.bf16) return a.D == 64 ? pick_norm_rope<bf16, 64>(a, st) : pick_norm_rope<bf16, 128>(a, st);
   return a.D == 64 ? pick_norm_rope<f16, 64>(a, st) : pick_norm_rope<f16, 128>(a, st);
+}
+
+size_t attention_paged_workspace(const PagedAttentionArgs& a) {
+  const PagedLaunch l = paged_launch(a);
+  return l.records * paged_record_bytes(l.rg, a.D);
 }
 
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st) {

@@ -7,6 +7,7 @@ output with torch.empty on the input's device, launch on that device's current s
 refusal (the reference's TORCH_CHECK messages). There is no fallback: without the built library every call raises.
 """
 import ctypes
+import functools
 import os
 import pathlib
 
@@ -67,6 +68,7 @@ SIGNATURES = {
                                 _i64, _i64, _i64, _int, _vp], _int),
     "lowbit_attention_paged": ([_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                 _i64, _i64, ctypes.c_float, _vp, ctypes.c_size_t, _vp], _int),
+    "lowbit_attention_paged_workspace": ([_i64] * 9, ctypes.c_size_t),
     "lowbit_token_logprobs": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, ctypes.c_size_t, _vp],
                               _int),
     "lowbit_hbm_read": ([_vp, _i64, _vp, _i64, _vp], _int),
@@ -163,8 +165,6 @@ WORKSPACE_COUNTER_BYTES = 16384
 WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (16 << 20)     # LOWBIT_WORKSPACE_BYTES
 PREFILL_WORKSPACE_BYTES = WORKSPACE_COUNTER_BYTES + (64 << 20)
 ATTENTION_WORKSPACE_BYTES = 4 << 20
-PAGED_SPLIT_KEYS = 256                  # attention_paged cuts longer sequences into parts of at least as many keys,
-PAGED_WHOLE_KEYS = 768                  # those of at most 32 query rows a KV head from more keys on
 PICK_WORKSPACE_BYTES = 1 << 20          # the greedy pick's keys: 8 bytes per 8 head rows
 _WORKSPACES = {}
 _CAPTURE_STREAMS = {}
@@ -305,6 +305,8 @@ class NativeExt:
         global torch
         import torch
         self.lib = lib()
+        # (of sizes alone, and every layer of a step asks for the same ones)
+        self._paged_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_attention_paged_workspace)
 
     def w4_gemv(self, x, w, s, group, version, rows_per_warp=0):
         m, n, k, index = _check_tensors(x, w, s, group)
@@ -756,10 +758,8 @@ class NativeExt:
         if t == 0 or batch == 0:
             return
         # the split tiles' records, from the caching allocator for this call alone: calls on several streams and captured
-        # graphs share none (LOWBIT_PAGED_WORKSPACE_BYTES(rows, D))
-        nbytes = 0
-        if split and max_keys > (PAGED_WHOLE_KEYS if max_new * hq <= 32 * hkv else PAGED_SPLIT_KEYS):
-            nbytes = (1024 * 32 if max_new * hq <= 32 * hkv else 2048 * 128) * (dim + 4) * 4
+        # graphs share none
+        nbytes = self._paged_workspace(t, batch, hq, hkv, dim, width, page_size, int(max_new), int(max_keys)) if split else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged(
             q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),

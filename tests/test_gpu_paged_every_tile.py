@@ -59,3 +59,20 @@ def test_small_workspaces_split_less(cuda, records, dt):
         out = called(x, lens, records * rows * (d + 4) * 4, d ** -0.5)
         check(out, x, lens, d ** -0.5)
         check(called(x, lens, records * rows * (d + 4) * 4 - 16, d ** -0.5), x, lens, d ** -0.5)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_more_workspace_than_asked_for_changes_nothing(cuda, dt):
+    for hq, hkv, d, lens in ((28, 4, 128, [(1, 900 + 97 * i) for i in range(31)]), (28, 4, 128, [(1, 30000), (1, 1)]), (12, 1, 128, [(2, 65000)]),
+                             (14, 2, 64, [(2, 5000), (1, 800), (3, 2000)]), (28, 4, 128, [(1, 1500)] * 200), (28, 4, 128, [(1, 100)] * 280 + [(1, 3000)]),
+                             (28, 4, 128, [(700, 700), (300, 2500), (1, 4000)]), (14, 2, 64, [(1500, 1500)]), (16, 2, 128, [(20, 1000), (9, 600)])):
+        x = paged.batch(lens, hq, hkv, d, 32, dt, len(lens))
+        asked = ops.ext().lib.lowbit_attention_paged_workspace(x[0].shape[0], len(lens), hq, hkv, d, x[3].shape[1], 32,
+                                                               max(n for n, _ in lens), max(k for _, k in lens))
+        print(hq, hkv, d, lens[:2], asked, flush=True)
+        assert asked
+        one = called(x, lens, asked, d ** -0.5)
+        assert torch.equal(one, called(x, lens, asked + (200 << 20), d ** -0.5))
+        out = torch.full_like(one, float("nan"))
+        ops.ext().attention_paged(*x[:6], out, max(n for n, _ in lens), max(k for _, k in lens), d ** -0.5)
+        assert torch.equal(out, one)
