@@ -335,8 +335,8 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
  * infinity or a NaN in a key's k or v reaches only the rows that attend the key. max_new and max_keys: bounds on a sequence's
  * new tokens and keys that size the launch (a captured graph keeps them); results do not depend on them beyond the order of
  * sums. workspace (optional, 16-byte aligned, no initial contents): lets few rows split their keys over the GPU, as far as its
- * size goes (lowbit_attention_paged_workspace: what the call has use for); calls that overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B * Hkv 2^22,
- * table_width * page_size 2^30. */
+ * size goes (lowbit_attention_paged_workspace: what the call has use for); calls that overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B 65536, B *
+ * Hkv 2^22, table_width * page_size 2^30. */
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,

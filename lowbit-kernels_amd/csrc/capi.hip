@@ -677,10 +677,12 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
 
 static int check_paged_batch(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t table_width, int64_t page_size,
                              int64_t max_new, int64_t max_keys) {
-  // (the launch's workgroups and the keys' numbers stay within 32 bits)
-  if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > (1 << 22) / Hkv || table_width > (1 << 30) / page_size)
-    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B * Hkv "
-                "2^22 and the table's keys 2^30");
+  // (the launch's workgroups and the keys' numbers stay within 32 bits; each workgroup walks the lengths of all sequences before
+  // its own, 64 a step: 64 ms for 65536 of 20 keys, 28 / 4 heads, and with the square of B beyond)
+  if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > 65536 || B > (1 << 22) / Hkv ||
+      table_width > (1 << 30) / page_size)
+    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B 65536, "
+                "B * Hkv 2^22 and the table's keys 2^30");
   if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
   return LOWBIT_OK;
 }

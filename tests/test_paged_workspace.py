@@ -37,3 +37,10 @@ def test_sizes():
         assert got <= 2 * tiles * -(-keys // 256) * 128 * (d + 4) * 4
         assert got == size(t, b, hq, hkv, d, 5000, 16, min(new, t), keys)         # at most t tokens are new
         assert size(t, b, hq, hkv, d, 5000, 16, new, 1 << 40) == size(t, b, hq, hkv, d, 5000, 16, new, 80000)
+
+
+def test_batches_whose_lengths_take_too_long_to_walk_are_refused():
+    from test_paged_refusals import attend
+    assert attend(b=65537, t=65537, hq=2, hkv=1) == 3
+    assert "B 65536" in _native.lib().lowbit_last_error().decode()
+    assert size(65537, 65537, 2, 1, 128, 9, 64, 1, 500) == 0 and size(1, 65536, 2, 1, 128, 99, 64, 1, 5000) > 0
