@@ -76,3 +76,26 @@ def test_more_workspace_than_asked_for_changes_nothing(cuda, dt):
         out = torch.full_like(one, float("nan"))
         ops.ext().attention_paged(*x[:6], out, max(n for n, _ in lens), max(k for _, k in lens), d ** -0.5)
         assert torch.equal(out, one)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,n", [(6, 2, 64, 65536), (28, 4, 128, 5001)])
+def test_as_many_sequences_as_are_taken(cuda, hq, hkv, d, n, dt):
+    """One token a sequence on 1 .. 16 keys of one page; pages are shared. Bound as in test_gpu_paged.py (16 keys)."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    kc, vc = (torch.randn(50, hkv, 16, d, generator=gen, device="cuda").to(dt) for _ in range(2))
+    q = torch.randn(n, hq, d, generator=gen, device="cuda").to(dt)
+    page, keys = (torch.randint(0, top, (n,), generator=gen, device="cuda", dtype=torch.int32) for top in (50, 16))
+    keys += 1
+    out = torch.full_like(q, float("nan"))
+    ops.ext().attention_paged(q, kc, vc, page[:, None].contiguous(), torch.arange(n + 1, dtype=torch.int32, device="cuda"), keys, out,
+                              1, 16, d ** -0.5)
+    at, dead = page.long(), torch.arange(16, device="cuda")[None, :] >= keys[:, None]
+    for h in range(hq):
+        k, v, x = kc[at, h // (hq // hkv)].double(), vc[at, h // (hq // hkv)].double(), q[:, h].double()
+        prod = k * x[:, None]
+        p = torch.softmax((prod.sum(-1) * d ** -0.5).masked_fill(dead, -float("inf")), -1)[..., None]
+        want, size = (p * v).sum(1), (p * v.abs()).sum(1)
+        ds = (d + 8) * paged.U * (prod.abs().sum(-1) * d ** -0.5).masked_fill(dead, 0).amax(-1, keepdim=True)
+        tol = size * (paged.half_step(dt) + 2 * ds + 65 * paged.U) + paged.half_step(dt) * want.abs() + paged.least(dt)
+        assert bool(((out[:, h].double() - want).abs() <= tol).all()), h
