@@ -356,8 +356,11 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // spilled) 546; two blocks ahead instead of three 519 .. 536.
 constexpr float kLag = 8.f;
 
-// of scores to powers of 2; a negative scale's sign goes into q
-__device__ __forceinline__ float score_scale(float scale) { return fmaxf(fabsf(scale) * 1.44269504088896340736f, FLT_MIN); }
+// of scores to powers of 2 (a NaN stays one); a negative scale's sign goes into q
+__device__ __forceinline__ float score_scale(float scale) {
+  const float c2 = fabsf(scale) * 1.44269504088896340736f;
+  return c2 < FLT_MIN ? FLT_MIN : c2;
+}
 
 template <typename T, int D, int RG, int KG>
 __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(

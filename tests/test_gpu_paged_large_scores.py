@@ -47,3 +47,11 @@ def test_large_scores(cuda, lens, hq, hkv, d, dt):
                 tol = room * (paged.half_step(dt) + (keys / 16 + 64) * paged.U) + paged.half_step(dt) * want.abs() + paged.least(dt)
                 got = out[x[7][b]:x[7][b + 1], h * (hq // hkv):(h + 1) * (hq // hkv)].double()
                 assert bool(((got - want).abs() <= tol).all()), (size, scale, b, h, got.isfinite().all())
+
+
+def test_a_scale_that_is_not_a_number_is_not_hidden(cuda):
+    for lens in ([(1, 40)], [(1, 5000)], [(200, 700)]):
+        x = paged.batch(lens, 16, 2, 128, 32, torch.float16, 2)
+        out = torch.zeros_like(x[0])
+        ops.ext().attention_paged(*x[:6], out, max(n for n, _ in lens), max(k for _, k in lens), float("nan"))
+        assert bool(out.isnan().all()), lens
