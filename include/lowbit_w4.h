@@ -319,8 +319,9 @@ int lowbit_f16_gemv_pick(const void* x, const void* w, void* y, int64_t N, int64
  * rotate-half position rotation of the pairs (i, i + D / 2) by positions[m] * inv_freq[i] (the angle in 64 bits), all in 32
  * bits and rounded once; q -> q_out [M][Hq][D], k and the v heads as they are -> the caches' slot slots[m]. A slot outside
  * the cache (a padded row's, e.g. -1) leaves the caches as they are; of several rows with one slot any one's values may
- * stay in any of its heads (the callers' tokens have slots of their own). M * (Hq + 2 Hkv) at most 2^25. permuted != 0: each head's D values lie in the RoPE-permuted order of lowbit_rope_kv (16-row
- * tiles: dims 8 t .. 8 t + 7, then D / 2 + 8 t ..). Outputs must not overlap inputs. */
+ * stay in any of its heads (the callers' tokens have slots of their own). M * (Hq + 2 Hkv) at most 2^25. permuted != 0: each
+ * head's D values lie in the RoPE-permuted order of lowbit_rope_kv (16-row tiles: dims 8 t .. 8 t + 7, then D / 2 + 8 t ..).
+ * Outputs must not overlap inputs. */
 int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const void* q_weight, const void* k_weight,
                            float eps, const int64_t* positions, const float* inv_freq, const int64_t* slots,
                            void* q_out, void* k_cache, void* v_cache, int64_t M, int64_t Hq, int64_t Hkv, int64_t D,
@@ -331,12 +332,13 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
  * 0 .. kv_lens[b] - 1, the last of them the new tokens' own, key j in row j % page_size of page page_table[b][j / page_size]
  * (page_table [B][table_width]; keys past the table are not attended, a page outside 0 .. pages - 1 reads as zeros). New
  * token i attends the keys up to kv_lens[b] - new + i; one that is left none (kv_lens[b] < new) gets zeros. Scores scaled by
- * `scale`; softmax, its sums and the output's sums in 32 bits. Rows past a sequence's keys may hold anything, and an
- * infinity or a NaN in a key's k or v reaches only the rows that attend the key. max_new and max_keys: bounds on a sequence's
- * new tokens and keys that size the launch (a captured graph keeps them); results do not depend on them beyond the order of
- * sums. workspace (optional, 16-byte aligned, no initial contents): lets few rows split their keys over the GPU, as far as its
- * size goes (lowbit_attention_paged_workspace: what the call has use for); calls that overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B 65536, B *
- * Hkv 2^22, table_width * page_size 2^30. */
+ * `scale`; scores, the softmax's sums and the output's sums in 32 bits, each weight rounded once to `dtype` before it meets v.
+ * Rows past a sequence's keys may hold anything, and an infinity or a NaN in a key's k or v reaches only the rows that attend the
+ * key. max_new and max_keys: bounds on a sequence's new tokens and keys that size the launch (a captured graph keeps them);
+ * results do not depend on them beyond the order of sums. workspace (optional, 16-byte aligned, no initial contents): lets few
+ * rows split their keys over the GPU, as far as its size goes (lowbit_attention_paged_workspace: what the call has use for);
+ * calls that overlap must not share one. The same bits on every call for given lengths and bounds. T * Hq at most 2^28, B
+ * 65536, B * Hkv 2^22, table_width * page_size 2^30. */
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                            int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,

@@ -192,9 +192,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int se
 
 // The parts' share in blocks. While tiles of one part leave a quarter of the GPU's slots free, the total over the free ones,
 // so that the parts, each sequence's rounded up, run at once; else the total over one and a half rounds of slots, so that only
-// keys far above the mean are cut (64 decode tokens on 300 .. 8000 keys, us: over the slots that two rounds leave free 132,
-// one round 133, one and a half 125, two 128; a prompt of 2000 tokens, 28 / 4 heads: 73, 60 and 78 with half a round, one and
-// two). s0: the first 64 sequences.
+// keys far above the mean are cut (us with half a round, one, one and a half and two: 64 decode tokens of 32 / 8 heads on 300 ..
+// 8000 keys 147, 133, 129 and 128; a prompt of 2000 tokens, 28 / 4 heads, 64, 71, 71 and 79; a mixed step 33.8, 34.2, 34.7 and
+// 34.8). s0: the first 64 sequences.
 template <int kRows, int kBlock>
 __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {
   if (p.cap == 1) return 0x3FFFFFFF;
@@ -339,7 +339,10 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 //   steps of 1 and more, and weights 2^(step / 2) too large leave fp16. Weights are 2^((score - reference) c2 + 15 - kLag), the
 //   largest between 2^(15 - kLag) and 2^15, rounded to T for the second product: half a step of T for each weight, the same
 //   relative step as the output's own rounding; in fp16 those below 2^-14 are off by 2^-25, i.e. 2^-32 of the largest. Their
-//   sum, in 32 bits, is of the rounded weights, as the output's is.
+//   sum, in 32 bits, is of the rounded weights, as the output's is. (As two halves, which leave the output's rounding alone: an
+//   error of 2.0e-4 for 2.4e-4 .. 2.9e-4 of the output in fp16, 1.7e-3 for 2.2e-3 in bf16; but prompts 527 -> 690 us, a mixed
+//   step 35.5 -> 40, one token 13.1 -> 13.8, 64 decode tokens 129.9 -> 130.6, and an infinity in V, times a second half of 0,
+//   would become a NaN.)
 //   O^T += V^T P^T: B = the weights as the lane holds them, A = V^T from LDS by transposing reads.
 // K and V go from the pages straight to LDS, rows as they are: a wave-load takes 1 KB, 512 / D keys, in groups of up to 16 keys
 // of one page, so that address and bound are scalar and looked up once a group; rows past the sequence's keys and pages
@@ -846,12 +849,12 @@ struct PagedLaunch {
 
 // Which tile serves a call; any serves every call. Sequences of at most 32 rows (decode, few drafted tokens) take four waves
 // on four key groups (RG 1, KG 4), one workgroup a CU; where there are more tiles than those and the keys are few, or very many
-// tiles, one wave, five a CU (28 / 4 heads, us, four waves / one: 100 tokens on 100 keys 12.7 / 8.7, 300 on 100 36 / 21, on 1000
-// 150 / 148, 30 tokens of 32 / 32 heads on up to 2000 63 / 57; but 40 on 500 14.5 / 17.3, 100 on 500 32.0 / 32.9, on 2000 89 /
-// 94, 64 of 32 / 8 heads on 300 .. 8000 125 / 139). More rows take four waves of 128 rows (RG 4), two workgroups a CU, or of 64
-// rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts (us, 128
-// rows / 64: 28 / 4 heads, one prompt of 500 24 / 19, of 1200 39 / 45, 500 on 2000 cached 41 / 51;
-// 300 with 40 decode tokens on 500 26 / 30; one of 8000 500 / 910).
+// tiles, one wave, five a CU (28 / 4 heads, us, four waves / one: 100 tokens on 100 keys 13.5 / 9.6, 300 on 100 39 / 22, on 1000
+// 153 / 152, 30 tokens of 32 / 32 heads on up to 2000 48 / 41; but 40 on 500 12.7 / 19.8, 100 on 2000 90 / 95, 64 of 32 / 8 heads
+// on 300 .. 8000 130 / 141; 100 on 500 lie on the line, 26 / 21). More rows take four waves of 128 rows (RG 4), two workgroups
+// a CU, or of 64 rows and two key groups while those tiles fit the CUs once and the keys are few, so that the serial walk counts
+// (us, 128 rows / 64: 28 / 4 heads, one prompt of 500 24.5 / 17.8, of 1200 42 / 50, 500 on 2000 cached 41 / 62, 300 on 500 with
+// 40 decode tokens 25.9 / 29.0; one of 8000 527 / 1042).
 PagedLaunch paged_launch(const PagedAttentionArgs& a) {
   const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T);   // with new tokens
   auto tiles = [&](int rows) { return ((int64_t)a.batch.T * G / rows + seqs) * a.Hkv; };   // at most
@@ -870,9 +873,10 @@ PagedLaunch paged_launch(const PagedAttentionArgs& a) {
   p.units = (((int64_t)a.batch.T * G + rows - 1) / rows + seqs) * a.Hkv;
   p.least = std::max(1, kPagedLeast / block);
   // no split, and no launch of the merge, where it does not pay: decode tiles of few keys, other tiles of not many that fill
-  // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.7 / 11.9, one launch less for
-  // the host; 40 on 800 18.8, on 760 whole 15.3; a prompt of 500 29.5 / 16.3; six prompts of 171 .. 794, 14 / 2 heads of 64,
-  // 23.6 / 20.3)
+  // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.8 / 13.0, where the host saves a
+  // launch, on 1000 12.0 / 15.5, on 3000 12.4 / 34; 8 on 500 12.1 / 11.0, on 1000 12.4 / 15.8; 40, which nearly fill the slots,
+  // on 760 18.3 / 15.7, on 1500 26.7 / 24.1 and on 3000 43.4 / 41.1: the keys alone do not tell those; a prompt of 500 30.0 /
+  // 17.7, of 900 34.0 / 29.3; six prompts of 171 .. 794, 14 / 2 heads of 64, 23.7 / 20.2)
   const bool whole = p.rg == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * p.units >= p.slots;
   p.cap = whole ? 1 : std::min(kPagedParts, (int)((((int64_t)a.max_keys + block - 1) / block + p.least - 1) / p.least));
   // twice the free slots that paged_share gives parts at most, and twice what the tiles can be cut into

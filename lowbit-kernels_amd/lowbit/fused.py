@@ -1,4 +1,5 @@
-"""A Qwen2 decoder forward assembled from the library's kernels, for batch-1 decoding with graph capture.
+"""A Qwen2 decoder forward assembled from the library's kernels, for decoding one sequence over a contiguous cache or a batch
+of sequences over paged ones, with graph capture.
 
 The stock transformers modules issue about fifty launches per decoder layer and token on ROCm (RMSNorm as five
 elementwise ops, RoPE as six, bias and residual adds, cache index copies, mask construction); on MI355X, where a
@@ -11,7 +12,8 @@ small launch costs ~3 us, that overhead, not the projections, dominates a decode
 cache write inside the q|k|v store, whose rows are permuted per head so that rotation partners share a tile: 6
 launches, the attention's partition merge included)
 
-with its own KV cache. The projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the
+with its own KV cache (forward_paged: rmsnorm -> qkv projection -> rotation + write into the pages -> attention over the pages,
+the rest alike, over the caller's caches). The projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the
 consumer fused into the store, for up to 64 rows; dequantize + hipBLASLt beyond) or fp16 (hipBLASLt through torch,
 bias and residual folded into addmm, silu * up as two torch ops), so the two variants share every other kernel and
 differ only in the projections. Weights come from a transformers Qwen2ForCausalLM; q|k|v are merged into one
@@ -128,7 +130,8 @@ def _torch_epilogue(x, w, epilogue, aux, out, round_first=False):
 
 
 class FusedQwen2:
-    """Batch-1 Qwen2 forward from the library's kernels (see the module docstring).
+    """Qwen2 forward from the library's kernels (see the module docstring): one sequence (forward, score), or a batch over paged
+    caches (paged_caches, forward_paged).
 
     build(model, max_len, quant, group, clip_grid): quant = "int4" quantizes every projection with the GPU quantizer
     (the same bits as lowbit.model.quantize_layers) and keeps only the packed weights; quant = "fp16" keeps fp16
