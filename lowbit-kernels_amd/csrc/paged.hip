@@ -352,11 +352,11 @@ constexpr int paged_rec() { return D + 4; }                  // floats of a row'
 // paged_ahead, and a block's scores are multiplied while the vector unit evaluates the block before. With one row group a
 // wave loads the keys it takes itself and no barrier is needed.
 // Bounds (MI355X): few rows, the read of K and V: 64 decode tokens of 32 / 8 heads on 300 .. 8000 keys (626 MB) 130 us, 4.8
-// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 70 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 514 us in fp16,
-// 0.90 PFLOP/s, 501 in bf16; the vector unit and the matrix cores are busy 50% and 44%. There,
-// measured and not kept: 64 rows a wave with one wave per SIMD (half the LDS reads) 703 us; eight waves in two turns, one four
-// on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three waves per SIMD (168 registers,
-// spilled) 546; two blocks ahead instead of three 519 .. 536.
+// TB/s; 3 tokens of 28 / 4 heads on 40000 .. 70000 70 us, 5.1 TB/s. Prompts, power: 8000 tokens of 28 / 4 heads 520 us in fp16
+// and 503 in bf16, 0.88 and 0.91 PFLOP/s, on zeros 422, where the vector unit and the matrix cores are busy 43% and 42%. There,
+// measured and not kept, against 500 us of that time's kernel: 64 rows a wave with one wave per SIMD (half the LDS reads) 703 us;
+// eight waves in two turns, one four on the matrix cores while the other is on the vector unit, 509 us and 454 on zeros; three
+// waves per SIMD (168 registers, spilled) 546; two blocks ahead instead of three 519 .. 536.
 constexpr float kLag = 8.f;
 
 // of scores to powers of 2 (a NaN stays one); a negative scale's sign goes into q
@@ -874,7 +874,7 @@ PagedLaunch paged_launch(const PagedAttentionArgs& a) {
   p.least = std::max(1, kPagedLeast / block);
   // no split, and no launch of the merge, where it does not pay: decode tiles of few keys, other tiles of not many that fill
   // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.8 / 13.0, where the host saves a
-  // launch, on 1000 12.0 / 15.5, on 3000 12.4 / 34; 8 on 500 12.1 / 11.0, on 1000 12.4 / 15.8; 40, which nearly fill the slots,
+  // launch, on 1000 12.0 / 15.5, on 3000 12.4 / 34; 8 on 500 12.1 / 11.0, on 1000 12.4 / 15.8; 40, whose tiles take 160 of the 256 slots,
   // on 760 18.3 / 15.7, on 1500 26.7 / 24.1 and on 3000 43.4 / 41.1: the keys alone do not tell those; a prompt of 500 30.0 /
   // 17.7, of 900 34.0 / 29.3; six prompts of 171 .. 794, 14 / 2 heads of 64, 23.7 / 20.2)
   const bool whole = p.rg == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * p.units >= p.slots;
