@@ -874,9 +874,9 @@ PagedLaunch paged_launch(const PagedAttentionArgs& a) {
   p.least = std::max(1, kPagedLeast / block);
   // no split, and no launch of the merge, where it does not pay: decode tiles of few keys, other tiles of not many that fill
   // half the slots (28 / 4 heads, us, split or its idle merge / whole: one token on 700 keys 11.8 / 13.0, where the host saves a
-  // launch, on 1000 12.0 / 15.5, on 3000 12.4 / 34; 8 on 500 12.1 / 11.0, on 1000 12.4 / 15.8; 40, whose tiles take 160 of the 256 slots,
-  // on 760 18.3 / 15.7, on 1500 26.7 / 24.1 and on 3000 43.4 / 41.1: the keys alone do not tell those; a prompt of 500 30.0 /
-  // 17.7, of 900 34.0 / 29.3; six prompts of 171 .. 794, 14 / 2 heads of 64, 23.7 / 20.2)
+  // launch, on 1000 12.0 / 15.5, on 3000 12.4 / 34; 8 on 500 12.1 / 11.0, on 1000 12.4 / 15.8; 40, whose tiles take 160 of the 256
+  // slots, on 760 18.3 / 15.7, on 1500 26.7 / 24.1 and on 3000 43.4 / 41.1: the keys alone do not tell those; a prompt of 500 30.0
+  // / 17.7, of 900 34.0 / 29.3; six prompts of 171 .. 794, 14 / 2 heads of 64, 23.7 / 20.2)
   const bool whole = p.rg == 1 ? a.max_keys <= kPagedWhole : a.max_keys <= 1024 && 2 * p.units >= p.slots;
   p.cap = whole ? 1 : std::min(kPagedParts, (int)((((int64_t)a.max_keys + block - 1) / block + p.least - 1) / p.least));
   // twice the free slots that paged_share gives parts at most, and twice what the tiles can be cut into
