@@ -350,6 +350,65 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
 size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                                         int64_t page_size, int64_t max_new, int64_t max_keys);
 
+/* lowbit_attention_paged where sequences' new tokens are trees of drafts (or any set that a mask describes): new token i attends the
+ * keys before its sequence's new ones (0 .. kv_lens[b] - new - 1) and, of the new ones', those whose bit is set in its words masks[t
+ * * words ..] (t its row of q; bit j % 64 of word j / 64 for new token j, its own among them only if it is set; new tokens past 64
+ * * words are attended by none; 1 <= words <= 16). One that attends nothing gets zeros. The same workspace. */
+int lowbit_attention_paged_tree(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                                int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, const uint64_t* masks,
+                                int64_t words, void* out, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t pages, int64_t page_size, int64_t max_new, int64_t max_keys, float scale,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* The tables of a step, from its sequences' lengths, without the host. Sequence b goes on from row r = rows[b] of page_table [R][width]
+ * (rows NULL: r = b, R = B; a row outside the table: a sequence without keys), whose first past[r] (int32 [R]) keys it has, by
+ * fresh[b] (int32 [B]) new tokens, numbered one after another over the sequences (those past T are left out):
+ *   q_starts [B + 1], kv_lens [B]: as lowbit_attention_paged takes them;
+ *   table_out [B][width]: the pages of the kept keys as they were, then free ones for the new keys; behind them -1, or, where
+ *     table_out is page_table (rows NULL), what was there. A page is free if no sequence of this call keeps it: the first free pages of
+ *     0 .. pages - 1 go to the sequences in order;
+ *   copies [B][2]: where a sequence's last page is partly filled, is to be written and holds keys of another sequence, the page and
+ *     the free one that takes its place (else -1, -1): of several that it is the last one of, the sequence with the most keys, then
+ *     the first that writes, keeps it, unless it lies within another's keys. With k_cache and v_cache [layers][pages][Hkv][page_size]
+ *     of row_bytes (both or neither NULL) the filled rows are copied too;
+ *   positions, slots [T]: token i of sequence b at position past + i in slot page * page_size + row; -1 without a page. Tokens of
+ *     no sequence: 0 and -1;
+ *   with parents [T] (NULL: none; node i of a sequence hangs below node parents[its row] < i, or is a root: anything else) the new
+ *     tokens are trees: positions are past + depth, and masks [T][words] hold each token's own bit and its ancestors';
+ *   missing [1]: pages that were wanted and not there (their table entries and slots are -1).
+ * past and fresh below 0 count as 0, past above the table's width as that. workspace: lowbit_plan_paged_workspace bytes (0 for small
+ * calls, NULL then), 16-byte aligned, no initial contents; calls that overlap must not share one. B at most 65536, T 2^28, width *
+ * page_size and B * width 2^30. */
+size_t lowbit_plan_paged_workspace(int64_t B, int64_t width, int64_t T, int64_t pages, int64_t page_size);
+int lowbit_plan_paged(const int32_t* page_table, int64_t R, int64_t width, const int32_t* past, const int32_t* fresh,
+                      const int32_t* rows, int64_t B, int64_t T, int64_t pages, int64_t page_size, const int32_t* parents,
+                      int64_t words, int32_t* table_out, int32_t* q_starts, int32_t* kv_lens, int64_t* positions, int64_t* slots,
+                      uint64_t* masks, int32_t* copies, int32_t* missing, void* k_cache, void* v_cache, int64_t layers,
+                      int64_t Hkv, int64_t row_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the model's own picks (int64 [T]: its choice after each token) confirm of drafted tokens (int64 [T]; parents as above, NULL:
+ * chains): sequence b's node 0, then again and again the first child whose token is the pick after the node before, at most
+ * `longest` <= 1024 in all: path [B][longest] (-1 behind), counts [B], accepted [B][longest] the picks after the path's nodes
+ * (the confirmed tokens, then one more; -1 behind), lens [B] = kv_lens - new + count. A sequence without new tokens has count 0.
+ * With k_cache and v_cache (as above) the rows of the path's nodes are moved to the places right behind the sequence's earlier
+ * keys, in every layer, so that its first lens[b] keys are those of the confirmed text; sequences' new tokens must lie in pages of
+ * their own. One launch. */
+int lowbit_accept_drafts(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* q_starts,
+                         const int32_t* kv_lens, const int32_t* page_table, int64_t width, void* k_cache, void* v_cache,
+                         int32_t* path, int32_t* counts, int64_t* accepted, int32_t* lens, int64_t T, int64_t B, int64_t longest,
+                         int64_t layers, int64_t pages, int64_t Hkv, int64_t page_size, int64_t row_bytes, void* stream);
+
+/* The n <= 32 best continuations of each request's beams <= 64: of scores[r][w] + log_softmax(logits[r * beams + w])[v] over all w and
+ * v, the largest in falling order, equal ones by w, then by v (to the sums' rounding: 32 bits; the rest in 64): out_scores,
+ * out_beams, out_tokens [requests][n]. finished (bytes [requests][beams], may be NULL): such a beam has its own score for the token
+ * `pad` and -inf for the others. A score that is no finite number, and a row with a NaN, a +inf or nothing above -inf, has -inf for
+ * every token. logits as lowbit_token_logprobs takes them, rows of beams that need none are not read. workspace required: 16-byte
+ * aligned, at least M * (16 + 8 n) bytes for M = requests * beams, no initial contents; (1024 + M) * (16 + 8 n) bytes serve every
+ * split of few rows; calls that overlap must not share one. */
+int lowbit_beam_select(const void* logits, int dtype, int64_t row_stride, const float* scores, const uint8_t* finished,
+                       float* out_scores, int64_t* out_beams, int64_t* out_tokens, int64_t requests, int64_t beams, int64_t V,
+                       int64_t n, int64_t pad, void* workspace, size_t workspace_bytes, void* stream);
+
 /* For M <= 2^22 rows of logits [V] (float32, float16 or bfloat16; row m at logits + m * row_stride values, any alignment of the
  * type): logprob[m] = log_softmax(logits[m])[targets[m]] (0 where the target is negative: none asked; NaN where it is V or
  * more), entropy[m] = - sum p log p (0 log 0 = 0), and the `top` <= 32 largest logits of the row in falling order, equal

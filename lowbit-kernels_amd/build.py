@@ -29,7 +29,7 @@ OUT = PKG / "lowbit" / "liblowbit_w4.so"
 OUT_FORMAT = PKG / "lowbit" / "liblowbit_format.so"
 ASAN = PKG / "_build_asan"
 SOURCES = ["capi.hip", "gemv.hip", "gemm_mfma.hip", "gemm_prefill.hip", "dequant.hip", "quantize.hip", "decode_ops.hip", "paged.hip",
-           "logprobs.hip", "hbm_probe.hip", "host_format.cpp", "status.cpp"]
+           "paged_tree.hip", "plan.hip", "logprobs.hip", "hbm_probe.hip", "host_format.cpp", "status.cpp"]
 FORMAT_SOURCES = ["host_format.cpp", "status.cpp"]
 # host-only sanitizers: on a hipcc line each -fsanitize= goes after -Xarch_host, so the device code is built without
 SANITIZE_HOST = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined", "-Xarch_host",

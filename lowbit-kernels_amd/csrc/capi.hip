@@ -1,6 +1,7 @@
 // The C ABI (include/lowbit_w4.h): argument validation with the reference's messages, then dispatch to the kernels.
 // The validation mirrors the reference's check() / TORCH_CHECKs (csrc/w4_gemv.cu:312-325,454-540); checks that need
 // tensor metadata (device, dtype, contiguity, dims) are done by the Python layer, which owns the tensors.
+#include <initializer_list>
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -710,11 +711,12 @@ size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_
   return attention_paged_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
 }
 
-int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
-                           int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
-                           int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
-                           int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
-                           void* stream) {
+// attention_paged and attention_paged_tree (masks not NULL)
+static int attend_pages(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                        int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
+                        int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
+                        int64_t max_new, int64_t max_keys, float scale, const uint64_t* masks, int64_t words, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
     return fail(LOWBIT_ERR_ARG, "null pointer argument");
   if (int rc = check_paged("attention_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
@@ -739,7 +741,119 @@ int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const 
   a.scale = scale;
   a.ws = workspace;
   a.ws_bytes = workspace ? workspace_bytes : 0;
-  return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
+  if (!masks) return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
+  a.batch.masks = masks;
+  a.batch.words = (int)words;
+  return hip_status(attention_paged_tree_launch(a, static_cast<hipStream_t>(stream)), "attention_paged_tree");
+}
+
+int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                           int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,
+                           int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
+                           int64_t max_new, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  return attend_pages(q, dtype, k_cache, v_cache, page_table, table_width, q_starts, kv_lens, out, T, B, Hq, Hkv, D, pages,
+                      page_size, max_new, max_keys, scale, nullptr, 0, workspace, workspace_bytes, stream);
+}
+
+int lowbit_attention_paged_tree(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                                int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, const uint64_t* masks,
+                                int64_t words, void* out, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t pages, int64_t page_size, int64_t max_new, int64_t max_keys, float scale,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  if (!masks) return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (words < 1 || words > kMaxMaskWords)
+    return fail(LOWBIT_ERR_SHAPE, "attention_paged_tree: a token's mask must have 1..%d words", kMaxMaskWords);
+  if (reinterpret_cast<uintptr_t>(masks) & 7) return fail(LOWBIT_ERR_ALIGN, "attention_paged_tree needs naturally aligned masks");
+  return attend_pages(q, dtype, k_cache, v_cache, page_table, table_width, q_starts, kv_lens, out, T, B, Hq, Hkv, D, pages,
+                      page_size, max_new, max_keys, scale, masks, words, workspace, workspace_bytes, stream);
+}
+
+// the caches of plan_paged and accept_drafts: [layers][pages][Hkv][page size][row_bytes]; both pointers or none
+static int check_layers(const char* what, const void* k, const void* v, int64_t layers, int64_t pages, int64_t Hkv,
+                        int64_t page_size, int64_t row_bytes) {
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))
+    return fail(LOWBIT_ERR_SHAPE, "%s: the page size must be a power of two from 16 to 65536", what);
+  if (pages < 1 || !fits_int(pages)) return fail(LOWBIT_ERR_SHAPE, "%s: pages must be positive", what);
+  if (!k != !v) return fail(LOWBIT_ERR_ARG, "%s: k_cache goes with v_cache", what);
+  if (!k) return LOWBIT_OK;
+  if (layers < 1 || layers > 65535 || Hkv < 1 || Hkv > 65536 || row_bytes < 16 || row_bytes > 32768 || row_bytes % 16 ||
+      page_size * row_bytes / 16 > (1 << 30) / Hkv)
+    return fail(LOWBIT_ERR_SHAPE, "%s: layers must be 1..65535, rows of the caches 16..32768 bytes, a multiple of 16, and a page of a "
+                "layer less than 2^34 bytes", what);
+  if (!aligned16(k) || !aligned16(v)) return fail(LOWBIT_ERR_ALIGN, "%s needs 16-byte aligned caches", what);
+  return LOWBIT_OK;
+}
+
+static bool aligned_to(std::initializer_list<const void*> p, uintptr_t n) {
+  for (const void* x : p)
+    if (reinterpret_cast<uintptr_t>(x) & (n - 1)) return false;
+  return true;
+}
+
+static int check_plan(int64_t R, int64_t B, int64_t width, int64_t T, int64_t pages, int64_t page_size) {
+  if (R < 1 || B < 1 || width < 1 || T < 0 || !fits_int(R) || B > 65536 || T > (1 << 28) || width > (1 << 30) / page_size ||
+      width > (1 << 30) / B)
+    return fail(LOWBIT_ERR_SHAPE, "plan_paged: R, B and the table's width must be positive, T not negative, B at most 65536, T 2^28, "
+                "the table's keys and B * width 2^30");
+  return LOWBIT_OK;
+}
+
+size_t lowbit_plan_paged_workspace(int64_t B, int64_t width, int64_t T, int64_t pages, int64_t page_size) {
+  if (check_layers("plan_paged", nullptr, nullptr, 0, pages, 0, page_size, 0) || check_plan(B, B, width, T, pages, page_size)) return 0;
+  PlanArgs a{};
+  a.B = (int)B;
+  a.width = (int)width;
+  a.T = (int)T;
+  a.pages = pages;
+  a.page_size = (int)page_size;
+  return plan_paged_workspace(a);
+}
+
+int lowbit_plan_paged(const int32_t* page_table, int64_t R, int64_t width, const int32_t* past, const int32_t* fresh,
+                      const int32_t* rows, int64_t B, int64_t T, int64_t pages, int64_t page_size, const int32_t* parents,
+                      int64_t words, int32_t* table_out, int32_t* q_starts, int32_t* kv_lens, int64_t* positions, int64_t* slots,
+                      uint64_t* masks, int32_t* copies, int32_t* missing, void* k_cache, void* v_cache, int64_t layers,
+                      int64_t Hkv, int64_t row_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!page_table || !past || !fresh || !table_out || !q_starts || !kv_lens || !copies || !missing ||
+      (T > 0 && (!positions || !slots)))
+    return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (int rc = check_layers("plan_paged", k_cache, v_cache, layers, pages, Hkv, page_size, row_bytes)) return rc;
+  if (int rc = check_plan(R, B, width, T, pages, page_size)) return rc;
+  if (!rows && R != B) return fail(LOWBIT_ERR_SHAPE, "plan_paged: without rows the table has a row for every sequence");
+  if (rows && table_out == page_table) return fail(LOWBIT_ERR_ARG, "plan_paged: rows need a table of their own to go to");
+  if (parents && (words < 1 || words > kMaxMaskWords || (T > 0 && !masks)))
+    return fail(LOWBIT_ERR_SHAPE, "plan_paged: trees need masks of 1..%d words a token", kMaxMaskWords);
+  if (!aligned_to({page_table, past, fresh, rows, parents, table_out, q_starts, kv_lens, copies, missing}, 4) ||
+      !aligned_to({positions, slots, masks}, 8))
+    return fail(LOWBIT_ERR_ALIGN, "plan_paged needs naturally aligned arguments");
+  PlanArgs a{page_table, past, fresh, rows, parents, (int)R, (int)B, (int)width, (int)T, parents ? (int)words : 0, (int)page_size,
+             pages, table_out, q_starts, kv_lens, copies, missing, positions, slots, masks, static_cast<uint8_t*>(k_cache),
+             static_cast<uint8_t*>(v_cache), (int)layers, (int)Hkv, (int)row_bytes, workspace};
+  const size_t need = plan_paged_workspace(a);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(LOWBIT_ERR_ARG, "plan_paged: these sizes need a 16-byte aligned workspace of %zu bytes", need);
+  if (int rc = check_device()) return rc;
+  return hip_status(plan_paged_launch(a, static_cast<hipStream_t>(stream)), "plan_paged");
+}
+
+int lowbit_accept_drafts(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* q_starts,
+                         const int32_t* kv_lens, const int32_t* page_table, int64_t width, void* k_cache, void* v_cache,
+                         int32_t* path, int32_t* counts, int64_t* accepted, int32_t* lens, int64_t T, int64_t B, int64_t longest,
+                         int64_t layers, int64_t pages, int64_t Hkv, int64_t page_size, int64_t row_bytes, void* stream) {
+  if (!tokens || !picks || !q_starts || !kv_lens || !page_table || !path || !counts || !accepted || !lens)
+    return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (int rc = check_layers("accept_drafts", k_cache, v_cache, layers, pages, Hkv, page_size, row_bytes)) return rc;
+  if (T < 1 || B < 1 || width < 1 || longest < 1 || T > (1 << 28) || B > 65536 || width > (1 << 30) / page_size || longest > 1024)
+    return fail(LOWBIT_ERR_SHAPE, "accept_drafts: T, B, the table's width and longest must be positive, T at most 2^28, B 65536, the "
+                "table's keys 2^30, longest 1024");
+  if (!aligned_to({tokens, picks, accepted}, 8) || !aligned_to({parents, q_starts, kv_lens, page_table, path, counts, lens}, 4))
+    return fail(LOWBIT_ERR_ALIGN, "accept_drafts needs naturally aligned arguments");
+  if (int rc = check_device()) return rc;
+  const AcceptArgs a{tokens, picks, parents, q_starts, kv_lens, page_table, static_cast<uint8_t*>(k_cache),
+                     static_cast<uint8_t*>(v_cache), path, counts, lens, accepted, (int)T, (int)B, (int)width, (int)longest,
+                     (int)layers, (int)Hkv, (int)row_bytes, (int)page_size, pages};
+  return hip_status(accept_drafts_launch(a, static_cast<hipStream_t>(stream)), "accept_drafts");
 }
 
 int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* targets, float* logprob,
@@ -760,6 +874,28 @@ int lowbit_token_logprobs(const void* logits, int dtype, int64_t row_stride, con
   const LogprobArgs a{logits, dtype, row_stride, targets, logprob, entropy, top_values, top_ids, (int)M, (int)V, top, workspace,
                       workspace ? workspace_bytes : 0};
   return hip_status(token_logprobs_launch(a, static_cast<hipStream_t>(stream)), "token_logprobs");
+}
+
+int lowbit_beam_select(const void* logits, int dtype, int64_t row_stride, const float* scores, const uint8_t* finished,
+                       float* out_scores, int64_t* out_beams, int64_t* out_tokens, int64_t requests, int64_t beams, int64_t V,
+                       int64_t n, int64_t pad, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!logits || !scores || !out_scores || !out_beams || !out_tokens || !workspace) return fail(LOWBIT_ERR_ARG, "null pointer argument");
+  if (dtype < LOWBIT_DTYPE_F32 || dtype > LOWBIT_DTYPE_BF16) return fail(LOWBIT_ERR_ARG, "beam_select: dtype is F32, F16 or BF16");
+  if (requests < 1 || beams < 1 || beams > kMaxBeams || requests > (1 << 22) / beams || V < 1 || !fits_int(V) || !fits_int(V + 65536) ||
+      row_stride < 0 || row_stride > ((int64_t)1 << 40))
+    return fail(LOWBIT_ERR_SHAPE, "beam_select: requests and V must be positive, beams 1..%d, requests * beams at most 2^22, the row "
+                "stride not negative", kMaxBeams);
+  if (n < 1 || n > kMaxTop || n > beams * V) return fail(LOWBIT_ERR_SHAPE, "beam_select: n must be 1..%d and at most beams * V", kMaxTop);
+  if (finished && (pad < 0 || pad >= V)) return fail(LOWBIT_ERR_ARG, "beam_select: pad must be a token");
+  if (!aligned_to({logits}, dtype == LOWBIT_DTYPE_F32 ? 4 : 2) || !aligned_to({scores, out_scores}, 4) ||
+      !aligned_to({out_beams, out_tokens}, 8))
+    return fail(LOWBIT_ERR_ALIGN, "beam_select needs naturally aligned arguments");
+  if (!aligned16(workspace) || workspace_bytes < (size_t)(requests * beams * (16 + 8 * n)))
+    return fail(LOWBIT_ERR_ARG, "beam_select: the workspace must be 16-byte aligned, of at least requests * beams * (16 + 8 n) bytes");
+  if (int rc = check_device()) return rc;
+  const BeamArgs a{logits, dtype, row_stride, scores, finished, out_scores, out_beams, out_tokens, (int)requests, (int)beams, (int)V,
+                   (int)n, (int)pad, workspace, workspace_bytes};
+  return hip_status(beam_select_launch(a, static_cast<hipStream_t>(stream)), "beam_select");
 }
 
 int lowbit_hbm_read(const void* src, int64_t bytes, void* sink, int64_t blocks, void* stream) {

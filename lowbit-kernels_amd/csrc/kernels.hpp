@@ -384,7 +384,11 @@ struct PagedBatch {
   const int* kv_lens;
   int T, B, table_width, page_size;
   int64_t pages;
+  // attention of a tree: bit i of row t's words (masks + t * words): the token attends its sequence's new token i
+  const uint64_t* masks;
+  int words;
 };
+constexpr int kMaxMaskWords = 16;
 struct PagedAttentionArgs {
   const void *q, *k_cache, *v_cache;
   void* out;
@@ -397,9 +401,38 @@ struct PagedAttentionArgs {
   size_t ws_bytes;
 };
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st);
+hipError_t attention_paged_tree_launch(const PagedAttentionArgs& a, hipStream_t st);   // (paged_tree.hip)
 size_t attention_paged_workspace(const PagedAttentionArgs& a);   // bytes that the launch has use for; reads sizes and bounds only
 
-// ---- log probabilities (logprobs.hip) ----
+// ---- a step's tables, and drafts accepted (plan.hip) ----
+struct PlanArgs {
+  const int *table, *past;         // [R][width] and [R]
+  const int *fresh, *rows;         // [B]: new tokens; the row each sequence goes on from (nullptr: its own, R == B)
+  const int* parents;              // [T] or nullptr
+  int R, B, width, T, words, page_size;
+  int64_t pages;
+  int *table_out, *q_starts, *kv_lens, *copies, *missing;   // table_out may be table where rows is nullptr
+  int64_t *positions, *slots;
+  uint64_t* masks;                 // [T][words], words 0 without parents
+  uint8_t *k, *v;                  // nullptr: no copies are made
+  int layers, Hkv, row_bytes;
+  void* ws;                        // plan_paged_workspace(a) bytes
+};
+hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st);
+size_t plan_paged_workspace(const PlanArgs& a);   // reads sizes only
+struct AcceptArgs {
+  const int64_t *tokens, *picks;   // [T]
+  const int *parents;              // [T], or nullptr: chains
+  const int *q_starts, *kv_lens, *table;
+  uint8_t *k, *v;                  // nullptr: no rows are moved
+  int *path, *counts, *lens;
+  int64_t* accepted;
+  int T, B, width, longest, layers, Hkv, row_bytes, page_size;
+  int64_t pages;
+};
+hipError_t accept_drafts_launch(const AcceptArgs& a, hipStream_t st);
+
+// ---- log probabilities and beams (logprobs.hip) ----
 constexpr int kMaxTop = 32;
 struct LogprobArgs {
   const void* logits;
@@ -413,6 +446,20 @@ struct LogprobArgs {
   size_t ws_bytes;
 };
 hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st);
+constexpr int kMaxBeams = 64;
+struct BeamArgs {
+  const void* logits;              // [requests * beams] rows
+  int dtype;                       // LOWBIT_DTYPE_*
+  int64_t stride;
+  const float* scores;             // [requests][beams]
+  const uint8_t* finished;         // the same, or nullptr
+  float* out_scores;               // [requests][n]
+  int64_t *out_beams, *out_tokens;
+  int requests, beams, V, n, pad;
+  void* ws;
+  size_t ws_bytes;                 // at least requests * beams * (16 + 8 * n)
+};
+hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st);
 
 hipError_t dequant_launch(const uint8_t* w, const f16* s, f16* out, int N, int K, int G, bool mfma, hipStream_t st);
 hipError_t relayout_launch(const uint8_t* src, uint8_t* dst, int N, int K, bool mfma, hipStream_t st);

@@ -1,4 +1,5 @@
-// Log probabilities of given tokens with the entropy and the most likely alternatives of each row of logits.
+// Log probabilities of given tokens with the entropy and the most likely alternatives of each row of logits (token_logprobs), and
+// the best continuations of several beams, which are chosen from the same (beam_select).
 //
 // A row is read once from memory. Every lane keeps, against its largest logit so far r, z = sum exp(x - r) and e = sum exp(x -
 // r) (x - r); when all is read, the sums are moved to the row's maximum m: log p(t) = (x_t - m) - log z, H = log z - e / z.
@@ -10,6 +11,7 @@
 // those are read again (from L2). What reaches the bound is ranked by counting.
 // Where there are few rows, each is cut into slices of one workgroup, whose sums and alternatives a second launch joins.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "kernels.hpp"
@@ -94,7 +96,8 @@ __device__ __forceinline__ void store_sums(const T* x, int V, int64_t t, const S
   *entropy = none ? NAN : lz - s.e / s.z;
 }
 
-// Workgroup (row, slice): see the top of the file. part (S > 1): [row][slice] Sums, then keys [row][slice][top].
+// Workgroup (row, slice): see the top of the file. part (S > 1, or beams): [row][slice] Sums, then keys [row][slice][top].
+// scores (beams): the rows' own, by which one that holds nothing or is finished is not read.
 // Bound: memory, 2047 rows of 151665 in fp16 (621 MB) 126 us, 4.9 TB/s; of few rows the chain of load, sums, bound, reread and
 // join: 48 rows of 151936 in fp32 18 us, one in fp16 13.
 template <typename T>
@@ -103,7 +106,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                                             float* __restrict__ logprob, float* __restrict__ entropy,
                                                             float* __restrict__ top_value, int64_t* __restrict__ top_id,
                                                             int V, int top, int S, Sums* __restrict__ part,
-                                                            uint64_t* __restrict__ part_keys) {
+                                                            uint64_t* __restrict__ part_keys,
+                                                            const float* __restrict__ scores,
+                                                            const uint8_t* __restrict__ finished) {
   constexpr int kN = 16 / sizeof(T);
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   float* s_max = reinterpret_cast<float*>(smem);              // [group][thread]
@@ -117,6 +122,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x / S;
   const int slice = blockIdx.x % S;
+  const bool parts = S > 1 || scores;
+  if (scores && (!(fabsf(scores[row]) <= FLT_MAX) || (finished && finished[row]))) return;
   const T* x = logits + row * stride;
   // the row's 16-byte vectors, after a head and before a tail of single logits, which slice 0 and the last slice take
   const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     s.e += o.e;
   }
   if (tid == 0) {
-    if (S == 1)
+    if (!parts)
       store_sums(x, V, targets[row], s, logprob + row, entropy + row);
     else
       part[blockIdx.x] = s;
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   const bool none = !(s.m > -INFINITY && s.m < INFINITY) || s.z != s.z;
   const float lz = logf(s.z);
   auto give = [&](int rank, uint64_t key) {                   // by the thread that holds it
-    if (S > 1) {
+    if (parts) {
       part_keys[(int64_t)blockIdx.x * top + rank] = key;
     } else {
       const int idx = rank_index(key);
@@ -314,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
         for (int k = 0; k < n; ++k) rank += s_list[k] > key;
         if (rank < top) give(rank, key);
       }
-      if (S > 1)                                              // a slice of fewer logits than `top`
+      if (parts)                                              // a slice of fewer logits than `top`
         for (int i = min(n, held) + tid; i < top; i += kThreads) give(i, 0);
       return;
     }
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     }
     if (single >= 0) offer((float)x[single], single);
     below = block_reduce(best, s_redk, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-    if (tid == 0) give(k, below);                             // (S > 1: 0 where the slice has no more)
+    if (tid == 0) give(k, below);                             // (of parts: 0 where the slice has no more)
   }
 }
 
@@ -394,22 +401,113 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   }
 }
 
-hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
-  // slices: up to 1024 workgroups, four a CU, of at least 2048 logits
-  int S = 1;
-  if (a.ws && a.M < 512) {
-    S = (int)std::min<int64_t>({1024 / a.M, a.V / 2048, (int64_t)kMaxSlices});
-    const size_t per = (size_t)a.M * (sizeof(Sums) + 4 + (size_t)a.top * 8);
-    S = (int)std::max<size_t>(1, std::min<size_t>((size_t)std::max(S, 1), a.ws_bytes / per));
+// ---- beam_select ----
+// A workgroup of `blockDim / 64` waves per request. A wave takes a beam: its slices' sums and alternatives are joined as above,
+// into the beam's n best, score + (x - max) - log z in 64 bits (which of two beams' tokens comes first goes by that difference).
+// Then all beams' n best are ranked by counting, a beam's list only as far as it comes before the candidate. A beam that holds
+// nothing (a score that is no finite number) or whose row has no distribution has -inf for every token, a finished one its score
+// for `pad` and -inf for the others; equal candidates rank by beam, then by token.
+__global__ __launch_bounds__(512) void beam_join_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ finished,
+                                                       float* __restrict__ out_scores, int64_t* __restrict__ out_beams,
+                                                       int64_t* __restrict__ out_tokens, int W, int V, int n, int pad, int S,
+                                                       const Sums* __restrict__ part, const uint64_t* __restrict__ part_keys) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, req = blockIdx.x;
+  double* s_value = reinterpret_cast<double*>(smem);          // [W][n]
+  int* s_token = reinterpret_cast<int*>(s_value + W * n);     // (rounded up to a multiple of two)
+  uint64_t* s_keys = reinterpret_cast<uint64_t*>(s_token + ((W * n + 1) & ~1)) + wave * (S + min(S, n)) * n;
+  uint64_t* s_list = s_keys + S * n;
+  const int have = min(n, V);                                 // candidates of a beam
+  for (int w = wave; w < W; w += waves) {
+    const int64_t row = (int64_t)req * W + w;
+    const float score = scores[row];
+    const bool held = fabsf(score) <= FLT_MAX, done = held && finished && finished[row];
+    bool none = !held;
+    if (held && !done) {
+      const uint64_t* keys = part_keys + row * S * n;
+      for (int i = lane; i < S * n; i += 64) s_keys[i] = keys[i];
+      Sums s = lane < S ? part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};
+      const float m = wave_max(s.m);
+      move_sums(s.m, m, s.z, s.e);
+      const float z = wave_sum(s.z);
+      none = !(m > -INFINITY && m < INFINITY) || z != z;
+      lds_wave_order();
+      if (!none) {
+        const double at = (double)score - log((double)z);
+        const uint64_t first = lane < S ? s_keys[lane * n] : 0;
+        int above = 0;
+        for (int l = 0; l < S; ++l) above += s_keys[l * n] > first;
+        const uint64_t at_bound = __ballot(lane < S && above == n - 1);   // (keys are distinct; none where S < n)
+        const uint64_t bound = at_bound ? s_keys[__builtin_ctzll(at_bound) * n] : 0;
+        int mine = 0;
+        if (lane < S)
+          while (mine < n && s_keys[lane * n + mine] >= max(bound, (uint64_t)1)) ++mine;
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int o = __shfl_up(upto, off, 64);
+          if (lane >= off) upto += o;
+        }
+        for (int i = 0; i < mine; ++i) s_list[upto - mine + i] = s_keys[lane * n + i];
+        const int all = __shfl(upto, 63, 64);
+        lds_wave_order();
+        for (int i = lane; i < all; i += 64) {
+          const uint64_t key = s_list[i];
+          int rank = 0;
+          for (int k = 0; k < all; ++k) rank += s_list[k] > key;
+          if (rank >= n) continue;
+          s_value[w * n + rank] = at + ((double)order_value((uint32_t)(key >> 32)) - (double)m);
+          s_token[w * n + rank] = rank_index(key);
+        }
+      }
+    }
+    if (none || done) {
+      for (int i = lane; i < have; i += 64) {
+        s_value[w * n + i] = done && i == 0 ? (double)score : -INFINITY;
+        s_token[w * n + i] = !done ? i : i == 0 ? pad : i - 1 < pad ? i - 1 : i;
+      }
+    }
   }
-  const int each = a.dtype == 0 ? 4 : 8;                      // logits of a vector
-  const int64_t vectors = (a.V / each + S - 1) / S, steps = (vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-  const size_t lds = (size_t)std::max<int64_t>(1, std::min<int64_t>(steps, kGroups)) * kThreads * sizeof(float);
+  __syncthreads();
+  for (int c = threadIdx.x; c < W * have; c += blockDim.x) {
+    const int w = c / have, i = c - w * have;
+    const double v = s_value[w * n + i];
+    int rank = i;                                             // (a beam's own list is in order)
+    for (int o = 0; o < W && rank < n; ++o) {
+      if (o == w) continue;
+      const double* theirs = s_value + o * n;
+      for (int k = 0; k < have && rank < n && (theirs[k] > v || (theirs[k] == v && o < w)); ++k) ++rank;
+    }
+    if (rank >= n) continue;
+    const int64_t to = (int64_t)req * n + rank;
+    out_scores[to] = (float)v;
+    out_beams[to] = w;
+    out_tokens[to] = s_token[w * n + i];
+  }
+}
+
+// slices: up to 1024 workgroups, four a CU, of at least 2048 logits
+static int row_slices(int M, int V, int top, size_t ws_bytes) {
+  const int S = M < 512 ? (int)std::min<int64_t>({1024 / M, V / 2048, (int64_t)kMaxSlices}) : 1;
+  const size_t per = (size_t)M * (sizeof(Sums) + 4 + (size_t)top * 8);
+  return (int)std::max<size_t>(1, std::min<size_t>((size_t)std::max(S, 1), ws_bytes / per));
+}
+// LDS of a slice's group maxima
+static size_t slice_lds(int V, int dtype, int S) {
+  const int each = dtype == 0 ? 4 : 8;                        // logits of a vector
+  const int64_t vectors = (V / each + S - 1) / S, steps = (vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  return (size_t)std::max<int64_t>(1, std::min<int64_t>(steps, kGroups)) * kThreads * sizeof(float);
+}
+
+hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
+  const int S = a.ws ? row_slices(a.M, a.V, a.top, a.ws_bytes) : 1;
+  const size_t lds = slice_lds(a.V, a.dtype, S);
   uint64_t* keys = static_cast<uint64_t*>(a.ws);              // [M][S][top] keys, then [M][S] sums
   Sums* part = reinterpret_cast<Sums*>(keys + (size_t)a.M * S * a.top);
   auto go = [&](auto first, auto second, auto* p) {
     hipError_t e = launch(first, dim3((unsigned)((int64_t)a.M * S)), dim3(kThreads), lds, st, p, a.stride, a.targets, a.logprob,
-                          a.entropy, a.top_value, a.top_id, a.V, a.top, S, part, keys);
+                          a.entropy, a.top_value, a.top_id, a.V, a.top, S, part, keys, static_cast<const float*>(nullptr),
+                          static_cast<const uint8_t*>(nullptr));
     if (e != hipSuccess || S == 1) return e;
     return launch(second, dim3((unsigned)a.M), dim3(256), 0, st, p, a.stride, a.targets, a.logprob, a.entropy, a.top_value,
                   a.top_id, a.V, a.top, S, part, keys);
@@ -417,6 +515,33 @@ hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
   if (a.dtype == 0) return go(logprobs_kernel<float>, logprobs_join_kernel<float>, static_cast<const float*>(a.logits));
   if (a.dtype == 1) return go(logprobs_kernel<f16>, logprobs_join_kernel<f16>, static_cast<const f16*>(a.logits));
   return go(logprobs_kernel<bf16>, logprobs_join_kernel<bf16>, static_cast<const bf16*>(a.logits));
+}
+
+hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st) {
+  const int M = a.requests * a.beams, S = row_slices(M, a.V, a.n, a.ws_bytes);
+  const size_t lds = slice_lds(a.V, a.dtype, S);
+  uint64_t* keys = static_cast<uint64_t*>(a.ws);              // [M][S][n] keys, then [M][S] sums
+  Sums* part = reinterpret_cast<Sums*>(keys + (size_t)M * S * a.n);
+  auto go = [&](auto first, auto* p) {
+    return launch(first, dim3((unsigned)((int64_t)M * S)), dim3(kThreads), lds, st, p, a.stride,
+                  static_cast<const int64_t*>(nullptr), static_cast<float*>(nullptr), static_cast<float*>(nullptr),
+                  static_cast<float*>(nullptr), static_cast<int64_t*>(nullptr), a.V, a.n, S, part, keys, a.scores, a.finished);
+  };
+  hipError_t e = a.dtype == 0   ? go(logprobs_kernel<float>, static_cast<const float*>(a.logits))
+                 : a.dtype == 1 ? go(logprobs_kernel<f16>, static_cast<const f16*>(a.logits))
+                                : go(logprobs_kernel<bf16>, static_cast<const bf16*>(a.logits));
+  if (e != hipSuccess) return e;
+  // waves: as many beams at once as LDS holds the lists of
+  const size_t fixed = (size_t)a.beams * a.n * 12 + 8, each = (size_t)(S + std::min(S, a.n)) * a.n * 8;
+  const int waves = (int)std::max<size_t>(1, std::min<size_t>({(size_t)8, (size_t)a.beams, (140 * 1024 - fixed) / each}));
+  const size_t join_lds = fixed + waves * each;
+  if (join_lds > 65536) {
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_lds_once(done, beam_join_kernel, 141 * 1024))) return e;
+  }
+  return launch(beam_join_kernel, dim3((unsigned)a.requests), dim3(64 * waves), join_lds, st, a.scores, a.finished, a.out_scores,
+                a.out_beams, a.out_tokens, a.beams, a.V, a.n, a.pad, S, static_cast<const Sums*>(part),
+                static_cast<const uint64_t*>(keys));
 }
 
 }  // namespace lowbit

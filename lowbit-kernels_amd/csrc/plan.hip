@@ -1,0 +1,512 @@
+// The tables of a batch's step over a paged KV cache, built on the GPU from its sequences' lengths (plan_paged), and what becomes
+// of a tree of drafted tokens once the model has picked its own (accept_drafts). Both are whole numbers and copies of rows of the
+// cache; a step of a captured graph runs them without the host.
+//
+// plan_paged. Sequence b goes on from row r = rows[b] of the table: its past[r] keys lie in the row's first ceil(past / page
+// size) pages, which it keeps. A page is in use while a sequence keeps it, free otherwise: no counts are carried from step to
+// step, so nothing leaks when a sequence ends, a draft is rejected or a beam gives way. The free pages, in order, go to the
+// sequences, in order. A page that a sequence is about to write (its last one, partly filled) and that another one reads is
+// replaced by a copy first; of several sequences that could write it, the one with the most keys, then the first, keeps it.
+#include "paged_attention.hpp"
+
+namespace lowbit {
+
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kWordsPer = 8;             // bitmap words of a thread in one step of the search for free pages
+// what one workgroup plans alone, its state in LDS
+constexpr int kSmallSeqs = 1024, kSmallTokens = 4096, kSmallList = kSmallTokens / 16 + 2 * kSmallSeqs;
+constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 16;
+
+// One sequence: its row of the table and keys there (none: a row outside the table), its new tokens as far as the call's T
+// reaches, its pages kept, and in all (`need`: those the row has place for).
+struct PlanSeq {
+  int row, past, fresh;
+};
+// The state of a call, in LDS or in the workspace: [B] each but start (as q_starts, [B + 1])
+struct PlanState {
+  int *row, *past, *fresh, *tail, *off, *start;   // tail: the last page kept; off: its first place in the list, ~off if that is a copy
+  uint32_t *held, *whole;                         // a bit a page: kept by a sequence; kept and full
+  int* hash_page;                                 // the pages that are partly filled, and whose they are (owner_key)
+  uint64_t* hash_owner;
+  int hash_mask;
+  int* list;                                      // the free pages handed out, -1 where they ran out
+  int list_cap;
+};
+
+__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int shift, int b) {
+  PlanSeq s;
+  s.row = a.rows ? a.rows[b] : b;
+  s.past = s.row >= 0 && s.row < a.R ? min(max(a.past[s.row], 0), a.width << shift) : 0;
+  s.fresh = min(max(a.fresh[b], 0), a.T);
+  return s;
+}
+__device__ __forceinline__ int pages_of(int keys, int shift) { return (keys + (1 << shift) - 1) >> shift; }
+
+// of the sequences that hold a partly filled page: the most keys, then one that writes, then the first
+__device__ __forceinline__ uint64_t owner_key(int past, int fresh, int b) {
+  return ((uint64_t)(uint32_t)past << 32) | (fresh > 0 ? 0x80000000u : 0u) | (uint32_t)(0x7FFFFFFF - b);
+}
+__device__ __forceinline__ int hash_slot(int page, int mask) { return (int)(((uint32_t)page * 2654435761u) >> 7) & mask; }
+
+// entry c of sequence b's row, a page that it keeps
+__device__ __forceinline__ void mark(const PlanState& s, int64_t pages, int shift, int b, int c, int page) {
+  const int past = s.past[b];
+  const bool last = c == pages_of(past, shift) - 1, part = last && (past & ((1 << shift) - 1));
+  if (last) s.tail[b] = page;
+  if (page < 0 || page >= pages) return;
+  atomicOr(s.held + (page >> 5), 1u << (page & 31));
+  if (!part) {
+    atomicOr(s.whole + (page >> 5), 1u << (page & 31));
+    return;
+  }
+  for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask) {   // (twice as many places as sequences)
+    const int was = atomicCAS(s.hash_page + at, -1, page);
+    if (was != -1 && was != page) continue;
+    atomicMax(reinterpret_cast<unsigned long long*>(s.hash_owner) + at, (unsigned long long)owner_key(past, s.fresh[b], b));
+    break;
+  }
+}
+
+// whether sequence b needs a copy of its last page
+__device__ __forceinline__ bool needs_copy(const PlanState& s, int64_t pages, int shift, int b) {
+  const int past = s.past[b], page = s.tail[b];
+  if (!(past & ((1 << shift) - 1)) || s.fresh[b] <= 0 || page < 0 || page >= pages) return false;
+  if (s.whole[page >> 5] >> (page & 31) & 1u) return true;
+  for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask)
+    if (s.hash_page[at] == page) return s.hash_owner[at] != owner_key(past, s.fresh[b], b);
+}
+
+// the sum of the threads' values up to and including this one's, held at `most`; *all: of all threads (values 0 .. most)
+__device__ __forceinline__ int block_scan(int v, int most, int* s_wave, int* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(v, off, 64);
+    if (lane >= off) v = min(v + o, most);
+  }
+  __syncthreads();
+  if (lane == 63) s_wave[wave] = v;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    before = w < wave ? min(before + s_wave[w], most) : before;
+    sum = min(sum + s_wave[w], most);
+  }
+  *all = sum;
+  return min(before + v, most);
+}
+
+// q_starts, kv_lens and the sequences' lengths, by one workgroup
+__device__ __forceinline__ void plan_lens(const PlanArgs& a, const PlanState& s, int shift, int* s_wave) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    PlanSeq q{-1, 0, 0};
+    if (b < a.B) q = plan_seq(a, shift, b);
+    int all;
+    const int upto = min(before + block_scan(q.fresh, a.T, s_wave, &all), a.T);
+    if (b < a.B) {
+      s.start[b + 1] = upto;                                  // (held at T: tokens past it are left out)
+      a.q_starts[b + 1] = upto;
+      s.row[b] = q.row;
+      s.past[b] = q.past;
+    }
+    if (b == 0) {
+      s.start[0] = 0;
+      a.q_starts[0] = 0;
+    }
+    __syncthreads();
+    if (b < a.B) {
+      const int fresh = s.start[b + 1] - s.start[b];
+      s.fresh[b] = fresh;
+      s.tail[b] = -1;
+      a.kv_lens[b] = q.past + fresh;
+    }
+    before = min(before + all, a.T);
+  }
+}
+
+// which sequences get how many of the free pages, and which pages those are, by one workgroup
+__device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, int* s_wave) {
+  int total = 0, over = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    int want = 0, past_width = 0;                             // pages; those that the table has no place for
+    bool copy = false;
+    if (b < a.B) {
+      const int past = s.past[b], have = pages_of(past, shift), need = pages_of(past + s.fresh[b], shift);
+      copy = needs_copy(s, a.pages, shift, b);
+      want = min(need, a.width) - have + (copy ? 1 : 0);
+      past_width = max(need - a.width, 0);
+    }
+    int all;
+    const int upto = block_scan(want, INT_MAX / 2, s_wave, &all);
+    if (b < a.B) s.off[b] = copy ? ~(total + upto - want) : total + upto - want;
+    total += all;
+    block_scan(past_width, INT_MAX / 2, s_wave, &all);
+    over += all;
+  }
+  total = min(total, s.list_cap);
+  const int words = (int)((a.pages + 31) >> 5);
+  int found = 0;
+  for (int w0 = 0; w0 < words && found < total; w0 += kThreads * kWordsPer) {
+    uint32_t free[kWordsPer];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kWordsPer; ++i) {
+      const int w = w0 + (int)threadIdx.x * kWordsPer + i;
+      const int64_t left = a.pages - 32 * (int64_t)w;
+      free[i] = w < words ? ~s.held[w] & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
+      n += __popc(free[i]);
+    }
+    int all;
+    int at = found + block_scan(n, INT_MAX / 2, s_wave, &all) - n;
+#pragma unroll
+    for (int i = 0; i < kWordsPer; ++i)
+      for (uint32_t f = free[i]; f && at < total; f &= f - 1, ++at)
+        s.list[at] = 32 * (w0 + (int)threadIdx.x * kWordsPer + i) + __ffs(f) - 1;
+    found = min(found + all, total);
+  }
+  for (int i = found + threadIdx.x; i < total; i += kThreads) s.list[i] = -1;
+  if (threadIdx.x == 0) {
+    *a.missing = over + total - found;
+    s.off[a.B] = total;
+  }
+}
+
+// the last b with of(b) <= v, of not falling and of(0) <= v
+template <typename F>
+__device__ __forceinline__ int last_at(int n, int v, F of) {
+  int lo = 0;
+  for (int hi = n; hi - lo > 1;) {
+    const int mid = (lo + hi) >> 1;
+    if (of(mid) <= v)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ int off_of(int v) { return v < 0 ? ~v : v; }
+
+// place j of the list: into the table
+__device__ __forceinline__ void give_page(const PlanArgs& a, const PlanState& s, int shift, int j) {
+  const int b = last_at(a.B, j, [&](int i) { return off_of(s.off[i]); });
+  const int off = s.off[b], first = off_of(off), have = pages_of(s.past[b], shift);
+  a.table_out[(int64_t)b * a.width + have + (j - first) - (off < 0 ? 1 : 0)] = s.list[j];
+}
+__device__ __forceinline__ void give_copy(const PlanArgs& a, const PlanState& s, int b) {
+  const bool copy = s.off[b] < 0;
+  a.copies[2 * b] = copy ? s.tail[b] : -1;
+  a.copies[2 * b + 1] = copy ? s.list[~s.off[b]] : -1;
+}
+
+// token t's position, slot and mask; parent: of node i of its sequence
+template <typename P>
+__device__ __forceinline__ void give_token(const PlanArgs& a, const PlanState& s, int shift, int t, P parent) {
+  if (t >= s.start[a.B]) {                                    // (a padded token)
+    a.positions[t] = 0;
+    a.slots[t] = -1;
+    for (int w = 0; w < a.words; ++w) a.masks[(int64_t)t * a.words + w] = 0;
+    return;
+  }
+  const int b = last_at(a.B, t, [&](int i) { return s.start[i]; });
+  const int first = s.start[b], i = t - first, past = s.past[b], key = past + i;
+  const int have = pages_of(past, shift), off = s.off[b], c = key >> shift;
+  int page = -1;
+  if (c < have && off >= 0)
+    page = s.tail[b];                                         // (key >= past: of the pages kept, the last)
+  else if (c < a.width)
+    page = s.list[off_of(off) + c - have + (off < 0 ? 1 : 0)];
+  a.slots[t] = page >= 0 && page < a.pages ? ((int64_t)page << shift) + (key & ((1 << shift) - 1)) : -1;
+  if (!a.parents) {
+    a.positions[t] = key;
+    return;
+  }
+  // up to the root, once a word
+  int depth = 0;
+  for (int w = 0; w < a.words; ++w) {
+    uint64_t bits = 0;
+    depth = 0;
+    for (int n = i;;) {
+      if (n >> 6 == w) bits |= (uint64_t)1 << (n & 63);
+      const int p = parent(first, n);
+      if (p < 0 || p >= n) break;                             // (a node hangs below an earlier one)
+      n = p;
+      ++depth;
+    }
+    a.masks[(int64_t)t * a.words + w] = bits;
+  }
+  a.positions[t] = past + depth;
+}
+
+}  // namespace
+
+// The whole plan by one workgroup.
+__global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, FastDiv by_width, int shift, int hash_mask) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
+  __shared__ int s_wave[kThreads / 64];
+  const int tid = threadIdx.x, words = ((int)((a.pages + 31) >> 5) + 3) & ~3;
+  PlanState s;
+  s.hash_mask = hash_mask;
+  s.list_cap = kSmallList;
+  s.hash_owner = reinterpret_cast<uint64_t*>(s_plan);
+  s.held = reinterpret_cast<uint32_t*>(s.hash_owner + hash_mask + 1);
+  s.whole = s.held + words;
+  s.hash_page = reinterpret_cast<int*>(s.whole + words);
+  s.row = s.hash_page + hash_mask + 1;
+  s.past = s.row + a.B;
+  s.fresh = s.past + a.B;
+  s.tail = s.fresh + a.B;
+  s.off = s.tail + a.B;
+  s.start = s.off + a.B + 1;
+  s.list = s.start + a.B + 1;
+  int* s_parent = s.list + kSmallList;
+  plan_lens(a, s, shift, s_wave);
+  for (int i = tid; i < 2 * (hash_mask + 1) + 2 * words; i += kThreads) s_plan[i] = 0;
+  for (int i = tid; i <= hash_mask; i += kThreads) s.hash_page[i] = -1;
+  if (a.parents)
+    for (int i = tid; i < a.T; i += kThreads) s_parent[i] = a.parents[i];
+  __syncthreads();
+  const int entries = a.B * a.width;
+  const bool other = a.table_out != a.table;
+  constexpr int kAhead = 4;
+  for (int i0 = tid; i0 < entries; i0 += kAhead * kThreads) {
+    int page[kAhead], b[kAhead], c[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u * kThreads, entries - 1);
+      b[u] = div(i, by_width);
+      c[u] = i - b[u] * a.width;
+      page[u] = -1;
+      if (c[u] < pages_of(s.past[b[u]], shift)) page[u] = a.table[(int64_t)s.row[b[u]] * a.width + c[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u * kThreads >= entries) break;
+      if (c[u] < pages_of(s.past[b[u]], shift)) mark(s, a.pages, shift, b[u], c[u], page[u]);
+      if (other) a.table_out[i0 + u * kThreads] = page[u];
+    }
+  }
+  __syncthreads();
+  plan_assign(a, s, shift, s_wave);
+  __syncthreads();
+  for (int j = tid; j < s.off[a.B]; j += kThreads) give_page(a, s, shift, j);
+  for (int b = tid; b < a.B; b += kThreads) give_copy(a, s, b);
+  for (int t = tid; t < a.T; t += kThreads) give_token(a, s, shift, t, [&](int first, int n) { return s_parent[first + n]; });
+}
+
+// The same in four launches, the state in the workspace: the lengths beside the clearing of the bitmaps; the pages kept; the
+// pages handed out; tables and tokens.
+__global__ __launch_bounds__(kThreads) void plan_lens_kernel(PlanArgs a, PlanState s, int shift, int words) {
+  __shared__ int s_wave[kThreads / 64];
+  if (blockIdx.x == 0) {
+    plan_lens(a, s, shift, s_wave);
+    return;
+  }
+  const int64_t n = 2 * (int64_t)(s.hash_mask + 1) + 2 * (int64_t)words, step = (int64_t)(gridDim.x - 1) * kThreads;
+  const int64_t at = (int64_t)(blockIdx.x - 1) * kThreads + threadIdx.x;
+  uint32_t* zero = reinterpret_cast<uint32_t*>(s.hash_owner);   // the bitmaps follow the owners
+  for (int64_t i = at; i < n; i += step) zero[i] = 0;
+  for (int64_t i = at; i <= s.hash_mask; i += step) s.hash_page[i] = -1;
+}
+
+__global__ __launch_bounds__(256) void plan_mark_kernel(PlanArgs a, PlanState s, FastDiv by_width, int shift) {
+  const int entries = a.B * a.width, step = gridDim.x * 256;
+  const bool other = a.table_out != a.table;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < entries; i += step) {
+    const int b = div(i, by_width), c = i - b * a.width;
+    int page = -1;
+    if (c < pages_of(s.past[b], shift)) {
+      page = a.table[(int64_t)s.row[b] * a.width + c];
+      mark(s, a.pages, shift, b, c, page);
+    }
+    if (other) a.table_out[i] = page;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanState s, int shift) {
+  __shared__ int s_wave[kThreads / 64];
+  plan_assign(a, s, shift, s_wave);
+}
+
+__global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s, int shift) {
+  const int step = gridDim.x * 256, at = blockIdx.x * 256 + threadIdx.x;
+  const int total = s.off[a.B];
+  for (int j = at; j < total; j += step) give_page(a, s, shift, j);
+  for (int b = at; b < a.B; b += step) give_copy(a, s, b);
+  for (int t = at; t < a.T; t += step)
+    give_token(a, s, shift, t, [&](int first, int n) { return a.parents[first + n]; });
+}
+
+// Workgroup (sequence, layer): the filled rows of the page that is replaced, every head of k and v.
+__global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ copies, const int* __restrict__ q_starts,
+                                                        const int* __restrict__ kv_lens, uint8_t* __restrict__ k,
+                                                        uint8_t* __restrict__ v, int64_t pages, int Hkv, int row_bytes, int shift) {
+  const int b = blockIdx.x, src = copies[2 * b], dst = copies[2 * b + 1];
+  if (src < 0 || dst < 0) return;
+  const int rows = (kv_lens[b] - (q_starts[b + 1] - q_starts[b])) & ((1 << shift) - 1);
+  const int64_t head = (int64_t)row_bytes << shift, page = head * Hkv, layer = (int64_t)blockIdx.y * pages;
+  const int vec = rows * (row_bytes / 16), n = vec * Hkv;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int h = i / vec, at = i - h * vec;
+    const int64_t from = (layer + src) * page + h * head + 16 * (int64_t)at, to = (layer + dst) * page + h * head + 16 * (int64_t)at;
+    const u32x4 x = load16(k + from), y = load16(v + from);
+    *reinterpret_cast<u32x4*>(k + to) = x;
+    *reinterpret_cast<u32x4*>(v + to) = y;
+  }
+}
+
+// accept_drafts. Workgroup (sequence, layer): its first wave follows the picks from node 0 down the tree, then the workgroup moves
+// the confirmed nodes' rows of its layer, every head of k and v, to the places behind the sequence's keys. Node d of the path
+// comes to lie at place d <= the node's own, so rows are read and written in order of the path, a chunk's all read before one is
+// written.
+constexpr int kMostPath = 1024;
+__global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
+  __shared__ int s_path[kMostPath];
+  __shared__ int s_count;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int first = min(max(a.q_starts[b], 0), a.T), new_all = min(max(a.q_starts[b + 1], first), a.T) - first;
+  const int past = a.kv_lens[b] - new_all;
+  if (tid < 64) {
+    const int64_t* tokens = a.tokens + first;
+    const int64_t* picks = a.picks + first;
+    const int* parents = a.parents ? a.parents + first : nullptr;
+    int count = 0, cur = 0;
+    while (count < a.longest && cur < new_all) {
+      if (lane == 0) s_path[count] = cur;
+      ++count;
+      const int64_t want = picks[cur];
+      int next = new_all;
+      for (int n0 = cur + 1; n0 < new_all && next == new_all; n0 += 64) {
+        const int n = n0 + lane;
+        const bool hit = n < new_all && (parents ? parents[n] : n - 1) == cur && tokens[n] == want;
+        const uint64_t any = __ballot(hit);
+        if (any) next = n0 + __builtin_ctzll(any);
+        if (!parents) break;                                  // (a chain: the next token or none)
+      }
+      cur = next;
+    }
+    if (lane == 0) s_count = count;
+    if (blockIdx.y == 0) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int d = lane; d < a.longest; d += 64) {
+        const int n = d < count ? s_path[d] : -1;
+        a.path[(int64_t)b * a.longest + d] = n;
+        a.accepted[(int64_t)b * a.longest + d] = n < 0 ? -1 : picks[n];   // (a confirmed node's token is its parent's pick)
+      }
+      if (lane == 0) {
+        a.counts[b] = count;
+        a.lens[b] = past + count;
+      }
+    }
+  }
+  __syncthreads();
+  const int count = s_count;
+  if (!a.k || count == 0 || s_path[count - 1] == count - 1) return;   // (a path that is in its place, as every chain's is)
+  const int pieces = a.row_bytes / 16, heads = 2 * a.Hkv;
+  const int64_t head = (int64_t)a.row_bytes << shift, page = head * a.Hkv, layer = (int64_t)blockIdx.y * a.pages;
+  const int* table = a.table + (int64_t)b * a.width;
+  // where key `key` lies in this layer, below 0: nowhere
+  auto place = [&](int key) -> int64_t {
+    const int c = key >> shift;
+    if (key < 0 || c >= a.width) return -1;
+    const int id = table[c];
+    return id < 0 || id >= a.pages ? -1 : (layer + id) * page + (int64_t)(key & ((1 << shift) - 1)) * a.row_bytes;
+  };
+  constexpr int kHeld = 8;                                    // pieces of a thread in a chunk
+  const int rows = min(count, kHeld * 256 / pieces), together = max(1, kHeld * 256 / pieces / rows);
+  for (int h0 = 0; h0 < heads; h0 += together)
+    for (int d0 = 0; d0 < count; d0 += rows) {
+      const int n = min(rows, count - d0), items = n * pieces * min(together, heads - h0);
+      u32x4 held[kHeld];
+      int64_t to[kHeld];
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int i = tid + 256 * u, r = i / pieces, hv = h0 + r / n, d = d0 + r % n;
+        to[u] = -1;
+        if (i >= items || s_path[d] == d) continue;
+        const int64_t src = place(past + s_path[d]), dst = place(past + d);
+        if (src < 0 || dst < 0) continue;
+        const int64_t at = (int64_t)(hv >> 1) * head + 16 * (i % pieces);
+        held[u] = load16((hv & 1 ? a.v : a.k) + src + at);
+        to[u] = 2 * (dst + at) + (hv & 1);
+      }
+      vm_drain();
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (to[u] >= 0) *reinterpret_cast<u32x4*>((to[u] & 1 ? a.v : a.k) + (to[u] >> 1)) = held[u];
+      __syncthreads();
+    }
+}
+
+namespace {
+
+bool plan_is_small(const PlanArgs& a) {
+  return a.B <= kSmallSeqs && a.T <= kSmallTokens && a.pages <= kSmallPages && (int64_t)a.B * a.width <= kSmallEntries;
+}
+int hash_places(int B) {
+  int n = 64;
+  while (n < 2 * B) n *= 2;
+  return n;
+}
+int64_t map_words(int64_t pages) { return ((pages + 31) / 32 + 3) & ~(int64_t)3; }
+int64_t list_places(const PlanArgs& a, int shift) { return (a.T >> shift) + 2 * (int64_t)a.B + 1; }
+
+}  // namespace
+
+size_t plan_paged_workspace(const PlanArgs& a) {
+  if (plan_is_small(a)) return 0;
+  const int64_t ints = 3 * (int64_t)hash_places(a.B) + 2 * map_words(a.pages) + 6 * (int64_t)a.B + 2 + list_places(a, log2_of(a.page_size));
+  return (size_t)(4 * ints + 15) / 16 * 16;
+}
+
+hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
+  const int shift = log2_of(a.page_size), places = hash_places(a.B);
+  const FastDiv by_width = fast_div(a.width);
+  hipError_t e;
+  if (plan_is_small(a)) {
+    const size_t words = (size_t)map_words(a.pages);
+    const size_t lds = 4 * (3 * (size_t)places + 2 * words + 6 * (size_t)a.B + 2 + kSmallList + kSmallTokens);
+    static_assert(4 * (3 * 2 * kSmallSeqs + 2 * kSmallPages / 32 + 6 * kSmallSeqs + 2 + kSmallList + kSmallTokens) < 160 * 1024 - 256, "LDS");
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_lds_once(done, plan_small_kernel, 160 * 1024 - 256))) return e;
+    e = launch(plan_small_kernel, dim3(1), dim3(kThreads), lds, st, a, by_width, shift, places - 1);
+  } else {
+    PlanState s;
+    s.hash_mask = places - 1;
+    s.hash_owner = static_cast<uint64_t*>(a.ws);
+    s.held = reinterpret_cast<uint32_t*>(s.hash_owner + places);
+    const int64_t words = map_words(a.pages);
+    s.whole = s.held + words;
+    s.hash_page = reinterpret_cast<int*>(s.whole + words);
+    s.row = s.hash_page + places;
+    s.past = s.row + a.B;
+    s.fresh = s.past + a.B;
+    s.tail = s.fresh + a.B;
+    s.off = s.tail + a.B;
+    s.start = s.off + a.B + 1;
+    s.list = s.start + a.B + 1;
+    s.list_cap = (int)list_places(a, shift);
+    const int64_t clear = (2 * (int64_t)places + 2 * words + kThreads - 1) / kThreads;
+    e = launch(plan_lens_kernel, dim3((unsigned)(1 + std::min<int64_t>(clear, 512))), dim3(kThreads), 0, st, a, s, shift, (int)words);
+    const int64_t entries = (int64_t)a.B * a.width;
+    if (e == hipSuccess)
+      e = launch(plan_mark_kernel, dim3((unsigned)std::min<int64_t>((entries + 255) / 256, 4096)), dim3(256), 0, st, a, s, by_width, shift);
+    if (e == hipSuccess) e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), 0, st, a, s, shift);
+    const int64_t items = std::max<int64_t>({(int64_t)a.T, (int64_t)a.B, 1});
+    if (e == hipSuccess) e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256), 0, st, a, s, shift);
+  }
+  if (e != hipSuccess || !a.k) return e;
+  return launch(plan_copy_kernel, dim3((unsigned)a.B, (unsigned)a.layers), dim3(256), 0, st, static_cast<const int*>(a.copies),
+                static_cast<const int*>(a.q_starts), static_cast<const int*>(a.kv_lens), a.k, a.v, a.pages, a.Hkv, a.row_bytes, shift);
+}
+
+hipError_t accept_drafts_launch(const AcceptArgs& a, hipStream_t st) {
+  return launch(accept_kernel, dim3((unsigned)a.B, (unsigned)(a.k ? a.layers : 1)), dim3(256), 0, st, a, log2_of(a.page_size));
+}
+
+}  // namespace lowbit

@@ -6,6 +6,7 @@ row_tiles=0), w4_dequant(w, s, group, mma_layout=False). Like the reference they
 output with torch.empty on the input's device, launch on that device's current stream and raise RuntimeError on any
 refusal (the reference's TORCH_CHECK messages). There is no fallback: without the built library every call raises.
 """
+import collections
 import ctypes
 import functools
 import os
@@ -69,6 +70,15 @@ SIGNATURES = {
     "lowbit_attention_paged": ([_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                 _i64, _i64, ctypes.c_float, _vp, ctypes.c_size_t, _vp], _int),
     "lowbit_attention_paged_workspace": ([_i64] * 9, ctypes.c_size_t),
+    "lowbit_attention_paged_tree": ([_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+                                     _i64, _i64, _i64, _i64, ctypes.c_float, _vp, ctypes.c_size_t, _vp], _int),
+    "lowbit_plan_paged_workspace": ([_i64] * 5, ctypes.c_size_t),
+    "lowbit_plan_paged": ([_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                           _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp], _int),
+    "lowbit_accept_drafts": ([_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                              _i64, _i64, _i64, _vp], _int),
+    "lowbit_beam_select": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp],
+                           _int),
     "lowbit_token_logprobs": ([_vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, ctypes.c_size_t, _vp],
                               _int),
     "lowbit_hbm_read": ([_vp, _i64, _vp, _i64, _vp], _int),
@@ -298,6 +308,11 @@ def _launch(index, call, nbytes=0, own=False):
         check(rc)
 
 
+# plan_paged's answer (its docstring says what each holds)
+PagedStep = collections.namedtuple("PagedStep", "page_table q_starts kv_lens positions slots masks copies missing")
+MAX_MASK_WORDS = 16                     # of a token's tree mask: trees of up to 1024 nodes
+
+
 class NativeExt:
     """The reference's extension surface (w4_gemv / w4_gemm_tc / w4_dequant) on the gfx950 library."""
 
@@ -307,6 +322,7 @@ class NativeExt:
         self.lib = lib()
         # (of sizes alone, and every layer of a step asks for the same ones)
         self._paged_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_attention_paged_workspace)
+        self._plan_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_plan_paged_workspace)
 
     def w4_gemv(self, x, w, s, group, version, rows_per_warp=0):
         m, n, k, index = _check_tensors(x, w, s, group)
@@ -686,8 +702,9 @@ class NativeExt:
                                                ptr(inv_freq), ptr(q_out), ptr(k_cache), ptr(v_cache), hq, hkv,
                                                k_cache.shape[1], _stream(x.device)))
 
-    # ---- a batch of sequences over a paged cache (lowbit_norm_rope_paged, lowbit_attention_paged), and what logits say of
-    # given tokens (lowbit_token_logprobs) ----
+    # ---- a batch of sequences over a paged cache (lowbit_norm_rope_paged, lowbit_attention_paged), its tables (lowbit_plan_paged),
+    # trees of drafts (lowbit_attention_paged_tree, lowbit_accept_drafts), and what logits say of given tokens
+    # (lowbit_token_logprobs) or of beams (lowbit_beam_select) ----
 
     def _paged_dtype(self, t):
         if t.dtype is torch.float16:
@@ -742,6 +759,18 @@ class NativeExt:
         page_table[b] (int32 [B, width]) of the caches [pages, hkv, page_size, D]. Rows of no sequence are not touched, rows
         left without a key are zeros. max_new, max_keys: bounds on a sequence's new tokens and keys, which size the launch.
         split=False keeps every row's keys in one workgroup, without a workspace."""
+        self._attend_pages(q, k_cache, v_cache, page_table, q_starts, kv_lens, None, out, max_new, max_keys, scale, split)
+
+    def attention_paged_tree(self, q, k_cache, v_cache, page_table, q_starts, kv_lens, masks, out, max_new, max_keys, scale,
+                             split=True):
+        """attention_paged where the new tokens are trees of drafts: masks (int64 [T, words], plan_paged's) has a bit for every new
+        token of the row's sequence that the row attends (bit j % 64 of word j // 64 for new token j; its own only if set), beside
+        all keys before the new ones. words is 1..16; rows that attend nothing are zeros."""
+        if masks.dim() != 2 or not 1 <= masks.shape[1] <= MAX_MASK_WORDS:
+            raise RuntimeError(f"masks must be [T, words] with 1..{MAX_MASK_WORDS} words, got {list(masks.shape)}")
+        self._attend_pages(q, k_cache, v_cache, page_table, q_starts, kv_lens, masks, out, max_new, max_keys, scale, split)
+
+    def _attend_pages(self, q, k_cache, v_cache, page_table, q_starts, kv_lens, masks, out, max_new, max_keys, scale, split):
         if not q.is_cuda or q.dim() != 3 or k_cache.dim() != 4 or page_table.dim() != 2:
             raise RuntimeError("q [T, Hq, D], the caches [pages, Hkv, page_size, D] and page_table [B, width] must be CUDA tensors")
         dtype, index = self._paged_dtype(q), q.get_device()
@@ -754,6 +783,8 @@ class NativeExt:
         _need_fast(page_table, "page_table", torch.int32, (batch, width), index, device)
         _need_fast(q_starts, "q_starts", torch.int32, (batch + 1,), index, device)
         _need_fast(kv_lens, "kv_lens", torch.int32, (batch,), index, device)
+        if masks is not None:
+            _need_fast(masks, "masks", torch.int64, (t, masks.shape[1]), index, device)
         pages, page_size = self._check_pages(k_cache, v_cache, q, hkv, dim)
         if t == 0 or batch == 0:
             return
@@ -761,10 +792,155 @@ class NativeExt:
         # graphs share none
         nbytes = self._paged_workspace(t, batch, hq, hkv, dim, width, page_size, int(max_new), int(max_keys)) if split else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        if masks is not None:
+            _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged_tree(
+                q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),
+                kv_lens.data_ptr(), masks.data_ptr(), masks.shape[1], out.data_ptr(), t, batch, hq, hkv, dim, pages, page_size,
+                int(max_new), int(max_keys), float(scale), ws.data_ptr() if nbytes else None, nbytes, stream))
+            return
         _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged(
             q.data_ptr(), dtype, k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), width, q_starts.data_ptr(),
             kv_lens.data_ptr(), out.data_ptr(), t, batch, hq, hkv, dim, pages, page_size, int(max_new), int(max_keys),
             float(scale), ws.data_ptr() if nbytes else None, nbytes, stream))
+
+    def _check_layers(self, caches, pages, page_size, index):
+        """(k, v) [layers, pages, hkv, page_size, D] (or [pages, ...], one layer) of one 2-byte type, or None; returns (layers,
+        hkv, bytes of a row)."""
+        if caches is None:
+            return 0, 0, 0
+        k, v = caches
+        shape = k.shape
+        if len(shape) not in (4, 5) or v.shape != shape or (pages is not None and (shape[-4], shape[-2]) != (pages, page_size)):
+            want = "page_size" if pages is None else f"{pages}, hkv, {page_size}"
+            raise RuntimeError(f"the caches must be [layers, {'pages, hkv, ' if pages is None else ''}{want}, D], got "
+                               f"{list(shape)} and {list(v.shape)}")
+        for t in caches:
+            if t.dtype not in (torch.float16, torch.bfloat16) or t.dtype is not k.dtype or not t.is_contiguous() or \
+                    t.get_device() != index:
+                raise RuntimeError("the caches must be contiguous float16 or bfloat16 tensors on the same GPU")
+        return (shape[0] if len(shape) == 5 else 1), shape[-3], 2 * shape[-1]
+
+    def plan_paged(self, page_table, past, new, tokens, pages, page_size, rows=None, parents=None, words=1, caches=None,
+                   out=None):
+        """The tables of a step from its sequences' lengths, built on the GPU (a captured step plans itself). Sequence b goes on
+        from row r = rows[b] (int32 [B]; None: b) of page_table (int32 [R, width]), whose first past[r] keys (int32 [R]) it keeps
+        (r outside the table: none), with new[b] new tokens (int32 [B]); `tokens` is the step's size T (tokens past it are left
+        out). Returns a PagedStep:
+          page_table [B, width]  the kept pages, then free ones for the new keys, -1 behind (`out` if given, which may be
+                                 page_table itself without rows: entries behind stay then). Free is what no sequence of the call
+                                 keeps; the first free of `pages` pages go to the sequences in order
+          q_starts [B + 1], kv_lens [B] (int32), positions, slots [T] (int64; 0 and -1 for tokens of no sequence)
+          masks [T, words]       with parents (int32 [T]: the node of its sequence, an earlier one, that a new token hangs below;
+                                 else a root): each token's bit and its ancestors' (int64); positions go by depth then. Else None
+          copies [B, 2]          the page that a sequence's partly filled last page was copied from and to, as it would be
+                                 written and another sequence reads it; -1 where there is none. With caches ((k, v) [layers,
+                                 pages, hkv, page_size, D]) its rows are copied in every layer
+          missing [1]            pages that were wanted and not there"""
+        if not page_table.is_cuda or page_table.dim() != 2 or new.dim() != 1:
+            raise RuntimeError("page_table [R, width] and new [B] must be CUDA tensors")
+        index, device, (held, width), batch = page_table.get_device(), page_table.device, page_table.shape, new.shape[0]
+        tokens, pages, page_size = int(tokens), int(pages), int(page_size)
+        _need_fast(page_table, "page_table", torch.int32, (held, width), index, device)
+        _need_fast(past, "past", torch.int32, (held,), index, device)
+        _need_fast(new, "new", torch.int32, (batch,), index, device)
+        if rows is not None:
+            _need_fast(rows, "rows", torch.int32, (batch,), index, device)
+        if parents is not None:
+            _need_fast(parents, "parents", torch.int32, (tokens,), index, device)
+            if not 1 <= words <= MAX_MASK_WORDS:
+                raise RuntimeError(f"words must be 1..{MAX_MASK_WORDS}, got {words}")
+        layers, hkv, row_bytes = self._check_layers(caches, pages, page_size, index)
+        if tokens < 0:
+            raise RuntimeError("tokens must not be negative")
+        if out is None:
+            out = torch.empty((batch, width), dtype=torch.int32, device=device)
+        else:
+            _need_fast(out, "out", torch.int32, (batch, width), index, device)
+            if rows is not None and out.data_ptr() == page_table.data_ptr():
+                raise RuntimeError("rows need a table of their own to go to")
+        ints = torch.empty(4 * batch + 2, dtype=torch.int32, device=device)
+        copies, q_starts, kv_lens, missing = ints.split_with_sizes((2 * batch, batch + 1, batch, 1))
+        positions = torch.empty(tokens, dtype=torch.int64, device=device)
+        slots = torch.empty(tokens, dtype=torch.int64, device=device)
+        masks = torch.empty((tokens, words), dtype=torch.int64, device=device) if parents is not None else None
+        nbytes = self._plan_workspace(batch, width, tokens, pages, page_size)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        opt = lambda t: None if t is None else t.data_ptr()                               # noqa: E731
+        _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_plan_paged(
+            page_table.data_ptr(), held, width, past.data_ptr(), new.data_ptr(), opt(rows), batch, tokens, pages, page_size,
+            opt(parents), words, out.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+            opt(masks), copies.data_ptr(), missing.data_ptr(), caches[0].data_ptr() if caches else None,
+            caches[1].data_ptr() if caches else None, layers, hkv, row_bytes, opt(ws), nbytes, stream))
+        return PagedStep(out, q_starts, kv_lens, positions, slots, masks, copies.view(batch, 2), missing)
+
+    def accept_drafts(self, tokens, picks, parents, q_starts, kv_lens, page_table, caches, longest):
+        """What the model's own picks (int64 [T], its choice after each token) confirm of drafted tokens (int64 [T]; parents as
+        plan_paged takes them, None: chains): from each sequence's node 0, the first child whose token is the pick after the
+        node before, and so on, at most `longest` <= 1024 nodes. Returns path (int32 [B, longest], -1 behind), counts (int32
+        [B]), accepted (int64 [B, longest]: the picks after the path's nodes, so the confirmed tokens and one more; -1 behind)
+        and lens (int32 [B]: the keys that the sequence keeps, kv_lens - new + counts). With caches ((k, v) [layers, pages,
+        hkv, page_size, D]; None: left to the caller) the confirmed nodes' rows are moved together behind the earlier keys."""
+        if not tokens.is_cuda or tokens.dim() != 1 or page_table.dim() != 2:
+            raise RuntimeError("tokens [T] and page_table [B, width] must be CUDA tensors")
+        index, device, t, (batch, width) = tokens.get_device(), tokens.device, tokens.shape[0], page_table.shape
+        _need_fast(tokens, "tokens", torch.int64, (t,), index, device)
+        _need_fast(picks, "picks", torch.int64, (t,), index, device)
+        if parents is not None:
+            _need_fast(parents, "parents", torch.int32, (t,), index, device)
+        _need_fast(q_starts, "q_starts", torch.int32, (batch + 1,), index, device)
+        _need_fast(kv_lens, "kv_lens", torch.int32, (batch,), index, device)
+        _need_fast(page_table, "page_table", torch.int32, (batch, width), index, device)
+        layers, hkv, row_bytes = self._check_layers(caches, None, None, index)
+        pages, page_size = (caches[0].shape[-4], caches[0].shape[-2]) if caches is not None else (1, 16)
+        longest = int(longest)
+        if not 1 <= longest <= 1024:
+            raise RuntimeError(f"longest must be 1..1024, got {longest}")
+        ints = torch.empty(batch * (longest + 2), dtype=torch.int32, device=device)
+        path, counts, lens = ints.split_with_sizes((batch * longest, batch, batch))
+        accepted = torch.empty((batch, longest), dtype=torch.int64, device=device)
+        _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_accept_drafts(
+            tokens.data_ptr(), picks.data_ptr(), None if parents is None else parents.data_ptr(), q_starts.data_ptr(),
+            kv_lens.data_ptr(), page_table.data_ptr(), width, caches[0].data_ptr() if caches else None,
+            caches[1].data_ptr() if caches else None, path.data_ptr(), counts.data_ptr(), accepted.data_ptr(), lens.data_ptr(),
+            t, batch, longest, layers, pages, hkv, page_size, row_bytes, stream))
+        return path.view(batch, longest), counts, accepted, lens
+
+    def beam_select(self, logits, scores, n, finished=None, pad=0):
+        """The n <= 32 best continuations of each request's beams: of scores[r, w] + log_softmax(logits[r * beams + w])[v] (scores
+        float32 [requests, beams <= 64], logits [requests * beams, V] float32, float16 or bfloat16, rows may lie apart), the
+        largest over all beams and tokens: (scores float32, beams int64, tokens int64), each [requests, n], in falling order,
+        equal ones by beam, then by token. finished (bool [requests, beams]): such a beam has its own score for the token `pad`
+        and -inf for the others. A score that is no finite number and a row without a distribution (a NaN, +inf, or nothing above
+        -inf) give -inf for every token. Scores are summed in 64 bits from a log sum of 32."""
+        dtype = DTYPE_F32 if logits.dtype is torch.float32 else DTYPE_F16 if logits.dtype is torch.float16 else DTYPE_BF16
+        if not logits.is_cuda or logits.dim() != 2 or (dtype == DTYPE_BF16 and logits.dtype is not torch.bfloat16):
+            raise RuntimeError("logits must be a 2-D float32, float16 or bfloat16 CUDA tensor [requests * beams, V]")
+        if scores.dim() != 2:
+            raise RuntimeError("scores must be [requests, beams]")
+        (m, v), (requests, beams) = logits.shape, scores.shape
+        if v > 1 and logits.stride(1) != 1:
+            raise RuntimeError("a row of logits must lie side by side")
+        if requests * beams != m:
+            raise RuntimeError(f"logits must have a row for each of the {requests} x {beams} scores, got {m}")
+        index, device, n, pad = logits.get_device(), logits.device, int(n), int(pad)
+        _need_fast(scores, "scores", torch.float32, (requests, beams), index, device)
+        if finished is not None:
+            _need_fast(finished, "finished", torch.bool, (requests, beams), index, device)
+        if not 1 <= n <= min(32, beams * v):
+            raise RuntimeError(f"n must be 1..32 and at most beams * V = {beams * v}, got {n}")
+        best = torch.empty((requests, n), dtype=torch.float32, device=device)
+        parent = torch.empty((requests, n), dtype=torch.int64, device=device)
+        token = torch.empty((requests, n), dtype=torch.int64, device=device)
+        if requests == 0:
+            return best, parent, token
+        # the slices' sums and alternatives, for this call alone
+        nbytes = (m + (1024 if m < 512 and v >= 4096 else 0)) * (16 + 8 * n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_beam_select(
+            logits.data_ptr(), dtype, logits.stride(0) if m > 1 else v, scores.data_ptr(),
+            None if finished is None else finished.data_ptr(), best.data_ptr(), parent.data_ptr(), token.data_ptr(), requests,
+            beams, v, n, pad, ws.data_ptr(), nbytes, stream))
+        return best, parent, token
 
     def token_logprobs(self, logits, targets, top=0):
         """Of logits [M, V] (float32, float16 or bfloat16; rows may lie apart): (log probability of targets [M] (int64;
