@@ -777,9 +777,9 @@ static int check_layers(const char* what, const void* k, const void* v, int64_t 
   if (pages < 1 || !fits_int(pages)) return fail(LOWBIT_ERR_SHAPE, "%s: pages must be positive", what);
   if (!k != !v) return fail(LOWBIT_ERR_ARG, "%s: k_cache goes with v_cache", what);
   if (!k) return LOWBIT_OK;
-  if (layers < 1 || layers > 65535 || Hkv < 1 || Hkv > 65536 || row_bytes < 16 || row_bytes > 32768 || row_bytes % 16 ||
+  if (layers < 1 || layers > 65535 || Hkv < 1 || Hkv > 65536 || row_bytes < 16 || row_bytes > 4096 || row_bytes % 16 ||
       page_size * row_bytes / 16 > (1 << 30) / Hkv)
-    return fail(LOWBIT_ERR_SHAPE, "%s: layers must be 1..65535, rows of the caches 16..32768 bytes, a multiple of 16, and a page of a "
+    return fail(LOWBIT_ERR_SHAPE, "%s: layers must be 1..65535, rows of the caches 16..4096 bytes, a multiple of 16, and a page of a "
                 "layer less than 2^34 bytes", what);
   if (!aligned16(k) || !aligned16(v)) return fail(LOWBIT_ERR_ALIGN, "%s needs 16-byte aligned caches", what);
   return LOWBIT_OK;

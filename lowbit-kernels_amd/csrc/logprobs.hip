@@ -402,87 +402,101 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
 }
 
 // ---- beam_select ----
-// A workgroup of `blockDim / 64` waves per request. A wave takes a beam: its slices' sums and alternatives are joined as above,
-// into the beam's n best, score + (x - max) - log z in 64 bits (which of two beams' tokens comes first goes by that difference).
-// Then all beams' n best are ranked by counting, a beam's list only as far as it comes before the candidate. A beam that holds
-// nothing (a score that is no finite number) or whose row has no distribution has -inf for every token, a finished one its score
-// for `pad` and -inf for the others; equal candidates rank by beam, then by token.
+// A workgroup of `blockDim / 64` waves per request. A wave takes a beam: its slices' sums are joined, and of their lists what
+// reaches a bound is ranked by counting, into the beam's n best, score + (x - max) - log z in 64 bits (which of two beams' tokens
+// comes first goes by that difference). The bound: at least n logits reach the n-th largest of the slices' first ones, or, of S < n
+// slices, the least of their ceil(n / S)-th ones. Then all beams' n best are ranked by counting, a few threads a candidate.
+// A beam that holds nothing (a score that is no finite number) or whose row has no distribution has -inf for every token, a
+// finished one its score for `pad` and -inf for the others; equal candidates rank by beam, then by token.
 __global__ __launch_bounds__(512) void beam_join_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ finished,
                                                        float* __restrict__ out_scores, int64_t* __restrict__ out_beams,
                                                        int64_t* __restrict__ out_tokens, int W, int V, int n, int pad, int S,
                                                        const Sums* __restrict__ part, const uint64_t* __restrict__ part_keys) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, req = blockIdx.x;
-  double* s_value = reinterpret_cast<double*>(smem);          // [W][n]
-  int* s_token = reinterpret_cast<int*>(s_value + W * n);     // (rounded up to a multiple of two)
-  uint64_t* s_keys = reinterpret_cast<uint64_t*>(s_token + ((W * n + 1) & ~1)) + wave * (S + min(S, n)) * n;
-  uint64_t* s_list = s_keys + S * n;
   const int have = min(n, V);                                 // candidates of a beam
+  double* s_value = reinterpret_cast<double*>(smem);          // [W][have]
+  int* s_token = reinterpret_cast<int*>(s_value + W * n);     // (rounded up to a multiple of two)
+  uint64_t* s_keys = reinterpret_cast<uint64_t*>(s_token + ((W * n + 1) & ~1)) + wave * 2 * S * n;
+  uint64_t* s_list = s_keys + S * n;
   for (int w = wave; w < W; w += waves) {
     const int64_t row = (int64_t)req * W + w;
+    const uint64_t* keys = part_keys + row * S * n;
     const float score = scores[row];
-    const bool held = fabsf(score) <= FLT_MAX, done = held && finished && finished[row];
+    const uint8_t flag = finished ? finished[row] : 0;
+    Sums s = lane < S ? part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};   // (of a row that was not read: not used)
+    const bool held = fabsf(score) <= FLT_MAX, done = held && flag;
     bool none = !held;
     if (held && !done) {
-      const uint64_t* keys = part_keys + row * S * n;
       for (int i = lane; i < S * n; i += 64) s_keys[i] = keys[i];
-      Sums s = lane < S ? part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};
       const float m = wave_max(s.m);
       move_sums(s.m, m, s.z, s.e);
       const float z = wave_sum(s.z);
       none = !(m > -INFINITY && m < INFINITY) || z != z;
       lds_wave_order();
       if (!none) {
-        const double at = (double)score - log((double)z);
-        const uint64_t first = lane < S ? s_keys[lane * n] : 0;
-        int above = 0;
-        for (int l = 0; l < S; ++l) above += s_keys[l * n] > first;
-        const uint64_t at_bound = __ballot(lane < S && above == n - 1);   // (keys are distinct; none where S < n)
-        const uint64_t bound = at_bound ? s_keys[__builtin_ctzll(at_bound) * n] : 0;
-        int mine = 0;
-        if (lane < S)
-          while (mine < n && s_keys[lane * n + mine] >= max(bound, (uint64_t)1)) ++mine;
-        int upto = mine;
+        uint64_t bound;
+        if (S >= n) {
+          const uint64_t first = lane < S ? s_keys[lane * n] : 0;
+          int above = 0;
+#pragma unroll 8
+          for (int l = 0; l < S; ++l) above += s_keys[l * n] > first;
+          bound = s_keys[__builtin_ctzll(__ballot(lane < S && above == n - 1)) * n];   // (first keys are distinct)
+        } else {
+          const int at = (n + S - 1) / S - 1;
+          bound = lane < S ? s_keys[lane * n + at] : ~(uint64_t)0;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const int o = __shfl_up(upto, off, 64);
-          if (lane >= off) upto += o;
+          for (int off = 1; off < 32; off <<= 1) bound = min(bound, (uint64_t)__shfl_xor((unsigned long long)bound, off, 64));   // (S < n <= 32)
+          bound = __shfl((unsigned long long)bound, 0, 64);
         }
-        for (int i = 0; i < mine; ++i) s_list[upto - mine + i] = s_keys[lane * n + i];
-        const int all = __shfl(upto, 63, 64);
+        if (bound == 0) bound = 1;                            // (slices with fewer logits end in zeros)
+        int all = 0;
+        for (int i0 = 0; i0 < S * n; i0 += 64) {
+          const uint64_t key = i0 + lane < S * n ? s_keys[i0 + lane] : 0;
+          const uint64_t in = __ballot(key >= bound);
+          if (key >= bound) s_list[all + __popcll(in & (((uint64_t)1 << lane) - 1))] = key;
+          all += __popcll(in);
+        }
         lds_wave_order();
+        const double at = (double)score - log((double)z);
         for (int i = lane; i < all; i += 64) {
           const uint64_t key = s_list[i];
           int rank = 0;
+#pragma unroll 8
           for (int k = 0; k < all; ++k) rank += s_list[k] > key;
-          if (rank >= n) continue;
-          s_value[w * n + rank] = at + ((double)order_value((uint32_t)(key >> 32)) - (double)m);
-          s_token[w * n + rank] = rank_index(key);
+          if (rank >= have) continue;
+          s_value[w * have + rank] = at + ((double)order_value((uint32_t)(key >> 32)) - (double)m);
+          s_token[w * have + rank] = rank_index(key);
         }
       }
     }
     if (none || done) {
       for (int i = lane; i < have; i += 64) {
-        s_value[w * n + i] = done && i == 0 ? (double)score : -INFINITY;
-        s_token[w * n + i] = !done ? i : i == 0 ? pad : i - 1 < pad ? i - 1 : i;
+        s_value[w * have + i] = done && i == 0 ? (double)score : -INFINITY;
+        s_token[w * have + i] = !done ? i : i == 0 ? pad : i - 1 < pad ? i - 1 : i;
       }
     }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < W * have; c += blockDim.x) {
-    const int w = c / have, i = c - w * have;
-    const double v = s_value[w * n + i];
-    int rank = i;                                             // (a beam's own list is in order)
-    for (int o = 0; o < W && rank < n; ++o) {
-      if (o == w) continue;
-      const double* theirs = s_value + o * n;
-      for (int k = 0; k < have && rank < n && (theirs[k] > v || (theirs[k] == v && o < w)); ++k) ++rank;
+  // a candidate's rank, counted by `per` lanes side by side
+  const int all = W * have;
+  int per = 1;
+  while (per < 16 && 2 * per * all <= (int)blockDim.x) per *= 2;
+  for (int c0 = 0; c0 < all; c0 += (int)blockDim.x / per) {
+    const int c = c0 + (int)threadIdx.x / per;
+    const double v = c < all ? s_value[c] : 0.0;
+    int rank = 0;
+#pragma unroll 4
+    for (int k = (int)threadIdx.x % per; k < all; k += per) {
+      const double o = s_value[k];
+      rank += o > v || (o == v && k < c);
     }
-    if (rank >= n) continue;
+    for (int off = 1; off < per; off <<= 1) rank += __shfl_xor(rank, off, 64);
+    if (c >= all || rank >= n || (int)threadIdx.x % per) continue;
     const int64_t to = (int64_t)req * n + rank;
     out_scores[to] = (float)v;
-    out_beams[to] = w;
-    out_tokens[to] = s_token[w * n + i];
+    out_beams[to] = c / have;
+    out_tokens[to] = s_token[c];
   }
 }
 
@@ -532,8 +546,8 @@ hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st) {
                                 : go(logprobs_kernel<bf16>, static_cast<const bf16*>(a.logits));
   if (e != hipSuccess) return e;
   // waves: as many beams at once as LDS holds the lists of
-  const size_t fixed = (size_t)a.beams * a.n * 12 + 8, each = (size_t)(S + std::min(S, a.n)) * a.n * 8;
-  const int waves = (int)std::max<size_t>(1, std::min<size_t>({(size_t)8, (size_t)a.beams, (140 * 1024 - fixed) / each}));
+  const size_t fixed = (size_t)a.beams * a.n * 12 + 8, each = (size_t)2 * S * a.n * 8;
+  const int waves = (int)std::max<size_t>(1, std::min<size_t>((size_t)8, (140 * 1024 - fixed) / each));
   const size_t join_lds = fixed + waves * each;
   if (join_lds > 65536) {
     static std::atomic<uint64_t> done{0};

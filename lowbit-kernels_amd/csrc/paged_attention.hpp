@@ -84,7 +84,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int se
 // keys far above the mean are cut (us with half a round, one, one and a half and two: 64 decode tokens of 32 / 8 heads on 300 ..
 // 8000 keys 147, 133, 129 and 128; a prompt of 2000 tokens, 28 / 4 heads, 64, 71, 71 and 79; a mixed step 33.8, 34.2, 34.7 and
 // 34.8). s0: the first 64 sequences.
-template <int kRows, int kBlock>
+template <int kRows, int kBlock, bool kTree>
 __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {
   if (p.cap == 1) return 0x3FFFFFFF;
   float total = wave_sum((float)s0.tiles * (float)s0.blocks), units = wave_sum((float)s0.tiles);
@@ -96,13 +96,36 @@ __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan&
   total *= (float)p.Hkv;
   units *= (float)p.Hkv;
   const float slots = (float)p.slots;
+  if (kTree && b.B <= 64) {
+    // the least share whose parts, each sequence's rounded up, run at once (as many rounds of slots as tiles of one part need)
+    const float room = fminf(ceilf(units / slots) * slots, fmaxf((float)p.most, units));
+    int lo = max(p.least, (int)fminf(total / room, 1e9f)), hi = 1 << 26;
+    auto fits = [&](int share) {
+      return wave_sum((float)(s0.tiles * max(1, min(p.cap, (s0.blocks + share - 1) / share)))) * (float)p.Hkv <= room;
+    };
+    if (fits(lo)) return lo;
+    int step = max(1, lo >> 4);
+    while (!fits(lo + step) && lo + step < hi) {
+      lo += step;
+      step += step;
+    }
+    hi = lo + step;
+    while (hi - lo > max(1, lo >> 5)) {
+      const int mid = (lo + hi) >> 1;
+      if (fits(mid))
+        hi = mid;
+      else
+        lo = mid;
+    }
+    return hi;
+  }
   const float free = fminf(units < 0.75f * slots ? slots - units : 1.5f * slots, (float)(p.most / 2));
   return max(p.least, (int)fminf(ceilf(total / free), 1e9f));
 }
 
 // The part of work `idx`; false past the last one. kMerge > 0: the chunk `idx` of kMerge rows (a divisor of kRows) of the split
 // tiles, pid counting the chunk in its tile and rec the tile's first part.
-template <int kRows, int kBlock, int kMerge>
+template <int kRows, int kBlock, int kMerge, bool kTree>
 __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int share, int idx,
                                            int lane, PagedUnit& u) {
   int before = 0, recs = 0;                                  // work and record groups of the sequences before
@@ -124,7 +147,15 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
       u.parts = p.cap == 1 ? 1 : pick(parts);
       const int at = idx - before - pick(upto - mine), rest = div(at, p.by_hkv);
       u.hk = at - rest * p.Hkv;                              // KV heads fastest: a head's keys stay in the L2 of its XCDs
-      if constexpr (kMerge == 0) {
+      if constexpr (kMerge == 0 && kTree) {
+        // a part's tiles, which walk the same keys, eight workgroups apart: the L2 of one XCD reads the keys once
+        const int all = u.parts * p.Hkv, chunk = (int)((uint32_t)at / (uint32_t)(8 * u.tiles));
+        const int in = at - chunk * 8 * u.tiles, wide = min(8, all - 8 * chunk), t = (int)((uint32_t)in / (uint32_t)wide);
+        const int part = 8 * chunk + in - t * wide;
+        u.pid = div(part, p.by_hkv);
+        u.hk = part - u.pid * p.Hkv;
+        u.tile = t;
+      } else if constexpr (kMerge == 0) {
         const int t = u.parts == 1 ? rest : (int)((uint32_t)rest / (uint32_t)u.parts);
         u.pid = rest - t * u.parts;
         u.tile = u.tiles - 1 - t;                            // the last rows, which have the most keys, first
@@ -299,7 +330,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
   const int j = lane & 31, h = lane >> 5;
   PagedUnit un;
   const PagedSeq s0 = paged_seq<kRows, BK>(bt, G, lane);
-  if (!paged_unit<kRows, BK, 0>(bt, plan, s0, paged_share<kRows, BK>(bt, plan, s0, lane), blockIdx.x, lane, un)) return;
+  if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, paged_share<kRows, BK, kTree>(bt, plan, s0, lane), blockIdx.x, lane, un)) return;
   const int rgrp = wave % RG, kgrp = wave / RG;
   const int cap = bt.table_width * bt.page_size;
   const int len = min(un.len, cap);                  // keys that can be read
@@ -700,9 +731,9 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
   const int lane = threadIdx.x & 63, grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   const float c2 = score_scale(scale);
   const PagedSeq s0 = paged_seq<kRows, kBlock>(bt, plan.G, lane);
-  const int share = paged_share<kRows, kBlock>(bt, plan, s0, lane);
+  const int share = paged_share<kRows, kBlock, kTree>(bt, plan, s0, lane);
   PagedUnit un;
-  for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
+  for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere, kTree>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
     const int r = un.pid * kHere + grp / PG, row = un.tile * kRows + r;
     const float* rec = part + ((size_t)un.rec * kRows + r) * kRec;
     const size_t step = (size_t)kRows * kRec;
@@ -830,7 +861,10 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
   PagedPlan p{l.slots, l.least, 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
   p.most = a.ws ? (int)std::min<size_t>((size_t)l.records, a.ws_bytes / paged_record_bytes(RG, D)) : 0;
   if (p.most >= 2) p.cap = l.cap;
-  const int64_t grid = p.cap == 1 ? l.units : std::min<int64_t>(l.units * p.cap, l.units + p.most / 2 + 1);
+  // (paged_share: parts take its free slots beside one a tile, or those of whole rounds)
+  const int64_t rounds = (l.units + l.slots - 1) / l.slots * l.slots;
+  const int64_t split = kTree && a.batch.B <= 64 ? std::max(l.units, std::min<int64_t>(rounds, p.most)) : l.units + p.most / 2 + 1;
+  const int64_t grid = p.cap == 1 ? l.units : std::min<int64_t>(l.units * p.cap, split);
   if (lds > 65536) {
     static std::atomic<uint64_t> done{0};
     if (hipError_t e = allow_lds_once(done, paged_attention<T, D, RG, KG, kTree>, most_lds)) return e;

@@ -14,20 +14,16 @@ namespace lowbit {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kWordsPer = 8;             // bitmap words of a thread in one step of the search for free pages
+constexpr int kMasksPer = 4;             // words of 32 pages that a thread looks through in one step of the search for free pages
 // what one workgroup plans alone, its state in LDS
 constexpr int kSmallSeqs = 1024, kSmallTokens = 4096, kSmallList = kSmallTokens / 16 + 2 * kSmallSeqs;
 constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 16;
+constexpr int kHashSeqs = 4096;          // sequences whose hash lies in LDS, and whose starts every workgroup copies there
 
-// One sequence: its row of the table and keys there (none: a row outside the table), its new tokens as far as the call's T
-// reaches, its pages kept, and in all (`need`: those the row has place for).
-struct PlanSeq {
-  int row, past, fresh;
-};
-// The state of a call, in LDS or in the workspace: [B] each but start (as q_starts, [B + 1])
+// The state of a call, in LDS or in the workspace: [B] each but off and start ([B + 1])
 struct PlanState {
   int *row, *past, *fresh, *tail, *off, *start;   // tail: the last page kept; off: its first place in the list, ~off if that is a copy
-  uint32_t *held, *whole;                         // a bit a page: kept by a sequence; kept and full
+  uint32_t* used;                                 // LDS: a bit a page, workspace: a byte: kept (while pages are marked: kept and full)
   int* hash_page;                                 // the pages that are partly filled, and whose they are (owner_key)
   uint64_t* hash_owner;
   int hash_mask;
@@ -35,14 +31,33 @@ struct PlanState {
   int list_cap;
 };
 
-__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int shift, int b) {
-  PlanSeq s;
-  s.row = a.rows ? a.rows[b] : b;
-  s.past = s.row >= 0 && s.row < a.R ? min(max(a.past[s.row], 0), a.width << shift) : 0;
-  s.fresh = min(max(a.fresh[b], 0), a.T);
-  return s;
-}
 __device__ __forceinline__ int pages_of(int keys, int shift) { return (keys + (1 << shift) - 1) >> shift; }
+
+template <bool kLds>
+__device__ __forceinline__ void use_page(const PlanState& s, int page) {
+  if constexpr (kLds)
+    atomicOr(s.used + (page >> 5), 1u << (page & 31));
+  else
+    reinterpret_cast<uint8_t*>(s.used)[page] = 1;             // (all writers write the same: no atomics)
+}
+template <bool kLds>
+__device__ __forceinline__ bool page_used(const PlanState& s, int page) {
+  if constexpr (kLds) return s.used[page >> 5] >> (page & 31) & 1u;
+  return reinterpret_cast<const uint8_t*>(s.used)[page];
+}
+// pages 32 w .. + 31 that are free, a bit each
+template <bool kLds>
+__device__ __forceinline__ uint32_t free_pages(const PlanState& s, int w) {
+  if constexpr (kLds) return ~s.used[w];
+  const u32x4 a = load16(s.used + 8 * (int64_t)w), b = load16(s.used + 8 * (int64_t)w + 4);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t t = ~(i < 4 ? a[i & 3] : b[i & 3]) & 0x01010101u;
+    m |= ((t | t >> 7 | t >> 14 | t >> 21) & 0xFu) << (4 * i);
+  }
+  return m;
+}
 
 // of the sequences that hold a partly filled page: the most keys, then one that writes, then the first
 __device__ __forceinline__ uint64_t owner_key(int past, int fresh, int b) {
@@ -50,37 +65,16 @@ __device__ __forceinline__ uint64_t owner_key(int past, int fresh, int b) {
 }
 __device__ __forceinline__ int hash_slot(int page, int mask) { return (int)(((uint32_t)page * 2654435761u) >> 7) & mask; }
 
-// entry c of sequence b's row, a page that it keeps
-__device__ __forceinline__ void mark(const PlanState& s, int64_t pages, int shift, int b, int c, int page) {
-  const int past = s.past[b];
-  const bool last = c == pages_of(past, shift) - 1, part = last && (past & ((1 << shift) - 1));
-  if (last) s.tail[b] = page;
-  if (page < 0 || page >= pages) return;
-  atomicOr(s.held + (page >> 5), 1u << (page & 31));
-  if (!part) {
-    atomicOr(s.whole + (page >> 5), 1u << (page & 31));
-    return;
-  }
-  for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask) {   // (twice as many places as sequences)
-    const int was = atomicCAS(s.hash_page + at, -1, page);
-    if (was != -1 && was != page) continue;
-    atomicMax(reinterpret_cast<unsigned long long*>(s.hash_owner) + at, (unsigned long long)owner_key(past, s.fresh[b], b));
-    break;
-  }
-}
-
-// whether sequence b needs a copy of its last page
-__device__ __forceinline__ bool needs_copy(const PlanState& s, int64_t pages, int shift, int b) {
-  const int past = s.past[b], page = s.tail[b];
-  if (!(past & ((1 << shift) - 1)) || s.fresh[b] <= 0 || page < 0 || page >= pages) return false;
-  if (s.whole[page >> 5] >> (page & 31) & 1u) return true;
-  for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask)
-    if (s.hash_page[at] == page) return s.hash_owner[at] != owner_key(past, s.fresh[b], b);
+// sequence b's partly filled last page, if it has one
+__device__ __forceinline__ int part_page(const PlanArgs& a, const PlanState& s, int shift, int b) {
+  const int page = s.tail[b];
+  return (s.past[b] & ((1 << shift) - 1)) && page >= 0 && page < a.pages ? page : -1;
 }
 
 // the sum of the threads' values up to and including this one's, held at `most`; *all: of all threads (values 0 .. most)
 __device__ __forceinline__ int block_scan(int v, int most, int* s_wave, int* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int o = __shfl_up(v, off, 64);
     if (lane >= off) v = min(v + o, most);
@@ -89,9 +83,8 @@ __device__ __forceinline__ int block_scan(int v, int most, int* s_wave, int* all
   if (lane == 63) s_wave[wave] = v;
   __syncthreads();
   int before = 0, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    before = w < wave ? min(before + s_wave[w], most) : before;
+  for (int w = 0; w < waves; ++w) {
+    before = w == wave ? sum : before;
     sum = min(sum + s_wave[w], most);
   }
   *all = sum;
@@ -101,17 +94,23 @@ __device__ __forceinline__ int block_scan(int v, int most, int* s_wave, int* all
 // q_starts, kv_lens and the sequences' lengths, by one workgroup
 __device__ __forceinline__ void plan_lens(const PlanArgs& a, const PlanState& s, int shift, int* s_wave) {
   int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.B; b0 += (int)blockDim.x) {
     const int b = b0 + threadIdx.x;
-    PlanSeq q{-1, 0, 0};
-    if (b < a.B) q = plan_seq(a, shift, b);
-    int all;
-    const int upto = min(before + block_scan(q.fresh, a.T, s_wave, &all), a.T);
+    int row = -1, past = 0, fresh = 0;
     if (b < a.B) {
-      s.start[b + 1] = upto;                                  // (held at T: tokens past it are left out)
+      row = a.rows ? a.rows[b] : b;
+      fresh = min(max(a.fresh[b], 0), a.T);
+      if (row >= 0 && row < a.R) past = min(max(a.past[row], 0), a.width << shift);
+    }
+    int all;
+    const int upto = min(before + block_scan(fresh, a.T, s_wave, &all), a.T);   // (held at T: tokens past it are left out)
+    int first = __shfl_up(upto, 1, 64);
+    if (b < a.B) {
+      s.start[b + 1] = upto;
       a.q_starts[b + 1] = upto;
-      s.row[b] = q.row;
-      s.past[b] = q.past;
+      s.row[b] = row;
+      s.past[b] = past;
+      s.tail[b] = -1;
     }
     if (b == 0) {
       s.start[0] = 0;
@@ -119,59 +118,81 @@ __device__ __forceinline__ void plan_lens(const PlanArgs& a, const PlanState& s,
     }
     __syncthreads();
     if (b < a.B) {
-      const int fresh = s.start[b + 1] - s.start[b];
-      s.fresh[b] = fresh;
-      s.tail[b] = -1;
-      a.kv_lens[b] = q.past + fresh;
+      if ((threadIdx.x & 63) == 0) first = s.start[b];
+      s.fresh[b] = upto - first;
+      a.kv_lens[b] = past + upto - first;
     }
     before = min(before + all, a.T);
   }
 }
 
-// which sequences get how many of the free pages, and which pages those are, by one workgroup
-__device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, int* s_wave) {
-  int total = 0, over = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+// Which sequences get how many of the free pages, and which pages those are, by one workgroup. The hash is empty before.
+template <bool kLds>
+__device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, int* s_wave, int* s_over) {
+  if (threadIdx.x == 0) *s_over = 0;
+  for (int b = threadIdx.x; b < a.B; b += (int)blockDim.x) {
+    const int page = part_page(a, s, shift, b);
+    if (page < 0) continue;
+    for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask) {   // (twice as many places as sequences)
+      const int was = atomicCAS(s.hash_page + at, -1, page);
+      if (was != -1 && was != page) continue;
+      atomicMax(reinterpret_cast<unsigned long long*>(s.hash_owner) + at, (unsigned long long)owner_key(s.past[b], s.fresh[b], b));
+      break;
+    }
+  }
+  __syncthreads();
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += (int)blockDim.x) {
     const int b = b0 + threadIdx.x;
-    int want = 0, past_width = 0;                             // pages; those that the table has no place for
+    int want = 0;
     bool copy = false;
     if (b < a.B) {
-      const int past = s.past[b], have = pages_of(past, shift), need = pages_of(past + s.fresh[b], shift);
-      copy = needs_copy(s, a.pages, shift, b);
+      const int past = s.past[b], fresh = s.fresh[b], have = pages_of(past, shift), need = pages_of(past + fresh, shift);
+      const int page = fresh > 0 ? part_page(a, s, shift, b) : -1;
+      if (page >= 0) {
+        copy = page_used<kLds>(s, page);                      // (within another's keys)
+        int at = hash_slot(page, s.hash_mask);
+        while (s.hash_page[at] != page) at = (at + 1) & s.hash_mask;
+        copy |= s.hash_owner[at] != owner_key(past, fresh, b);
+      }
       want = min(need, a.width) - have + (copy ? 1 : 0);
-      past_width = max(need - a.width, 0);
+      if (need > a.width) atomicAdd(s_over, need - a.width);  // pages that the table has no place for
     }
     int all;
     const int upto = block_scan(want, INT_MAX / 2, s_wave, &all);
     if (b < a.B) s.off[b] = copy ? ~(total + upto - want) : total + upto - want;
     total += all;
-    block_scan(past_width, INT_MAX / 2, s_wave, &all);
-    over += all;
   }
   total = min(total, s.list_cap);
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.B; b += (int)blockDim.x) {
+    const int page = part_page(a, s, shift, b);
+    if (page >= 0) use_page<kLds>(s, page);
+  }
+  __syncthreads();
   const int words = (int)((a.pages + 31) >> 5);
   int found = 0;
-  for (int w0 = 0; w0 < words && found < total; w0 += kThreads * kWordsPer) {
-    uint32_t free[kWordsPer];
+  for (int w0 = 0; w0 < words && found < total; w0 += (int)blockDim.x * kMasksPer) {
+    uint32_t free[kMasksPer];
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kWordsPer; ++i) {
-      const int w = w0 + (int)threadIdx.x * kWordsPer + i;
+    for (int i = 0; i < kMasksPer; ++i) {
+      const int w = w0 + (int)threadIdx.x * kMasksPer + i;
       const int64_t left = a.pages - 32 * (int64_t)w;
-      free[i] = w < words ? ~s.held[w] & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
+      free[i] = w < words ? free_pages<kLds>(s, w) & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
       n += __popc(free[i]);
     }
     int all;
     int at = found + block_scan(n, INT_MAX / 2, s_wave, &all) - n;
 #pragma unroll
-    for (int i = 0; i < kWordsPer; ++i)
+    for (int i = 0; i < kMasksPer; ++i)
       for (uint32_t f = free[i]; f && at < total; f &= f - 1, ++at)
-        s.list[at] = 32 * (w0 + (int)threadIdx.x * kWordsPer + i) + __ffs(f) - 1;
+        s.list[at] = 32 * (w0 + (int)threadIdx.x * kMasksPer + i) + __ffs(f) - 1;
     found = min(found + all, total);
   }
-  for (int i = found + threadIdx.x; i < total; i += kThreads) s.list[i] = -1;
+  for (int i = found + threadIdx.x; i < total; i += (int)blockDim.x) s.list[i] = -1;
   if (threadIdx.x == 0) {
-    *a.missing = over + total - found;
+    *a.missing = *s_over + total - found;
     s.off[a.B] = total;
   }
 }
@@ -247,15 +268,14 @@ __device__ __forceinline__ void give_token(const PlanArgs& a, const PlanState& s
 // The whole plan by one workgroup.
 __global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, FastDiv by_width, int shift, int hash_mask) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
-  __shared__ int s_wave[kThreads / 64];
-  const int tid = threadIdx.x, words = ((int)((a.pages + 31) >> 5) + 3) & ~3;
+  __shared__ int s_wave[kThreads / 64], s_over;
+  const int tid = threadIdx.x, threads = blockDim.x, words = ((int)((a.pages + 31) >> 5) + 3) & ~3;
   PlanState s;
   s.hash_mask = hash_mask;
   s.list_cap = kSmallList;
   s.hash_owner = reinterpret_cast<uint64_t*>(s_plan);
-  s.held = reinterpret_cast<uint32_t*>(s.hash_owner + hash_mask + 1);
-  s.whole = s.held + words;
-  s.hash_page = reinterpret_cast<int*>(s.whole + words);
+  s.used = reinterpret_cast<uint32_t*>(s.hash_owner + hash_mask + 1);
+  s.hash_page = reinterpret_cast<int*>(s.used + words);
   s.row = s.hash_page + hash_mask + 1;
   s.past = s.row + a.B;
   s.fresh = s.past + a.B;
@@ -264,75 +284,102 @@ __global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, FastDi
   s.start = s.off + a.B + 1;
   s.list = s.start + a.B + 1;
   int* s_parent = s.list + kSmallList;
-  plan_lens(a, s, shift, s_wave);
-  for (int i = tid; i < 2 * (hash_mask + 1) + 2 * words; i += kThreads) s_plan[i] = 0;
-  for (int i = tid; i <= hash_mask; i += kThreads) s.hash_page[i] = -1;
   if (a.parents)
-    for (int i = tid; i < a.T; i += kThreads) s_parent[i] = a.parents[i];
+    for (int i = tid; i < a.T; i += threads) s_parent[i] = a.parents[i];
+  for (int i = tid; i < 2 * (hash_mask + 1) + words; i += threads) s_plan[i] = 0;
+  for (int i = tid; i <= hash_mask; i += threads) s.hash_page[i] = -1;
+  plan_lens(a, s, shift, s_wave);
   __syncthreads();
   const int entries = a.B * a.width;
   const bool other = a.table_out != a.table;
-  constexpr int kAhead = 4;
-  for (int i0 = tid; i0 < entries; i0 += kAhead * kThreads) {
-    int page[kAhead], b[kAhead], c[kAhead];
+  constexpr int kAhead = 8;
+  for (int i0 = tid; i0 < entries; i0 += kAhead * threads) {
+    int page[kAhead], b[kAhead], c[kAhead], have[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int i = min(i0 + u * kThreads, entries - 1);
+      const int i = min(i0 + u * threads, entries - 1);
       b[u] = div(i, by_width);
       c[u] = i - b[u] * a.width;
-      page[u] = -1;
-      if (c[u] < pages_of(s.past[b[u]], shift)) page[u] = a.table[(int64_t)s.row[b[u]] * a.width + c[u]];
+      have[u] = s.past[b[u]];
+      page[u] = s.row[b[u]];
     }
 #pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      page[u] = c[u] < pages_of(have[u], shift) ? a.table[(int64_t)page[u] * a.width + c[u]] : -1;
+#pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (i0 + u * kThreads >= entries) break;
-      if (c[u] < pages_of(s.past[b[u]], shift)) mark(s, a.pages, shift, b[u], c[u], page[u]);
-      if (other) a.table_out[i0 + u * kThreads] = page[u];
+      if (i0 + u * threads >= entries) break;
+      if (c[u] == pages_of(have[u], shift) - 1) s.tail[b[u]] = page[u];
+      if (c[u] < have[u] >> shift && page[u] >= 0 && page[u] < a.pages) use_page<true>(s, page[u]);
+      if (other) a.table_out[i0 + u * threads] = page[u];
     }
   }
   __syncthreads();
-  plan_assign(a, s, shift, s_wave);
+  plan_assign<true>(a, s, shift, s_wave, &s_over);
   __syncthreads();
-  for (int j = tid; j < s.off[a.B]; j += kThreads) give_page(a, s, shift, j);
-  for (int b = tid; b < a.B; b += kThreads) give_copy(a, s, b);
-  for (int t = tid; t < a.T; t += kThreads) give_token(a, s, shift, t, [&](int first, int n) { return s_parent[first + n]; });
+  for (int j = tid; j < s.off[a.B]; j += threads) give_page(a, s, shift, j);
+  for (int b = tid; b < a.B; b += threads) give_copy(a, s, b);
+  for (int t = tid; t < a.T; t += threads) give_token(a, s, shift, t, [&](int first, int n) { return s_parent[first + n]; });
 }
 
-// The same in four launches, the state in the workspace: the lengths beside the clearing of the bitmaps; the pages kept; the
-// pages handed out; tables and tokens.
-__global__ __launch_bounds__(kThreads) void plan_lens_kernel(PlanArgs a, PlanState s, int shift, int words) {
+// The same in four launches, the state in the workspace: the lengths, beside the clearing of what the pages are marked in; the
+// pages kept, 1024 entries of a row a workgroup; the pages handed out; tables and tokens.
+__global__ __launch_bounds__(kThreads) void plan_lens_kernel(PlanArgs a, PlanState s, int shift, int64_t clear) {
   __shared__ int s_wave[kThreads / 64];
   if (blockIdx.x == 0) {
     plan_lens(a, s, shift, s_wave);
     return;
   }
-  const int64_t n = 2 * (int64_t)(s.hash_mask + 1) + 2 * (int64_t)words, step = (int64_t)(gridDim.x - 1) * kThreads;
-  const int64_t at = (int64_t)(blockIdx.x - 1) * kThreads + threadIdx.x;
-  uint32_t* zero = reinterpret_cast<uint32_t*>(s.hash_owner);   // the bitmaps follow the owners
-  for (int64_t i = at; i < n; i += step) zero[i] = 0;
-  for (int64_t i = at; i <= s.hash_mask; i += step) s.hash_page[i] = -1;
+  const int64_t step = (int64_t)(gridDim.x - 1) * kThreads, at = (int64_t)(blockIdx.x - 1) * kThreads + threadIdx.x;
+  u32x4* zero = reinterpret_cast<u32x4*>(s.used);             // (the owners of a hash in the workspace follow)
+  for (int64_t i = at; i < clear; i += step) zero[i] = u32x4{0u, 0u, 0u, 0u};
+  if (s.hash_page)
+    for (int64_t i = at; i <= s.hash_mask; i += step) s.hash_page[i] = -1;
 }
 
-__global__ __launch_bounds__(256) void plan_mark_kernel(PlanArgs a, PlanState s, FastDiv by_width, int shift) {
-  const int entries = a.B * a.width, step = gridDim.x * 256;
+__global__ __launch_bounds__(256) void plan_mark_kernel(PlanArgs a, PlanState s, int chunks, int shift) {
+  const int b = blockIdx.x / chunks, c0 = (blockIdx.x - b * chunks) * 1024 + threadIdx.x;
+  const int row = s.row[b], past = s.past[b], have = pages_of(past, shift);
   const bool other = a.table_out != a.table;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < entries; i += step) {
-    const int b = div(i, by_width), c = i - b * a.width;
-    int page = -1;
-    if (c < pages_of(s.past[b], shift)) {
-      page = a.table[(int64_t)s.row[b] * a.width + c];
-      mark(s, a.pages, shift, b, c, page);
-    }
-    if (other) a.table_out[i] = page;
+  int page[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) page[u] = c0 + 256 * u < have ? a.table[(int64_t)row * a.width + c0 + 256 * u] : -1;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int c = c0 + 256 * u;
+    if (c == have - 1) s.tail[b] = page[u];
+    if (c < past >> shift && page[u] >= 0 && page[u] < a.pages) use_page<false>(s, page[u]);
+    if (other && c < a.width) a.table_out[(int64_t)b * a.width + c] = page[u];
   }
 }
 
 __global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanState s, int shift) {
-  __shared__ int s_wave[kThreads / 64];
-  plan_assign(a, s, shift, s_wave);
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
+  __shared__ int s_wave[kThreads / 64], s_over;
+  if (!s.hash_page) {
+    s.hash_owner = reinterpret_cast<uint64_t*>(s_plan);
+    s.hash_page = reinterpret_cast<int*>(s.hash_owner + s.hash_mask + 1);
+    for (int i = threadIdx.x; i <= s.hash_mask; i += kThreads) {
+      s.hash_owner[i] = 0;
+      s.hash_page[i] = -1;
+    }
+    __syncthreads();
+  }
+  plan_assign<false>(a, s, shift, s_wave, &s_over);
 }
 
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s, int shift) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
+  if (a.B <= kHashSeqs) {                                     // the searches' arrays
+    int* copy = reinterpret_cast<int*>(s_plan);
+    for (int i = threadIdx.x; i <= a.B; i += 256) {
+      copy[i] = s.start[i];
+      copy[a.B + 1 + i] = s.off[i];
+    }
+    s.start = copy;
+    s.off = copy + a.B + 1;
+    __syncthreads();
+  }
   const int step = gridDim.x * 256, at = blockIdx.x * 256 + threadIdx.x;
   const int total = s.off[a.B];
   for (int j = at; j < total; j += step) give_page(a, s, shift, j);
@@ -346,8 +393,8 @@ __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ 
                                                         const int* __restrict__ kv_lens, uint8_t* __restrict__ k,
                                                         uint8_t* __restrict__ v, int64_t pages, int Hkv, int row_bytes, int shift) {
   const int b = blockIdx.x, src = copies[2 * b], dst = copies[2 * b + 1];
-  if (src < 0 || dst < 0) return;
   const int rows = (kv_lens[b] - (q_starts[b + 1] - q_starts[b])) & ((1 << shift) - 1);
+  if (src < 0 || dst < 0) return;
   const int64_t head = (int64_t)row_bytes << shift, page = head * Hkv, layer = (int64_t)blockIdx.y * pages;
   const int vec = rows * (row_bytes / 16), n = vec * Hkv;
   for (int i = threadIdx.x; i < n; i += 256) {
@@ -359,33 +406,48 @@ __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ 
   }
 }
 
-// accept_drafts. Workgroup (sequence, layer): its first wave follows the picks from node 0 down the tree, then the workgroup moves
-// the confirmed nodes' rows of its layer, every head of k and v, to the places behind the sequence's keys. Node d of the path
-// comes to lie at place d <= the node's own, so rows are read and written in order of the path, a chunk's all read before one is
-// written.
+// accept_drafts. Workgroup (sequence, layer): its first wave follows the picks from node 0 down the tree (the first 64 nodes in its
+// lanes, a ballot a step), then the workgroup moves the confirmed nodes' rows of its layer, every head of k and v, to the places
+// behind the sequence's keys: one launch, the walk repeated in every layer. Node d of the path comes to lie at place d <= the
+// node's own, so rows are read and written in order of the path, a chunk's all read before one is written.
 constexpr int kMostPath = 1024;
+__device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+                   (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
 __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
-  __shared__ int s_path[kMostPath];
+  __shared__ int s_path[kMostPath], s_table[64];
   __shared__ int s_count;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int first = min(max(a.q_starts[b], 0), a.T), new_all = min(max(a.q_starts[b + 1], first), a.T) - first;
-  const int past = a.kv_lens[b] - new_all;
+  const int first = min(max(a.q_starts[b], 0), a.T), nodes = min(max(a.q_starts[b + 1], first), a.T) - first;
+  const int past = a.kv_lens[b] - nodes;
+  const int* table = a.table + (int64_t)b * a.width;
+  const int c0 = max(past, 0) >> shift;                       // s_table: the entries from there on
   if (tid < 64) {
     const int64_t* tokens = a.tokens + first;
     const int64_t* picks = a.picks + first;
     const int* parents = a.parents ? a.parents + first : nullptr;
+    int64_t token = 0, pick = 0;
+    int parent = -1;
+    if (lane < nodes) {
+      token = tokens[lane];
+      pick = picks[lane];
+      parent = parents ? parents[lane] : lane - 1;
+    }
     int count = 0, cur = 0;
-    while (count < a.longest && cur < new_all) {
+    while (count < a.longest && cur < nodes) {
       if (lane == 0) s_path[count] = cur;
       ++count;
-      const int64_t want = picks[cur];
-      int next = new_all;
-      for (int n0 = cur + 1; n0 < new_all && next == new_all; n0 += 64) {
-        const int n = n0 + lane;
-        const bool hit = n < new_all && (parents ? parents[n] : n - 1) == cur && tokens[n] == want;
-        const uint64_t any = __ballot(hit);
-        if (any) next = n0 + __builtin_ctzll(any);
-        if (!parents) break;                                  // (a chain: the next token or none)
+      const int64_t want = cur < 64 ? readlane64(pick, cur) : picks[cur];
+      const uint64_t hit = __ballot(lane > cur && lane < nodes && parent == cur && token == want);
+      int next = hit ? __builtin_ctzll(hit) : nodes;
+      if (!hit && (parents || cur >= 63)) {
+        for (int n0 = max(64, cur + 1); n0 < nodes && next == nodes; n0 += 64) {
+          const int n = n0 + lane;
+          const uint64_t any = __ballot(n < nodes && (parents ? parents[n] : n - 1) == cur && tokens[n] == want);
+          if (any) next = n0 + __builtin_ctzll(any);
+          if (!parents) break;                                // (a chain: the next token or none)
+        }
       }
       cur = next;
     }
@@ -402,35 +464,47 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
         a.lens[b] = past + count;
       }
     }
+  } else if (tid < 128 && a.k) {
+    s_table[lane] = c0 + lane < a.width ? table[c0 + lane] : -1;
   }
   __syncthreads();
   const int count = s_count;
   if (!a.k || count == 0 || s_path[count - 1] == count - 1) return;   // (a path that is in its place, as every chain's is)
-  const int pieces = a.row_bytes / 16, heads = 2 * a.Hkv;
+  int from = 0;                                               // the first node that is not in its place; none behind it is
+  for (int n = count - 1; from < n;) {
+    const int mid = (from + n) >> 1;
+    if (s_path[mid] == mid)
+      from = mid + 1;
+    else
+      n = mid;
+  }
+  const int pieces = a.row_bytes / 16, heads = 2 * a.Hkv, groups = 256 / pieces;
   const int64_t head = (int64_t)a.row_bytes << shift, page = head * a.Hkv, layer = (int64_t)blockIdx.y * a.pages;
-  const int* table = a.table + (int64_t)b * a.width;
   // where key `key` lies in this layer, below 0: nowhere
   auto place = [&](int key) -> int64_t {
     const int c = key >> shift;
     if (key < 0 || c >= a.width) return -1;
-    const int id = table[c];
+    const int id = c - c0 < 64 ? s_table[c - c0] : table[c];
     return id < 0 || id >= a.pages ? -1 : (layer + id) * page + (int64_t)(key & ((1 << shift) - 1)) * a.row_bytes;
   };
-  constexpr int kHeld = 8;                                    // pieces of a thread in a chunk
-  const int rows = min(count, kHeld * 256 / pieces), together = max(1, kHeld * 256 / pieces / rows);
+  // a lane group a row of one head; kHeld rows of a group in a chunk
+  constexpr int kHeld = 8;
+  const int grp = tid / pieces, piece = tid - grp * pieces;
+  const int rows = min(count - from, kHeld * groups), together = max(1, kHeld * groups / rows);
   for (int h0 = 0; h0 < heads; h0 += together)
-    for (int d0 = 0; d0 < count; d0 += rows) {
-      const int n = min(rows, count - d0), items = n * pieces * min(together, heads - h0);
+    for (int d0 = from; d0 < count; d0 += rows) {
+      const int n = min(rows, count - d0), items = n * min(together, heads - h0);
       u32x4 held[kHeld];
       int64_t to[kHeld];
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
-        const int i = tid + 256 * u, r = i / pieces, hv = h0 + r / n, d = d0 + r % n;
+        const int i = grp + groups * u;
         to[u] = -1;
-        if (i >= items || s_path[d] == d) continue;
+        if (grp >= groups || i >= items) continue;
+        const int q = (int)((uint32_t)i / (uint32_t)n), hv = h0 + q, d = d0 + i - q * n;
         const int64_t src = place(past + s_path[d]), dst = place(past + d);
         if (src < 0 || dst < 0) continue;
-        const int64_t at = (int64_t)(hv >> 1) * head + 16 * (i % pieces);
+        const int64_t at = (int64_t)(hv >> 1) * head + 16 * piece;
         held[u] = load16((hv & 1 ? a.v : a.k) + src + at);
         to[u] = 2 * (dst + at) + (hv & 1);
       }
@@ -458,32 +532,37 @@ int64_t list_places(const PlanArgs& a, int shift) { return (a.T >> shift) + 2 * 
 
 }  // namespace
 
+// [used][hash_owner, beyond kHashSeqs][hash_page, likewise][row .. start][list]
+static int64_t plan_clear(const PlanArgs& a) {   // 16-byte pieces that have to be zero before
+  return (a.pages + 31) / 32 * 2 + (a.B > kHashSeqs ? hash_places(a.B) / 2 : 0);
+}
 size_t plan_paged_workspace(const PlanArgs& a) {
   if (plan_is_small(a)) return 0;
-  const int64_t ints = 3 * (int64_t)hash_places(a.B) + 2 * map_words(a.pages) + 6 * (int64_t)a.B + 2 + list_places(a, log2_of(a.page_size));
+  const int64_t ints = 4 * plan_clear(a) + (a.B > kHashSeqs ? hash_places(a.B) : 0) + 6 * (int64_t)a.B + 2 + list_places(a, log2_of(a.page_size));
   return (size_t)(4 * ints + 15) / 16 * 16;
 }
 
 hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
   const int shift = log2_of(a.page_size), places = hash_places(a.B);
-  const FastDiv by_width = fast_div(a.width);
   hipError_t e;
   if (plan_is_small(a)) {
     const size_t words = (size_t)map_words(a.pages);
-    const size_t lds = 4 * (3 * (size_t)places + 2 * words + 6 * (size_t)a.B + 2 + kSmallList + kSmallTokens);
-    static_assert(4 * (3 * 2 * kSmallSeqs + 2 * kSmallPages / 32 + 6 * kSmallSeqs + 2 + kSmallList + kSmallTokens) < 160 * 1024 - 256, "LDS");
+    const size_t lds = 4 * (3 * (size_t)places + words + 6 * (size_t)a.B + 2 + kSmallList + kSmallTokens);
+    constexpr size_t most = 4 * (3 * 2 * kSmallSeqs + kSmallPages / 32 + 6 * kSmallSeqs + 2 + kSmallList + kSmallTokens);
+    static_assert(most <= 158 * 1024, "LDS");
     static std::atomic<uint64_t> done{0};
-    if ((e = allow_lds_once(done, plan_small_kernel, 160 * 1024 - 256))) return e;
-    e = launch(plan_small_kernel, dim3(1), dim3(kThreads), lds, st, a, by_width, shift, places - 1);
+    if ((e = allow_lds_once(done, plan_small_kernel, most))) return e;
+    const bool few = a.B <= 256 && a.T <= 1024 && (int64_t)a.B * a.width <= 2048 && a.pages <= 32768;
+    e = launch(plan_small_kernel, dim3(1), dim3(few ? 256 : kThreads), lds, st, a, fast_div(a.width), shift, places - 1);
   } else {
+    const bool far = a.B > kHashSeqs;                         // the hash in the workspace
     PlanState s;
     s.hash_mask = places - 1;
-    s.hash_owner = static_cast<uint64_t*>(a.ws);
-    s.held = reinterpret_cast<uint32_t*>(s.hash_owner + places);
-    const int64_t words = map_words(a.pages);
-    s.whole = s.held + words;
-    s.hash_page = reinterpret_cast<int*>(s.whole + words);
-    s.row = s.hash_page + places;
+    s.used = static_cast<uint32_t*>(a.ws);
+    int* at = reinterpret_cast<int*>(s.used + 4 * plan_clear(a));
+    s.hash_owner = far ? reinterpret_cast<uint64_t*>(s.used + (a.pages + 31) / 32 * 8) : nullptr;
+    s.hash_page = far ? at : nullptr;
+    s.row = at + (far ? places : 0);
     s.past = s.row + a.B;
     s.fresh = s.past + a.B;
     s.tail = s.fresh + a.B;
@@ -491,14 +570,20 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     s.start = s.off + a.B + 1;
     s.list = s.start + a.B + 1;
     s.list_cap = (int)list_places(a, shift);
-    const int64_t clear = (2 * (int64_t)places + 2 * words + kThreads - 1) / kThreads;
-    e = launch(plan_lens_kernel, dim3((unsigned)(1 + std::min<int64_t>(clear, 512))), dim3(kThreads), 0, st, a, s, shift, (int)words);
-    const int64_t entries = (int64_t)a.B * a.width;
+    const int64_t clear = plan_clear(a);
+    e = launch(plan_lens_kernel, dim3((unsigned)(1 + std::min<int64_t>((clear + kThreads - 1) / kThreads, 512))), dim3(kThreads), 0, st,
+               a, s, shift, clear);
+    const int chunks = (a.width + 1023) / 1024;
+    if (e == hipSuccess) e = launch(plan_mark_kernel, dim3((unsigned)(a.B * chunks)), dim3(256), 0, st, a, s, chunks, shift);
+    if (e == hipSuccess && !far && 12 * places > 65536) {
+      static std::atomic<uint64_t> done{0};
+      e = allow_lds_once(done, plan_assign_kernel, 12 * 2 * kHashSeqs);
+    }
+    if (e == hipSuccess) e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places, st, a, s, shift);
+    const int64_t items = std::max<int64_t>(a.T, a.B);
     if (e == hipSuccess)
-      e = launch(plan_mark_kernel, dim3((unsigned)std::min<int64_t>((entries + 255) / 256, 4096)), dim3(256), 0, st, a, s, by_width, shift);
-    if (e == hipSuccess) e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), 0, st, a, s, shift);
-    const int64_t items = std::max<int64_t>({(int64_t)a.T, (int64_t)a.B, 1});
-    if (e == hipSuccess) e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256), 0, st, a, s, shift);
+      e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256),
+                 far ? 0 : 8 * (size_t)(a.B + 1), st, a, s, shift);
   }
   if (e != hipSuccess || !a.k) return e;
   return launch(plan_copy_kernel, dim3((unsigned)a.B, (unsigned)a.layers), dim3(256), 0, st, static_cast<const int*>(a.copies),

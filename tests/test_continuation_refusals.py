@@ -39,7 +39,7 @@ beam = call("lowbit_beam_select", dict(
 
 LAYERS = [(dict(v=None, k=FAKE), 1, "goes with"), (dict(k=None, v=FAKE), 1, "goes with"), (dict(k=FAKE, v=FAKE, layers=0), 3, "layers"),
           (dict(k=FAKE, v=FAKE, layers=65536), 3, "layers"), (dict(k=FAKE, v=FAKE, row=24), 3, "multiple of 16"),
-          (dict(k=FAKE, v=FAKE, row=0), 3, "multiple of 16"), (dict(k=FAKE, v=FAKE, row=32784), 3, "multiple of 16"),
+          (dict(k=FAKE, v=FAKE, row=0), 3, "multiple of 16"), (dict(k=FAKE, v=FAKE, row=4112), 3, "multiple of 16"),
           (dict(k=FAKE, v=FAKE, hkv=0), 3, "layers"), (dict(k=FAKE, v=FAKE, hkv=65536, ps=65536), 3, "2^34"),
           (dict(k=ODD8, v=FAKE), 4, "16-byte"), (dict(k=FAKE, v=ODD8), 4, "16-byte"), (dict(ps=24), 3, "power of two"),
           (dict(ps=8), 3, "power of two"), (dict(ps=1 << 17), 3, "power of two"), (dict(pages=0), 3, "pages"),
