@@ -353,12 +353,16 @@ size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_
 /* lowbit_attention_paged where sequences' new tokens are trees of drafts (or any set that a mask describes): new token i attends the
  * keys before its sequence's new ones (0 .. kv_lens[b] - new - 1) and, of the new ones', those whose bit is set in its words masks[t
  * * words ..] (t its row of q; bit j % 64 of word j / 64 for new token j, its own among them only if it is set; new tokens past 64
- * * words are attended by none; 1 <= words <= 16). One that attends nothing gets zeros. The same workspace. */
+ * * words are attended by none; 1 <= words <= 16). One that attends nothing gets zeros. workspace as there,
+ * lowbit_attention_paged_tree_workspace says how much the call has use for. */
 int lowbit_attention_paged_tree(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                                 int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, const uint64_t* masks,
                                 int64_t words, void* out, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                 int64_t pages, int64_t page_size, int64_t max_new, int64_t max_keys, float scale,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+size_t lowbit_attention_paged_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                                             int64_t page_size, int64_t max_new, int64_t max_keys);
 
 /* The tables of a step, from its sequences' lengths, without the host. Sequence b goes on from row r = rows[b] of page_table [R][width]
  * (rows NULL: r = b, R = B; a row outside the table: a sequence without keys), whose first past[r] (int32 [R]) keys it has, by

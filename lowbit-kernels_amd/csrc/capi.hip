@@ -711,6 +711,14 @@ size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_
   return attention_paged_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
 }
 
+size_t lowbit_attention_paged_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
+                                             int64_t page_size, int64_t max_new, int64_t max_keys) {
+  if (check_paged("attention_paged_tree", LOWBIT_DTYPE_F16, Hq, Hkv, D, 1, page_size) ||
+      check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
+    return 0;
+  return attention_paged_tree_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
+}
+
 // attention_paged and attention_paged_tree (masks not NULL)
 static int attend_pages(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
                         int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens, void* out, int64_t T,

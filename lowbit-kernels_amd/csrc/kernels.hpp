@@ -402,6 +402,7 @@ struct PagedAttentionArgs {
 };
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st);
 hipError_t attention_paged_tree_launch(const PagedAttentionArgs& a, hipStream_t st);   // (paged_tree.hip)
+size_t attention_paged_tree_workspace(const PagedAttentionArgs& a);
 size_t attention_paged_workspace(const PagedAttentionArgs& a);   // bytes that the launch has use for; reads sizes and bounds only
 
 // ---- a step's tables, and drafts accepted (plan.hip) ----

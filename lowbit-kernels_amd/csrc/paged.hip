@@ -150,8 +150,8 @@ size_t attention_paged_workspace(const PagedAttentionArgs& a) {
 }
 
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st) {
-  if (a.bf16) return a.D == 64 ? pick_paged_attention<bf16, 64, false>(a, st) : pick_paged_attention<bf16, 128, false>(a, st);
-  return a.D == 64 ? pick_paged_attention<f16, 64, false>(a, st) : pick_paged_attention<f16, 128, false>(a, st);
+  if (a.bf16) return a.D == 64 ? pick_paged_attention<bf16, 64>(a, st) : pick_paged_attention<bf16, 128>(a, st);
+  return a.D == 64 ? pick_paged_attention<f16, 64>(a, st) : pick_paged_attention<f16, 128>(a, st);
 }
 
 }  // namespace lowbit

@@ -47,8 +47,11 @@ struct PagedPlan {
   int Hq, Hkv, G;
   FastDiv by_hkv, by_g;
 };
+struct PagedTile {   // kTree: a tile as the join of its parts finds it
+  int first, nq, len, tile, hk, parts, rec, unused;
+};
 struct PagedUnit {
-  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec;   // first: the sequence's first row of q; rec: the part's record (parts > 1)
+  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec, tile_no;   // tile_no (kTree): of the split tiles; first: the sequence's first row of q; rec: the part's record (parts > 1)
 };
 
 // sum of the lanes up to and including this one
@@ -84,6 +87,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int se
 // keys far above the mean are cut (us with half a round, one, one and a half and two: 64 decode tokens of 32 / 8 heads on 300 ..
 // 8000 keys 147, 133, 129 and 128; a prompt of 2000 tokens, 28 / 4 heads, 64, 71, 71 and 79; a mixed step 33.8, 34.2, 34.7 and
 // 34.8). s0: the first 64 sequences.
+constexpr int kEvenSeqs = 256;
 template <int kRows, int kBlock, bool kTree>
 __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {
   if (p.cap == 1) return 0x3FFFFFFF;
@@ -96,21 +100,30 @@ __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan&
   total *= (float)p.Hkv;
   units *= (float)p.Hkv;
   const float slots = (float)p.slots;
-  if (kTree && b.B <= 64) {
+  if (kTree && b.B <= kEvenSeqs) {
     // the least share whose parts, each sequence's rounded up, run at once (as many rounds of slots as tiles of one part need)
     const float room = fminf(ceilf(units / slots) * slots, fmaxf((float)p.most, units));
-    int lo = max(p.least, (int)fminf(total / room, 1e9f)), hi = 1 << 26;
-    auto fits = [&](int share) {
-      return wave_sum((float)(s0.tiles * max(1, min(p.cap, (s0.blocks + share - 1) / share)))) * (float)p.Hkv <= room;
-    };
-    if (fits(lo)) return lo;
-    int step = max(1, lo >> 4);
-    while (!fits(lo + step) && lo + step < hi) {
-      lo += step;
-      step += step;
+    int tiles[kEvenSeqs / 64], blocks[kEvenSeqs / 64];
+    tiles[0] = s0.tiles;
+    blocks[0] = s0.blocks;
+#pragma unroll
+    for (int i = 1; i < kEvenSeqs / 64; ++i) {
+      const PagedSeq s = paged_seq<kRows, kBlock>(b, p.G, 64 * i + lane);
+      tiles[i] = s.tiles;
+      blocks[i] = s.blocks;
     }
-    hi = lo + step;
-    while (hi - lo > max(1, lo >> 5)) {
+    auto fits = [&](int share) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kEvenSeqs / 64; ++i)
+        if (64 * i < b.B) n += tiles[i] * max(1, min(p.cap, (int)((uint32_t)(blocks[i] + share - 1) / (uint32_t)share)));
+      return wave_sum((float)n) * (float)p.Hkv <= room;
+    };
+    const float free = room - units;                          // (parts rounded up: at most total / share and one a tile)
+    if (free < 1.f) return 1 << 26;
+    int lo = max(p.least, (int)fminf(total / room, 1e8f)), hi = max(lo, (int)fminf(ceilf(total / free), 1e8f));
+    if (fits(lo)) return lo;
+    while (hi - lo > max(1, lo >> 4)) {                       // (lo does not fit, hi does)
       const int mid = (lo + hi) >> 1;
       if (fits(mid))
         hi = mid;
@@ -128,12 +141,13 @@ __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan&
 template <int kRows, int kBlock, int kMerge, bool kTree>
 __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int share, int idx,
                                            int lane, PagedUnit& u) {
-  int before = 0, recs = 0;                                  // work and record groups of the sequences before
+  int before = 0, recs = 0, tiles_before = 0;                // work, record groups and tiles of the sequences before
   for (int b0 = 0; b0 < b.B; b0 += 64) {
     const PagedSeq s = b0 == 0 ? s0 : paged_seq<kRows, kBlock>(b, p.G, b0 + lane);
     const int parts = p.cap == 1 ? 1 : max(1, min(p.cap, (s.blocks + share - 1) / share));
     const int tiles = s.tiles * p.Hkv, split = parts > 1 ? tiles * parts : 0;
     const int mine = kMerge == 0 ? tiles * parts : parts > 1 ? (s.nq * p.G + max(kMerge, 1) - 1) / max(kMerge, 1) * p.Hkv : 0;
+    [[maybe_unused]] const int tiles_upto = kTree ? wave_scan(parts > 1 ? tiles : 0) : 0;
     const int upto = wave_scan(mine), recs_upto = p.cap == 1 ? 0 : wave_scan(split);
     const uint64_t hit = __ballot(idx - before < upto);
     if (hit) {
@@ -155,6 +169,7 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
         u.pid = div(part, p.by_hkv);
         u.hk = part - u.pid * p.Hkv;
         u.tile = t;
+        u.tile_no = tiles_before + pick(tiles_upto - tiles) + t * p.Hkv + u.hk;   // (used of more than one part)
       } else if constexpr (kMerge == 0) {
         const int t = u.parts == 1 ? rest : (int)((uint32_t)rest / (uint32_t)u.parts);
         u.pid = rest - t * u.parts;
@@ -170,6 +185,7 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, const PagedPlan&
              (u.parts == 1 || (u.rec >= 0 && u.rec <= p.most - (kMerge == 0 ? 1 : u.parts)));
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    if constexpr (kTree) tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
     if (p.cap > 1) recs += __builtin_amdgcn_readlane(recs_upto, 63);
   }
   return false;
@@ -308,7 +324,7 @@ __device__ __forceinline__ float score_scale(float scale) {
 template <typename T, int D, int RG, int KG, bool kTree>
 __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, PagedBatch bt, PagedPlan plan,
-    T* __restrict__ out, float* __restrict__ part, int shift, float scale) {
+    T* __restrict__ out, float* __restrict__ part, PagedTile* __restrict__ tiles, int shift, float scale) {
   constexpr int NW = RG * KG;
   constexpr int RB = D * 2;                                  // bytes of a row
   constexpr int PR = RB / 16;                                // its pieces
@@ -330,7 +346,20 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
   const int j = lane & 31, h = lane >> 5;
   PagedUnit un;
   const PagedSeq s0 = paged_seq<kRows, BK>(bt, G, lane);
-  if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, paged_share<kRows, BK, kTree>(bt, plan, s0, lane), blockIdx.x, lane, un)) return;
+  const int share = paged_share<kRows, BK, kTree>(bt, plan, s0, lane);
+  if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, share, blockIdx.x, lane, un)) return;
+  if constexpr (kTree) {                                      // for the join: tiles[0].parts is how many follow
+    if (plan.cap > 1 && blockIdx.x == 0 && wave == 0) {
+      float split = 0.f;                                      // (below 2^24: exact)
+      for (int at = 0; at < bt.B; at += 64) {
+        const PagedSeq s = at == 0 ? s0 : paged_seq<kRows, BK>(bt, G, at + lane);
+        split += wave_sum((float)(s.blocks > share ? s.tiles : 0));
+      }
+      if (lane == 0) tiles[0].parts = (int)split * Hkv;
+    }
+    if (un.parts > 1 && un.pid == 0 && tid == 0)
+      tiles[1 + un.tile_no] = PagedTile{un.first, un.nq, un.len, un.tile, un.hk, un.parts, un.rec, 0};
+  }
   const int rgrp = wave % RG, kgrp = wave / RG;
   const int cap = bt.table_width * bt.page_size;
   const int len = min(un.len, cap);                  // keys that can be read
@@ -720,7 +749,7 @@ template <int kRows>
 constexpr int paged_merge_groups() { return kRows == 32 ? 4 : 1; }
 template <int D, int kRows>
 constexpr int paged_merge_rows() { return 1024 / D / paged_merge_groups<kRows>(); }
-template <typename T, int D, int kRows, int kBlock, bool kTree>
+template <typename T, int D, int kRows, int kBlock>
 __global__ __launch_bounds__(256) void paged_attention_merge(const float* __restrict__ part, PagedBatch bt, PagedPlan plan,
                                                              T* __restrict__ out, float scale) {
   constexpr int kLanes = D / 4, PG = paged_merge_groups<kRows>(), kHere = paged_merge_rows<D, kRows>(), kRec = paged_rec<D>();
@@ -731,9 +760,9 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
   const int lane = threadIdx.x & 63, grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   const float c2 = score_scale(scale);
   const PagedSeq s0 = paged_seq<kRows, kBlock>(bt, plan.G, lane);
-  const int share = paged_share<kRows, kBlock, kTree>(bt, plan, s0, lane);
+  const int share = paged_share<kRows, kBlock, false>(bt, plan, s0, lane);
   PagedUnit un;
-  for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere, kTree>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
+  for (int idx = blockIdx.x; paged_unit<kRows, kBlock, kHere, false>(bt, plan, s0, share, idx, lane, un); idx += gridDim.x) {
     const int r = un.pid * kHere + grp / PG, row = un.tile * kRows + r;
     const float* rec = part + ((size_t)un.rec * kRows + r) * kRec;
     const size_t step = (size_t)kRows * kRec;
@@ -794,9 +823,97 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
       }
       const int tok = div(row, plan.by_g), g = row - tok * plan.G;
       store_row<T>(out + ((int64_t)(un.first + tok) * plan.Hq + un.hk * plan.G + g) * D + 4 * c, num, den,
-                   some_key<kTree>(bt, un, tok));
+                   un.len - un.nq + tok >= 0);
     }
     if constexpr (PG > 1) __syncthreads();
+  }
+}
+
+// The same for trees: the main kernel leaves the split tiles in tiles[], so that no workgroup looks for its own (at 16 sequences, whose
+// share takes some steps to find, the join takes 7.2 us instead of 14.3). PG groups of D / 4 lanes a row, each for a run of the parts: a lane reads the references and sums of one part each, and the
+// output's four values of all of them.
+template <typename T, int D, int kRows, int PG>
+__global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict__ part, const PagedTile* __restrict__ tiles,
+                                                        PagedBatch bt, PagedPlan plan, T* __restrict__ out, float scale) {
+  constexpr int kLanes = D / 4, kHere = 256 / kLanes / PG, kChunks = kRows / kHere, kRec = paged_rec<D>();
+  __shared__ f32x4 s_num[PG > 1 ? 256 : 1];
+  __shared__ float s_top[256 / kLanes], s_den[256 / kLanes];
+  const int c = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int work = tiles[0].parts * kChunks;
+  const float c2 = score_scale(scale);
+  for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
+    const PagedTile t = tiles[1 + idx / kChunks];
+    const int r = idx % kChunks * kHere + grp / PG, row = t.tile * kRows + r;
+    const float* rec = part + ((size_t)t.rec * kRows + r) * kRec;
+    const size_t step = (size_t)kRows * kRec;
+    const int per = (t.parts + PG - 1) / PG, p1 = min(t.parts, (grp % PG + 1) * per);
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f, top = -INFINITY;
+    if (row < t.nq * plan.G) {
+      for (int p0 = grp % PG * per; p0 < p1; p0 += kLanes) {
+        const int n = min(kLanes, p1 - p0);
+        float m = -INFINITY, l = 0.f;
+        if (c < n) {
+          const float2 ml = *reinterpret_cast<const float2*>(rec + (size_t)(p0 + c) * step);
+          m = ml.x;
+          l = ml.y;
+        }
+        float nm = fmaxf(top, m);
+#pragma unroll
+        for (int off = 1; off < kLanes; off <<= 1) nm = fmaxf(nm, __shfl_xor(nm, off, kLanes));
+        const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - nm) * c2);
+        num *= f0;
+        top = nm;
+        // (no score of a part's keys above -inf: its sums are zeros, or NaN where a score was, which factor 0 keeps)
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c2);
+        float d = f * l;
+#pragma unroll
+        for (int off = 1; off < kLanes; off <<= 1) d += __shfl_xor(d, off, kLanes);
+        den = fmaf(den, f0, d);
+        const float* at = rec + (size_t)p0 * step + 4 + 4 * c;
+        for (int i = 0; i < n; i += 8) {                      // eight records' loads in flight
+          f32x4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4*>(at + (size_t)min(i + u, n - 1) * step);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float g = __shfl(f, min(i + u, n - 1), kLanes);
+            if (i + u < n) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) num[e] = fmaf(g, v[u][e], num[e]);
+            }
+          }
+        }
+      }
+    }
+    if constexpr (PG > 1) {
+      __syncthreads();                                        // (the round before has been read)
+      s_num[threadIdx.x] = num;
+      if (c == 0) {
+        s_top[grp] = top;
+        s_den[grp] = den;
+      }
+      __syncthreads();
+      if (grp % PG) continue;
+#pragma unroll
+      for (int i = 1; i < PG; ++i) top = fmaxf(top, s_top[grp + i]);
+      num = f32x4{0.f, 0.f, 0.f, 0.f};
+      den = 0.f;
+#pragma unroll
+      for (int i = 0; i < PG; ++i) {
+        const float m = s_top[grp + i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c2);
+        den = fmaf(f, s_den[grp + i], den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + i * kLanes][e], num[e]);
+      }
+    }
+    if (row >= t.nq * plan.G) continue;
+    const int tok = div(row, plan.by_g), g = row - tok * plan.G;
+    PagedUnit un{};
+    un.first = t.first;
+    un.nq = t.nq;
+    un.len = t.len;
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den, some_key<true>(bt, un, tok));
   }
 }
 
@@ -850,6 +967,32 @@ inline PagedLaunch paged_launch(const PagedAttentionArgs& a) {
   return p;
 }
 
+// The same for trees, whose rows all attend nearly all keys. Two tiles: 32 rows on four key groups while those tiles fit the CUs and
+// the products are few, so that latency counts, else 128 rows (28 / 4 heads, graph-timed us, 32 / 128 rows: one tree of 64 nodes on
+// 500 keys 14.3 / 18.4, on 3000 21.1 / 24.3, on 30000 79 / 55; 4 of 32 on 1000 18.8 / 21.3; 8 of 16 on 2000 22.7 / 23.3; 16 of 31 .. 63
+// on 300 .. 8000 92 / 50; 14 / 2 heads of 64, 16 of 26 on 300 8.7 / 12.3). One launch, keys not split, where a split and its join (5 to
+// 10 us) cost more than the longest tile's walk is shortened by: 32 rows, whole / split: one tree of 26 on 926 keys, 16 / 2 heads,
+// 16.9 / 13.5, one of 64 on 564 14.3 / 15.9, 4 of 32 on 1000 18.8 / 22.0; 128 rows: 32 of 16 on 500 21.5 / 27.9, 64 of 32 on 1000 54 /
+// 60, 40 of 5 on 2000 51 / 42.
+inline PagedLaunch tree_launch(const PagedAttentionArgs& a) {
+  const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T), rows = (int64_t)a.batch.T * G;
+  auto tiles = [&](int n) { return ((rows + n - 1) / n + seqs) * a.Hkv; };   // at most
+  PagedLaunch p{};
+  const bool small = tiles(32) <= 256 && (rows / 32 + 1) * a.Hkv * (a.max_keys / 32 + 1) <= 12288;
+  p.rg = small ? 1 : 4;
+  p.kg = small ? 4 : 1;
+  const int block = 32 * p.kg;
+  p.slots = 256 * paged_per_cu(p.rg, p.kg);
+  p.units = tiles(32 * p.rg);
+  p.least = small ? 1 : kPagedLeast / block;
+  const int64_t blocks = ((int64_t)a.max_keys + block - 1) / block;
+  const bool whole = small ? a.max_keys <= kPagedWhole || (a.max_keys <= 2 * kPagedWhole && p.units >= 64)
+                           : blocks <= 64 && blocks * (p.slots - p.units) <= 5120;
+  p.cap = whole ? 1 : std::min(kPagedParts, (int)((blocks + p.least - 1) / p.least));
+  p.records = p.cap == 1 ? 0 : (int)std::min<int64_t>(small ? 1024 : 2048, 2 * p.units * p.cap);
+  return p;
+}
+
 inline size_t paged_record_bytes(int rg, int D) { return (size_t)32 * rg * (D == 64 ? paged_rec<64>() : paged_rec<128>()) * sizeof(float); }
 
 template <typename T, int D, int RG, int KG, bool kTree>
@@ -859,11 +1002,15 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
   constexpr int kRows = 32 * RG, kBlock = 32 * KG;
   const int G = a.Hq / a.Hkv;
   PagedPlan p{l.slots, l.least, 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
-  p.most = a.ws ? (int)std::min<size_t>((size_t)l.records, a.ws_bytes / paged_record_bytes(RG, D)) : 0;
+  // kTree: the tiles' descriptions before the records
+  const size_t head = kTree ? (size_t)(l.units + 1) * sizeof(PagedTile) : 0;
+  p.most = a.ws && a.ws_bytes > head ? (int)std::min<size_t>((size_t)l.records, (a.ws_bytes - head) / paged_record_bytes(RG, D)) : 0;
   if (p.most >= 2) p.cap = l.cap;
+  PagedTile* tiles = kTree && p.cap > 1 ? static_cast<PagedTile*>(a.ws) : nullptr;
+  float* records = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + head);
   // (paged_share: parts take its free slots beside one a tile, or those of whole rounds)
   const int64_t rounds = (l.units + l.slots - 1) / l.slots * l.slots;
-  const int64_t split = kTree && a.batch.B <= 64 ? std::max(l.units, std::min<int64_t>(rounds, p.most)) : l.units + p.most / 2 + 1;
+  const int64_t split = kTree && a.batch.B <= kEvenSeqs ? std::max(l.units, std::min<int64_t>(rounds, p.most)) : l.units + p.most / 2 + 1;
   const int64_t grid = p.cap == 1 ? l.units : std::min<int64_t>(l.units * p.cap, split);
   if (lds > 65536) {
     static std::atomic<uint64_t> done{0};
@@ -872,20 +1019,35 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
   const int shift = log2_of(a.batch.page_size);
   hipError_t e = launch(paged_attention<T, D, RG, KG, kTree>, dim3((unsigned)grid), dim3(64 * RG * KG), lds, st,
                         static_cast<const T*>(a.q), static_cast<const T*>(a.k_cache), static_cast<const T*>(a.v_cache),
-                        a.batch, p, static_cast<T*>(a.out), static_cast<float*>(a.ws), shift, a.scale);
+                        a.batch, p, static_cast<T*>(a.out), records, tiles, shift, a.scale);
   if (e != hipSuccess || p.cap == 1) return e;
+  if constexpr (kTree) {
+    // four groups a row while that many workgroups run at once: few rows of many parts
+    const int64_t work = l.units * (kRows * D / 1024);
+    auto join = [&](auto kernel, int64_t n) {
+      return launch(kernel, dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(256), 0, st, static_cast<const float*>(records),
+                    static_cast<const PagedTile*>(tiles), a.batch, p, static_cast<T*>(a.out), a.scale);
+    };
+    return 4 * work <= 2048 ? join(paged_tree_merge<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge<T, D, kRows, 1>, work);
+  } else {
   constexpr int kHere = paged_merge_rows<D, kRows>();
   const int64_t seqs = std::min(a.batch.B, a.batch.T), chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
-  return launch(paged_attention_merge<T, D, kRows, kBlock, kTree>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
+  return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
                 static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.scale);
+  }
 }
 
-template <typename T, int D, bool kTree>
+template <typename T, int D>
 hipError_t pick_paged_attention(const PagedAttentionArgs& a, hipStream_t st) {
   const PagedLaunch l = paged_launch(a);
-  if (l.rg == 4) return launch_paged_attention<T, D, 4, 1, kTree>(a, l, st);
-  if (l.rg == 2) return launch_paged_attention<T, D, 2, 2, kTree>(a, l, st);
-  return l.kg == 4 ? launch_paged_attention<T, D, 1, 4, kTree>(a, l, st) : launch_paged_attention<T, D, 1, 1, kTree>(a, l, st);
+  if (l.rg == 4) return launch_paged_attention<T, D, 4, 1, false>(a, l, st);
+  if (l.rg == 2) return launch_paged_attention<T, D, 2, 2, false>(a, l, st);
+  return l.kg == 4 ? launch_paged_attention<T, D, 1, 4, false>(a, l, st) : launch_paged_attention<T, D, 1, 1, false>(a, l, st);
+}
+template <typename T, int D>
+hipError_t pick_tree_attention(const PagedAttentionArgs& a, hipStream_t st) {
+  const PagedLaunch l = tree_launch(a);
+  return l.rg == 4 ? launch_paged_attention<T, D, 4, 1, true>(a, l, st) : launch_paged_attention<T, D, 1, 4, true>(a, l, st);
 }
 
 }  // namespace lowbit

@@ -4,9 +4,14 @@
 
 namespace lowbit {
 
+size_t attention_paged_tree_workspace(const PagedAttentionArgs& a) {
+  const PagedLaunch l = tree_launch(a);
+  return l.cap == 1 ? 0 : (l.units + 1) * sizeof(PagedTile) + l.records * paged_record_bytes(l.rg, a.D);
+}
+
 hipError_t attention_paged_tree_launch(const PagedAttentionArgs& a, hipStream_t st) {
-  if (a.bf16) return a.D == 64 ? pick_paged_attention<bf16, 64, true>(a, st) : pick_paged_attention<bf16, 128, true>(a, st);
-  return a.D == 64 ? pick_paged_attention<f16, 64, true>(a, st) : pick_paged_attention<f16, 128, true>(a, st);
+  if (a.bf16) return a.D == 64 ? pick_tree_attention<bf16, 64>(a, st) : pick_tree_attention<bf16, 128>(a, st);
+  return a.D == 64 ? pick_tree_attention<f16, 64>(a, st) : pick_tree_attention<f16, 128>(a, st);
 }
 
 }  // namespace lowbit

@@ -72,6 +72,7 @@ SIGNATURES = {
     "lowbit_attention_paged_workspace": ([_i64] * 9, ctypes.c_size_t),
     "lowbit_attention_paged_tree": ([_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
                                      _i64, _i64, _i64, _i64, ctypes.c_float, _vp, ctypes.c_size_t, _vp], _int),
+    "lowbit_attention_paged_tree_workspace": ([_i64] * 9, ctypes.c_size_t),
     "lowbit_plan_paged_workspace": ([_i64] * 5, ctypes.c_size_t),
     "lowbit_plan_paged": ([_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                            _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp], _int),
@@ -322,6 +323,7 @@ class NativeExt:
         self.lib = lib()
         # (of sizes alone, and every layer of a step asks for the same ones)
         self._paged_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_attention_paged_workspace)
+        self._tree_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_attention_paged_tree_workspace)
         self._plan_workspace = functools.lru_cache(maxsize=64)(self.lib.lowbit_plan_paged_workspace)
 
     def w4_gemv(self, x, w, s, group, version, rows_per_warp=0):
@@ -790,7 +792,8 @@ class NativeExt:
             return
         # the split tiles' records, from the caching allocator for this call alone: calls on several streams and captured
         # graphs share none
-        nbytes = self._paged_workspace(t, batch, hq, hkv, dim, width, page_size, int(max_new), int(max_keys)) if split else 0
+        use = self._paged_workspace if masks is None else self._tree_workspace
+        nbytes = use(t, batch, hq, hkv, dim, width, page_size, int(max_new), int(max_keys)) if split else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         if masks is not None:
             _launch(index, lambda stream, _ws, _nbytes: self.lib.lowbit_attention_paged_tree(

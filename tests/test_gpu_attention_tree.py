@@ -144,12 +144,17 @@ def test_any_mask(cuda, dt):
 
 
 def test_a_causal_mask_is_causal_attention(cuda):
+    """Both calls lie within the definition's bound of it, so within twice that of each other (not the same bits: the two calls cut
+    rows and keys differently, which changes the order of the sums)."""
     lens = [(30, 200), (1, 900), (64, 64)]
     x = batch(lens, 28, 4, 128, 16, torch.float16, 4)
     causal = call(x, torch.cat([pack(torch.ones(n, n).tril().bool(), 1) for n, _ in lens]).cuda(), 0.09, 64, 900)
     out = torch.empty_like(x[0])
     ops.ext().attention_paged(*x[:6], out, 64, 900, 0.09)
-    assert torch.equal(causal, out)
+    for b, (n, keys) in enumerate(lens):
+        rows = slice(x[7][b], x[7][b + 1])
+        _, tol, _ = want_of(x[0][rows], *x[6][b], n, keys, torch.ones(n, n).tril().bool(), 0.09)
+        assert bool(((causal[rows].double() - out[rows].double()).abs() <= 2 * tol).all())
 
 
 def test_rows_without_keys(cuda):
