@@ -402,33 +402,46 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
 }
 
 // ---- beam_select ----
-// A workgroup of `blockDim / 64` waves per request. A wave takes a beam: its slices' sums are joined, and of their lists what
-// reaches a bound is ranked by counting, into the beam's n best, score + (x - max) - log z in 64 bits (which of two beams' tokens
-// comes first goes by that difference). The bound: at least n logits reach the n-th largest of the slices' first ones, or, of S < n
-// slices, the least of their ceil(n / S)-th ones. Then all beams' n best are ranked by counting, a few threads a candidate.
+// A workgroup per request. The slices' sums are joined, 16 lanes a beam; a candidate's score is then score + (x - max) - log z, in 64
+// bits (which of two beams' tokens comes first goes by that difference). The n-th largest of 64 maxima, each of some of the slices'
+// first scores, bounds what can be among the n best: of all slices' lists what reaches it is ranked by counting, a few lanes a
+// candidate. Where that is too little (few beams hold anything) or too much (ties), each beam's own n best are made first, a
+// wave a beam, and those ranked.
 // A beam that holds nothing (a score that is no finite number) or whose row has no distribution has -inf for every token, a
 // finished one its score for `pad` and -inf for the others; equal candidates rank by beam, then by token.
-__global__ __launch_bounds__(512) void beam_join_kernel(const float* __restrict__ scores, const uint8_t* __restrict__ finished,
-                                                       float* __restrict__ out_scores, int64_t* __restrict__ out_beams,
-                                                       int64_t* __restrict__ out_tokens, int W, int V, int n, int pad, int S,
-                                                       const Sums* __restrict__ part, const uint64_t* __restrict__ part_keys) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, req = blockIdx.x;
+constexpr int kBeamSlices = 16, kBeamThreads = 512;
+constexpr int kBeamList = 1024;
+constexpr int kBeamWhole = 128 * 1024;   // LDS of the lists of whole beams
+struct BeamJoin {
+  const float* scores;
+  const uint8_t* finished;
+  float* out_scores;
+  int64_t *out_beams, *out_tokens;
+  int W, V, n, pad, S, depth;                                 // depth: of each slice's list, scores that the bound is taken of
+  const Sums* part;
+  const uint64_t* keys;
+};
+
+// each beam's n best, then the n best of those
+__device__ __forceinline__ void beam_join_whole(const BeamJoin& a, uint8_t* smem, int req) {
+  const int W = a.W, V = a.V, n = a.n, S = a.S, pad = a.pad;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int have = min(n, V);                                 // candidates of a beam
   double* s_value = reinterpret_cast<double*>(smem);          // [W][have]
   int* s_token = reinterpret_cast<int*>(s_value + W * n);     // (rounded up to a multiple of two)
-  uint64_t* s_keys = reinterpret_cast<uint64_t*>(s_token + ((W * n + 1) & ~1)) + wave * 2 * S * n;
-  uint64_t* s_list = s_keys + S * n;
-  for (int w = wave; w < W; w += waves) {
+  uint64_t* s_all = reinterpret_cast<uint64_t*>(s_token + ((W * n + 1) & ~1));
+  const int waves = max(1, min(kBeamThreads / 64, (kBeamWhole - W * n * 12 - 8) / (16 * S * n)));   // as many as LDS holds the lists of
+  uint64_t *s_keys = s_all + wave * 2 * S * n, *s_list = s_keys + S * n;
+  for (int w = wave; w < W && wave < waves; w += waves) {
     const int64_t row = (int64_t)req * W + w;
-    const uint64_t* keys = part_keys + row * S * n;
-    const float score = scores[row];
-    const uint8_t flag = finished ? finished[row] : 0;
-    Sums s = lane < S ? part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};   // (of a row that was not read: not used)
+    const uint64_t* keys = a.keys + row * S * n;
+    const float score = a.scores[row];
+    const uint8_t flag = a.finished ? a.finished[row] : 0;
+    Sums s = lane < S ? a.part[row * S + lane] : Sums{-INFINITY, 0.f, 0.f};   // (of a row that was not read: not used)
+    for (int i = lane; i < S * n; i += 64) s_keys[i] = keys[i];
     const bool held = fabsf(score) <= FLT_MAX, done = held && flag;
     bool none = !held;
     if (held && !done) {
-      for (int i = lane; i < S * n; i += 64) s_keys[i] = keys[i];
       const float m = wave_max(s.m);
       move_sums(s.m, m, s.z, s.e);
       const float z = wave_sum(s.z);
@@ -481,8 +494,8 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const float* __restrict_
   // a candidate's rank, counted by `per` lanes side by side
   const int all = W * have;
   int per = 1;
-  while (per < 16 && 2 * per * all <= (int)blockDim.x) per *= 2;
-  for (int c0 = 0; c0 < all; c0 += (int)blockDim.x / per) {
+  while (per < 16 && 2 * per * all <= kBeamThreads) per *= 2;
+  for (int c0 = 0; c0 < all; c0 += kBeamThreads / per) {
     const int c = c0 + (int)threadIdx.x / per;
     const double v = c < all ? s_value[c] : 0.0;
     int rank = 0;
@@ -494,15 +507,142 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const float* __restrict_
     for (int off = 1; off < per; off <<= 1) rank += __shfl_xor(rank, off, 64);
     if (c >= all || rank >= n || (int)threadIdx.x % per) continue;
     const int64_t to = (int64_t)req * n + rank;
-    out_scores[to] = (float)v;
-    out_beams[to] = c / have;
-    out_tokens[to] = s_token[c];
+    a.out_scores[to] = (float)v;
+    a.out_beams[to] = c / have;
+    a.out_tokens[to] = s_token[c];
   }
 }
 
-// slices: up to 1024 workgroups, four a CU, of at least 2048 logits
-static int row_slices(int M, int V, int top, size_t ws_bytes) {
-  const int S = M < 512 ? (int)std::min<int64_t>({1024 / M, V / 2048, (int64_t)kMaxSlices}) : 1;
+// the sum, or the largest, over the 16 lanes of a row; every lane of the row gets it
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp<kQuadSwap1>(v));
+  v = fmaxf(v, dpp<kQuadSwap2>(v));
+  v = fmaxf(v, dpp<kRowHalfMirror>(v));
+  return fmaxf(v, dpp<kRowMirror>(v));
+}
+
+__global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamJoin a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ double s_at[kMaxBeams];                          // score - log z
+  __shared__ float s_max[kMaxBeams];                          // the row's largest logit; NaN: no candidate but, perhaps, `pad`
+  __shared__ double s_value[kBeamList];
+  __shared__ uint64_t s_key[kBeamList];
+  __shared__ int s_beam[kBeamList], s_count;
+  const int W = a.W, n = a.n, S = a.S, req = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const uint64_t* keys = a.keys + (int64_t)req * W * S * n;
+  const int lists = W * S, all = lists * n;
+  // the first keys of the lists and the first four of the thread's, asked for before anything is known (of rows that were not
+  // read: not used)
+  constexpr int kFirst = kMaxBeams * 8 / 64, kAhead = 4;
+  uint64_t first[kFirst], mine[kAhead];
+  const int firsts = lists * a.depth;
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int e = lane + 64 * i, l = (int)((uint32_t)e / (uint32_t)a.depth);
+    first[i] = e < firsts ? keys[l * n + (e - l * a.depth)] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) mine[i] = tid + kBeamThreads * i < all ? keys[tid + kBeamThreads * i] : 0;
+  if (tid == 0) s_count = 0;
+  for (int w0 = 0; w0 < W; w0 += kBeamThreads / 16) {
+    const int w = w0 + tid / 16, l = tid & 15;
+    const int64_t row = (int64_t)req * W + min(w, W - 1);
+    const float score = a.scores[row];
+    const bool held = fabsf(score) <= FLT_MAX, done = held && a.finished && a.finished[row];
+    Sums s = l < S ? a.part[row * S + l] : Sums{-INFINITY, 0.f, 0.f};
+    const float m = row_max(s.m);
+    move_sums(s.m, m, s.z, s.e);
+    const float z = row_sum(s.z);
+    const bool none = !held || done || !(m > -INFINITY && m < INFINITY) || z != z;
+    const double at = (double)score - log((double)z);
+    if (l == 0 && w < W) {
+      s_at[w] = at;
+      s_max[w] = none ? NAN : m;
+    }
+  }
+  __syncthreads();
+  // a finished beam's one candidate (key 0: none of a list has it)
+  auto push = [&](bool in, double v, uint64_t key, int w) {
+    const uint64_t vote = __ballot(in);
+    if (!vote) return;
+    int at = 0;
+    if (lane == __builtin_ctzll(vote)) at = atomicAdd(&s_count, __popcll(vote));
+    at = __builtin_amdgcn_readlane(at, __builtin_ctzll(vote)) + __popcll(vote & (((uint64_t)1 << lane) - 1));
+    if (in && at < kBeamList) {
+      s_value[at] = v;
+      s_key[at] = key;
+      s_beam[at] = w;
+    }
+  };
+  auto value = [&](uint64_t key, int w) { return s_at[w] + ((double)order_value((uint32_t)(key >> 32)) - (double)s_max[w]); };
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int e = lane + 64 * i;
+    if (e >= firsts) break;
+    const int w = (int)((uint32_t)e / (uint32_t)(S * a.depth));
+    if (s_max[w] == s_max[w] && first[i]) top = fmaxf(top, (float)value(first[i], w));
+  }
+  const uint32_t k = order_key(top);
+  uint32_t nth = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t trial = nth | (1u << bit);
+    if (__popcll(__ballot(k >= trial)) >= n) nth = trial;
+  }
+  // (as a float it may be a step above the score itself; -inf where too few lanes hold anything)
+  const float f = order_value(nth);
+  const double bound = f == -INFINITY ? -DBL_MAX : (double)f - fabs((double)f) * 0x1p-22 - 0x1p-140;
+  for (int i0 = 0; i0 < all; i0 += kAhead * kBeamThreads) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = i0 + tid + kBeamThreads * i;
+      if (i0 + kBeamThreads * i >= all) break;
+      const uint64_t key = i0 == 0 ? mine[i] : at < all ? keys[at] : 0;
+      const int w = min((int)((uint32_t)at / (uint32_t)(S * n)), W - 1);
+      const bool live = key != 0 && s_max[w] == s_max[w];
+      const double v = live ? value(key, w) : -INFINITY;
+      push(live && v >= bound, v, key, w);
+    }
+  }
+  if (tid < 64 && a.finished)
+    for (int w0 = 0; w0 < W; w0 += 64) {
+      const int w = min(w0 + lane, W - 1);
+      const int64_t row = (int64_t)req * W + w;
+      const float score = a.scores[row];
+      push(w0 + lane < W && fabsf(score) <= FLT_MAX && a.finished[row], (double)score, 0, w);
+    }
+  __syncthreads();
+  const int found = s_count;
+  if (found < n || found > kBeamList) {                       // (uniform)
+    beam_join_whole(a, smem, req);
+    return;
+  }
+  int per = 1;                                                // lanes side by side that count a candidate's rank
+  while (per < 16 && 2 * per * found <= kBeamThreads) per *= 2;
+  for (int c0 = 0; c0 < found; c0 += kBeamThreads / per) {
+    const int c = c0 + tid / per;
+    const double v = c < found ? s_value[c] : 0.0;
+    const uint64_t key = c < found ? s_key[c] : 0;
+    const int w = c < found ? s_beam[c] : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int i = tid % per; i < found; i += per) {
+      const double o = s_value[i];
+      rank += o > v || (o == v && (s_beam[i] < w || (s_beam[i] == w && s_key[i] > key)));
+    }
+    for (int off = 1; off < per; off <<= 1) rank += __shfl_xor(rank, off, 64);
+    if (c >= found || rank >= n || tid % per) continue;
+    const int64_t to = (int64_t)req * n + rank;
+    a.out_scores[to] = (float)v;
+    a.out_beams[to] = w;
+    a.out_tokens[to] = key ? rank_index(key) : a.pad;
+  }
+}
+
+// slices of at least 2048 logits: up to `most` a row and `all` workgroups
+static int row_slices(int M, int V, int top, int most, int all, size_t ws_bytes) {
+  const int S = std::min({all / M, V / 2048, most});
   const size_t per = (size_t)M * (sizeof(Sums) + 4 + (size_t)top * 8);
   return (int)std::max<size_t>(1, std::min<size_t>((size_t)std::max(S, 1), ws_bytes / per));
 }
@@ -514,7 +654,8 @@ static size_t slice_lds(int V, int dtype, int S) {
 }
 
 hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
-  const int S = a.ws ? row_slices(a.M, a.V, a.top, a.ws_bytes) : 1;
+  // (four workgroups a CU; rows whole from 512 on)
+  const int S = a.ws && a.M < 512 ? row_slices(a.M, a.V, a.top, kMaxSlices, 1024, a.ws_bytes) : 1;
   const size_t lds = slice_lds(a.V, a.dtype, S);
   uint64_t* keys = static_cast<uint64_t*>(a.ws);              // [M][S][top] keys, then [M][S] sums
   Sums* part = reinterpret_cast<Sums*>(keys + (size_t)a.M * S * a.top);
@@ -531,8 +672,11 @@ hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
   return go(logprobs_kernel<bf16>, logprobs_join_kernel<bf16>, static_cast<const bf16*>(a.logits));
 }
 
+// few slices, whose lists the join has to read: 512 workgroups, two a CU (vocabulary 151936, fp16, graph-timed us with 16 slices a
+// row / 64: 1 x 4 beams 11.0 / 12.9, 1 x 8 17.1 / 20.4; with 512 workgroups in all / 1024: 8 x 4 13.0 / 17.2, 16 x 8 23.7 / 28.2, 32 x 8
+// 32.5 / 37.7, 64 x 8 46.7 / 55.1)
 hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st) {
-  const int M = a.requests * a.beams, S = row_slices(M, a.V, a.n, a.ws_bytes);
+  const int M = a.requests * a.beams, S = row_slices(M, a.V, a.n, kBeamSlices, 512, a.ws_bytes);
   const size_t lds = slice_lds(a.V, a.dtype, S);
   uint64_t* keys = static_cast<uint64_t*>(a.ws);              // [M][S][n] keys, then [M][S] sums
   Sums* part = reinterpret_cast<Sums*>(keys + (size_t)M * S * a.n);
@@ -545,17 +689,15 @@ hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st) {
                  : a.dtype == 1 ? go(logprobs_kernel<f16>, static_cast<const f16*>(a.logits))
                                 : go(logprobs_kernel<bf16>, static_cast<const bf16*>(a.logits));
   if (e != hipSuccess) return e;
-  // waves: as many beams at once as LDS holds the lists of
+  const int depth = std::min(a.n, std::max(1, 64 / (a.beams * S)));
+  const BeamJoin j{a.scores, a.finished, a.out_scores, a.out_beams, a.out_tokens, a.beams, a.V, a.n, a.pad, S, depth, part, keys};
   const size_t fixed = (size_t)a.beams * a.n * 12 + 8, each = (size_t)2 * S * a.n * 8;
-  const int waves = (int)std::max<size_t>(1, std::min<size_t>((size_t)8, (140 * 1024 - fixed) / each));
-  const size_t join_lds = fixed + waves * each;
-  if (join_lds > 65536) {
+  const size_t join_lds = std::min<size_t>(kBeamWhole, fixed + kBeamThreads / 64 * each);
+  if (join_lds > 32768) {
     static std::atomic<uint64_t> done{0};
-    if ((e = allow_lds_once(done, beam_join_kernel, 141 * 1024))) return e;
+    if ((e = allow_lds_once(done, beam_join_kernel, kBeamWhole))) return e;
   }
-  return launch(beam_join_kernel, dim3((unsigned)a.requests), dim3(64 * waves), join_lds, st, a.scores, a.finished, a.out_scores,
-                a.out_beams, a.out_tokens, a.beams, a.V, a.n, a.pad, S, static_cast<const Sums*>(part),
-                static_cast<const uint64_t*>(keys));
+  return launch(beam_join_kernel, dim3((unsigned)a.requests), dim3(kBeamThreads), join_lds, st, j);
 }
 
 }  // namespace lowbit

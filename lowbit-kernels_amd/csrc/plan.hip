@@ -14,11 +14,12 @@ namespace lowbit {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kMasksPer = 4;             // words of 32 pages that a thread looks through in one step of the search for free pages
+constexpr int kMasksPer = 4;             // words of 32 pages that a thread looks through in a later step of the search for free pages
 // what one workgroup plans alone, its state in LDS
 constexpr int kSmallSeqs = 1024, kSmallTokens = 4096, kSmallList = kSmallTokens / 16 + 2 * kSmallSeqs;
-constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 16;
-constexpr int kHashSeqs = 4096;          // sequences whose hash lies in LDS, and whose starts every workgroup copies there
+constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 15;
+constexpr int kHashSeqs = 1024;          // sequences whose hash lies in LDS
+constexpr int kStartSeqs = 4096;         // sequences whose starts every workgroup copies to LDS
 
 // The state of a call, in LDS or in the workspace: [B] each but off and start ([B + 1])
 struct PlanState {
@@ -66,135 +67,8 @@ __device__ __forceinline__ uint64_t owner_key(int past, int fresh, int b) {
 __device__ __forceinline__ int hash_slot(int page, int mask) { return (int)(((uint32_t)page * 2654435761u) >> 7) & mask; }
 
 // sequence b's partly filled last page, if it has one
-__device__ __forceinline__ int part_page(const PlanArgs& a, const PlanState& s, int shift, int b) {
-  const int page = s.tail[b];
-  return (s.past[b] & ((1 << shift) - 1)) && page >= 0 && page < a.pages ? page : -1;
-}
-
-// the sum of the threads' values up to and including this one's, held at `most`; *all: of all threads (values 0 .. most)
-__device__ __forceinline__ int block_scan(int v, int most, int* s_wave, int* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(v, off, 64);
-    if (lane >= off) v = min(v + o, most);
-  }
-  __syncthreads();
-  if (lane == 63) s_wave[wave] = v;
-  __syncthreads();
-  int before = 0, sum = 0;
-  for (int w = 0; w < waves; ++w) {
-    before = w == wave ? sum : before;
-    sum = min(sum + s_wave[w], most);
-  }
-  *all = sum;
-  return min(before + v, most);
-}
-
-// q_starts, kv_lens and the sequences' lengths, by one workgroup
-__device__ __forceinline__ void plan_lens(const PlanArgs& a, const PlanState& s, int shift, int* s_wave) {
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += (int)blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    int row = -1, past = 0, fresh = 0;
-    if (b < a.B) {
-      row = a.rows ? a.rows[b] : b;
-      fresh = min(max(a.fresh[b], 0), a.T);
-      if (row >= 0 && row < a.R) past = min(max(a.past[row], 0), a.width << shift);
-    }
-    int all;
-    const int upto = min(before + block_scan(fresh, a.T, s_wave, &all), a.T);   // (held at T: tokens past it are left out)
-    int first = __shfl_up(upto, 1, 64);
-    if (b < a.B) {
-      s.start[b + 1] = upto;
-      a.q_starts[b + 1] = upto;
-      s.row[b] = row;
-      s.past[b] = past;
-      s.tail[b] = -1;
-    }
-    if (b == 0) {
-      s.start[0] = 0;
-      a.q_starts[0] = 0;
-    }
-    __syncthreads();
-    if (b < a.B) {
-      if ((threadIdx.x & 63) == 0) first = s.start[b];
-      s.fresh[b] = upto - first;
-      a.kv_lens[b] = past + upto - first;
-    }
-    before = min(before + all, a.T);
-  }
-}
-
-// Which sequences get how many of the free pages, and which pages those are, by one workgroup. The hash is empty before.
-template <bool kLds>
-__device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, int* s_wave, int* s_over) {
-  if (threadIdx.x == 0) *s_over = 0;
-  for (int b = threadIdx.x; b < a.B; b += (int)blockDim.x) {
-    const int page = part_page(a, s, shift, b);
-    if (page < 0) continue;
-    for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask) {   // (twice as many places as sequences)
-      const int was = atomicCAS(s.hash_page + at, -1, page);
-      if (was != -1 && was != page) continue;
-      atomicMax(reinterpret_cast<unsigned long long*>(s.hash_owner) + at, (unsigned long long)owner_key(s.past[b], s.fresh[b], b));
-      break;
-    }
-  }
-  __syncthreads();
-  int total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += (int)blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    int want = 0;
-    bool copy = false;
-    if (b < a.B) {
-      const int past = s.past[b], fresh = s.fresh[b], have = pages_of(past, shift), need = pages_of(past + fresh, shift);
-      const int page = fresh > 0 ? part_page(a, s, shift, b) : -1;
-      if (page >= 0) {
-        copy = page_used<kLds>(s, page);                      // (within another's keys)
-        int at = hash_slot(page, s.hash_mask);
-        while (s.hash_page[at] != page) at = (at + 1) & s.hash_mask;
-        copy |= s.hash_owner[at] != owner_key(past, fresh, b);
-      }
-      want = min(need, a.width) - have + (copy ? 1 : 0);
-      if (need > a.width) atomicAdd(s_over, need - a.width);  // pages that the table has no place for
-    }
-    int all;
-    const int upto = block_scan(want, INT_MAX / 2, s_wave, &all);
-    if (b < a.B) s.off[b] = copy ? ~(total + upto - want) : total + upto - want;
-    total += all;
-  }
-  total = min(total, s.list_cap);
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.B; b += (int)blockDim.x) {
-    const int page = part_page(a, s, shift, b);
-    if (page >= 0) use_page<kLds>(s, page);
-  }
-  __syncthreads();
-  const int words = (int)((a.pages + 31) >> 5);
-  int found = 0;
-  for (int w0 = 0; w0 < words && found < total; w0 += (int)blockDim.x * kMasksPer) {
-    uint32_t free[kMasksPer];
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < kMasksPer; ++i) {
-      const int w = w0 + (int)threadIdx.x * kMasksPer + i;
-      const int64_t left = a.pages - 32 * (int64_t)w;
-      free[i] = w < words ? free_pages<kLds>(s, w) & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
-      n += __popc(free[i]);
-    }
-    int all;
-    int at = found + block_scan(n, INT_MAX / 2, s_wave, &all) - n;
-#pragma unroll
-    for (int i = 0; i < kMasksPer; ++i)
-      for (uint32_t f = free[i]; f && at < total; f &= f - 1, ++at)
-        s.list[at] = 32 * (w0 + (int)threadIdx.x * kMasksPer + i) + __ffs(f) - 1;
-    found = min(found + all, total);
-  }
-  for (int i = found + threadIdx.x; i < total; i += (int)blockDim.x) s.list[i] = -1;
-  if (threadIdx.x == 0) {
-    *a.missing = *s_over + total - found;
-    s.off[a.B] = total;
-  }
+__device__ __forceinline__ int part_page(const PlanArgs& a, int shift, int past, int tail) {
+  return (past & ((1 << shift) - 1)) && tail >= 0 && tail < a.pages ? tail : -1;
 }
 
 // the last b with of(b) <= v, of not falling and of(0) <= v
@@ -210,6 +84,186 @@ __device__ __forceinline__ int last_at(int n, int v, F of) {
   }
   return lo;
 }
+
+// Sums over the threads of a workgroup, held at `most` (values 0 .. most): of those before a thread and of all. s_wave has two rows,
+// taken in turn, so that one barrier a sum is enough.
+struct Scan {
+  int before, all;
+};
+struct ScanWaves {
+  int at[2][16];                                              // (zeros before: a smaller workgroup has fewer waves)
+};
+__device__ __forceinline__ Scan block_scan(int v, int most, ScanWaves& s, int& turn) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* at = s.at[turn];
+  turn ^= 1;
+  // (as wave_scan adds them, held at `most` in every step)
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false), most);
+  v = min(v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false), most);
+  if (lane == 63) at[wave] = v;
+  const int ahead = __builtin_amdgcn_update_dpp(0, v, 0x138, 0xF, 0xF, false);   // wave_shr 1
+  lds_barrier();
+  int w[16], before = 0, sum = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) *reinterpret_cast<u32x4*>(w + i) = *reinterpret_cast<const u32x4*>(at + i);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    before = i == wave ? sum : before;
+    sum = min(sum + w[i], most);
+  }
+  return {min(before + ahead, most), sum};
+}
+
+// q_starts, kv_lens and the sequences' lengths, by one workgroup
+__device__ __forceinline__ void plan_lens(const PlanArgs& a, const PlanState& s, int shift, ScanWaves& s_wave, int& turn) {
+  int done = 0;
+  for (int b0 = 0; b0 < a.B; b0 += (int)blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    int row = -1, past = 0, fresh = 0;
+    if (b < a.B) {
+      row = a.rows ? a.rows[b] : b;
+      fresh = min(max(a.fresh[b], 0), a.T);
+      if (row >= 0 && row < a.R) past = min(max(a.past[row], 0), a.width << shift);
+    }
+    const Scan sum = block_scan(fresh, a.T, s_wave, turn);
+    if (b < a.B) {
+      const int first = min(done + sum.before, a.T), upto = min(first + fresh, a.T);   // (held at T: tokens past it are left out)
+      s.start[b + 1] = upto;
+      a.q_starts[b + 1] = upto;
+      s.row[b] = row;
+      s.past[b] = past;
+      s.tail[b] = -1;
+      s.fresh[b] = upto - first;
+      a.kv_lens[b] = past + upto - first;
+      if (b == 0) {
+        s.start[0] = 0;
+        a.q_starts[0] = 0;
+      }
+    }
+    done = min(done + sum.all, a.T);
+  }
+}
+
+// Which sequences get how many of the free pages, and which pages those are, by one workgroup. The hash is empty before. s_free: a word
+// of each step's pages (zeros before); s_before: how many free ones come before a thread's.
+// The workspace's bytes of the first 32768 pages are asked for at once, before those of the last pages are marked: s_free has
+// a bit for each of these.
+template <bool kLds>
+__device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, ScanWaves& s_wave, int& turn,
+                                            int* s_over, uint32_t* s_free, int* s_before) {
+  const int tid = threadIdx.x, threads = blockDim.x, words = (int)((a.pages + 31) >> 5);
+  auto mask = [&](int w) {
+    const int64_t left = a.pages - 32 * (int64_t)w;
+    return w < words ? free_pages<kLds>(s, w) & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
+  };
+  uint32_t first_mask = 0;
+  if constexpr (!kLds) first_mask = mask(tid);
+  if (tid == 0) *s_over = 0;
+  // a thread's first sequence in registers
+  int past0 = 0, fresh0 = 0, tail0 = -1;
+  if (tid < a.B) {
+    past0 = s.past[tid];
+    fresh0 = s.fresh[tid];
+    tail0 = s.tail[tid];
+  }
+  auto sequence = [&](int b, int& past, int& fresh, int& page) {
+    const bool first = b == tid;
+    past = first ? past0 : s.past[b];
+    fresh = first ? fresh0 : s.fresh[b];
+    page = part_page(a, shift, past, first ? tail0 : s.tail[b]);
+  };
+  for (int b = tid; b < a.B; b += threads) {
+    int past, fresh, page;
+    sequence(b, past, fresh, page);
+    if (page < 0) continue;
+    for (int at = hash_slot(page, s.hash_mask);; at = (at + 1) & s.hash_mask) {   // (twice as many places as sequences)
+      const int was = atomicCAS(s.hash_page + at, -1, page);
+      if (was != -1 && was != page) continue;
+      atomicMax(reinterpret_cast<unsigned long long*>(s.hash_owner) + at, (unsigned long long)owner_key(past, fresh, b));
+      break;
+    }
+  }
+  lds_barrier();
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += threads) {
+    const int b = b0 + tid;
+    int want = 0;
+    bool copy = false;
+    if (b < a.B) {
+      int past, fresh, page;
+      sequence(b, past, fresh, page);
+      const int have = pages_of(past, shift), need = pages_of(past + fresh, shift);
+      if (fresh > 0 && page >= 0) {
+        copy = page_used<kLds>(s, page);                      // (within another's keys)
+        int at = hash_slot(page, s.hash_mask);
+        while (s.hash_page[at] != page) at = (at + 1) & s.hash_mask;
+        copy |= s.hash_owner[at] != owner_key(past, fresh, b);
+      }
+      want = min(need, a.width) - have + (copy ? 1 : 0);
+      if (need > a.width) atomicAdd(s_over, need - a.width);  // pages that the table has no place for
+    }
+    const Scan sum = block_scan(want, INT_MAX / 2, s_wave, turn);
+    if (b < a.B) s.off[b] = copy ? ~(total + sum.before) : total + sum.before;
+    total += sum.all;
+  }
+  total = min(total, s.list_cap);
+  // (every sequence has looked for its page among the full ones: the barrier of the last sum)
+  for (int b = tid; b < a.B; b += threads) {
+    int past, fresh, page;
+    sequence(b, past, fresh, page);
+    if (page < 0) continue;
+    if (kLds || page >= 32 * threads)
+      use_page<kLds>(s, page);
+    else
+      atomicOr(s_free + (page >> 5), 1u << (page & 31));
+  }
+  __syncthreads();
+  int found = 0, per = 1;
+  for (int w0 = 0; w0 < words && found < total; w0 += threads * per, per = kMasksPer) {
+    if (w0 > 0) lds_barrier();                                // (the step before has been read)
+    int n = 0;
+    for (int i = 0; i < per; ++i) {
+      const uint32_t m = kLds || w0 > 0 ? mask(w0 + tid * per + i) : first_mask & ~s_free[tid];
+      s_free[tid * per + i] = m;
+      n += __popc(m);
+    }
+    const Scan sum = block_scan(n, INT_MAX / 2, s_wave, turn);
+    s_before[tid] = sum.before;
+    lds_barrier();
+    // a thread a page: whose words hold it, then which bit it is
+    for (int j = tid; j < min(sum.all, total - found); j += threads) {
+      const int t = last_at(threads, j, [&](int i) { return s_before[i]; });
+      int rest = j - s_before[t], w = t * per;
+      for (int c = __popc(s_free[w]); rest >= c; c = __popc(s_free[w])) {
+        rest -= c;
+        ++w;
+      }
+      uint32_t m = s_free[w];
+      int bit = 0;
+#pragma unroll
+      for (int half = 16; half > 0; half >>= 1) {
+        const int c = __popc(m & ((1u << half) - 1u));
+        if (rest >= c) {
+          rest -= c;
+          m >>= half;
+          bit += half;
+        }
+      }
+      s.list[found + j] = 32 * (w0 + w) + bit;
+    }
+    found = min(found + sum.all, total);
+  }
+  for (int i = found + tid; i < total; i += threads) s.list[i] = -1;
+  if (tid == 0) {
+    *a.missing = *s_over + total - found;
+    s.off[a.B] = total;
+  }
+}
+
 __device__ __forceinline__ int off_of(int v) { return v < 0 ? ~v : v; }
 
 // place j of the list: into the table
@@ -218,8 +272,10 @@ __device__ __forceinline__ void give_page(const PlanArgs& a, const PlanState& s,
   const int off = s.off[b], first = off_of(off), have = pages_of(s.past[b], shift);
   a.table_out[(int64_t)b * a.width + have + (j - first) - (off < 0 ? 1 : 0)] = s.list[j];
 }
-__device__ __forceinline__ void give_copy(const PlanArgs& a, const PlanState& s, int b) {
+__device__ __forceinline__ void give_copy(const PlanArgs& a, const PlanState& s, int shift, int b) {
   const bool copy = s.off[b] < 0;
+  const int have = pages_of(s.past[b], shift);
+  if (!copy && have > 0 && a.table_out != a.table) a.table_out[(int64_t)b * a.width + have - 1] = s.tail[b];
   a.copies[2 * b] = copy ? s.tail[b] : -1;
   a.copies[2 * b + 1] = copy ? s.list[~s.off[b]] : -1;
 }
@@ -266,9 +322,12 @@ __device__ __forceinline__ void give_token(const PlanArgs& a, const PlanState& s
 }  // namespace
 
 // The whole plan by one workgroup.
-__global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, FastDiv by_width, int shift, int hash_mask) {
+__global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, int lanes_log, int shift, int hash_mask) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
-  __shared__ int s_wave[kThreads / 64], s_over;
+  __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
+  __shared__ int s_over, s_before[kThreads];
+  __shared__ uint32_t s_free[kThreads * kMasksPer];
+  int turn = 0;
   const int tid = threadIdx.x, threads = blockDim.x, words = ((int)((a.pages + 31) >> 5) + 3) & ~3;
   PlanState s;
   s.hash_mask = hash_mask;
@@ -286,48 +345,70 @@ __global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, FastDi
   int* s_parent = s.list + kSmallList;
   if (a.parents)
     for (int i = tid; i < a.T; i += threads) s_parent[i] = a.parents[i];
+  if (tid < 32) s_wave.at[0][tid] = 0;
   for (int i = tid; i < 2 * (hash_mask + 1) + words; i += threads) s_plan[i] = 0;
   for (int i = tid; i <= hash_mask; i += threads) s.hash_page[i] = -1;
-  plan_lens(a, s, shift, s_wave);
-  __syncthreads();
-  const int entries = a.B * a.width;
+  lds_barrier();
+  plan_lens(a, s, shift, s_wave, turn);
+  lds_barrier();
   const bool other = a.table_out != a.table;
-  constexpr int kAhead = 8;
-  for (int i0 = tid; i0 < entries; i0 += kAhead * threads) {
-    int page[kAhead], b[kAhead], c[kAhead], have[kAhead];
+  // 2^lanes_log threads a row, four rows and four pieces of each in flight
+  const int lanes = 1 << lanes_log, step = threads >> lanes_log, c1 = tid & (lanes - 1);
+  constexpr int kAhead = 4;
+  for (int b0 = tid >> lanes_log; b0 < a.B; b0 += kAhead * step) {
+    int past[kAhead];
+    int64_t row[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int i = min(i0 + u * threads, entries - 1);
-      b[u] = div(i, by_width);
-      c[u] = i - b[u] * a.width;
-      have[u] = s.past[b[u]];
-      page[u] = s.row[b[u]];
+      const int b = b0 + u * step;
+      past[u] = b < a.B ? s.past[b] : 0;
+      row[u] = b < a.B ? (int64_t)s.row[b] * a.width : 0;
     }
+    for (int c0 = c1; c0 < a.width; c0 += kAhead * lanes) {
+      int page[kAhead][kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      page[u] = c[u] < pages_of(have[u], shift) ? a.table[(int64_t)page[u] * a.width + c[u]] : -1;
+      for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (i0 + u * threads >= entries) break;
-      if (c[u] == pages_of(have[u], shift) - 1) s.tail[b[u]] = page[u];
-      if (c[u] < have[u] >> shift && page[u] >= 0 && page[u] < a.pages) use_page<true>(s, page[u]);
-      if (other) a.table_out[i0 + u * threads] = page[u];
+        for (int i = 0; i < kAhead; ++i) {
+          const int c = c0 + i * lanes;
+          page[u][i] = -1;
+          if (c < pages_of(past[u], shift)) page[u][i] = a.table[row[u] + c];
+        }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int b = b0 + u * step;
+        if (b >= a.B) break;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int c = c0 + i * lanes, got = page[u][i];
+          if (c >= a.width) break;
+          const bool last = c == pages_of(past[u], shift) - 1;
+          if (last) s.tail[b] = got;
+          if (c < past[u] >> shift && got >= 0 && got < a.pages) use_page<true>(s, got);
+          if (other && !last) a.table_out[b * a.width + c] = got;   // (the last page kept, or its copy: below)
+        }
+      }
     }
   }
-  __syncthreads();
-  plan_assign<true>(a, s, shift, s_wave, &s_over);
-  __syncthreads();
+  lds_barrier();
+  plan_assign<true>(a, s, shift, s_wave, turn, &s_over, s_free, s_before);
+  lds_barrier();
   for (int j = tid; j < s.off[a.B]; j += threads) give_page(a, s, shift, j);
-  for (int b = tid; b < a.B; b += threads) give_copy(a, s, b);
+  for (int b = tid; b < a.B; b += threads) give_copy(a, s, shift, b);
   for (int t = tid; t < a.T; t += threads) give_token(a, s, shift, t, [&](int first, int n) { return s_parent[first + n]; });
 }
 
 // The same in four launches, the state in the workspace: the lengths, beside the clearing of what the pages are marked in; the
-// pages kept, 1024 entries of a row a workgroup; the pages handed out; tables and tokens.
+// pages kept, 1024 entries of a row a workgroup; the pages handed out; tables and tokens. (256 sequences on 300 .. 30000 keys in pages
+// of 16, us: 2.4, 4.4, 6.2 and 4.1. The pages handed out by the last workgroup that marks, whose marks then go past the L2: 17.9
+// for both.)
 __global__ __launch_bounds__(kThreads) void plan_lens_kernel(PlanArgs a, PlanState s, int shift, int64_t clear) {
-  __shared__ int s_wave[kThreads / 64];
+  __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
+  int turn = 0;
   if (blockIdx.x == 0) {
-    plan_lens(a, s, shift, s_wave);
+    if (threadIdx.x < 32) s_wave.at[0][threadIdx.x] = 0;
+    lds_barrier();
+    plan_lens(a, s, shift, s_wave, turn);
     return;
   }
   const int64_t step = (int64_t)(gridDim.x - 1) * kThreads, at = (int64_t)(blockIdx.x - 1) * kThreads + threadIdx.x;
@@ -349,13 +430,18 @@ __global__ __launch_bounds__(256) void plan_mark_kernel(PlanArgs a, PlanState s,
     const int c = c0 + 256 * u;
     if (c == have - 1) s.tail[b] = page[u];
     if (c < past >> shift && page[u] >= 0 && page[u] < a.pages) use_page<false>(s, page[u]);
-    if (other && c < a.width) a.table_out[(int64_t)b * a.width + c] = page[u];
+    if (other && c < a.width && c != have - 1) a.table_out[(int64_t)b * a.width + c] = page[u];
   }
 }
 
 __global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanState s, int shift) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
-  __shared__ int s_wave[kThreads / 64], s_over;
+  __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
+  __shared__ int s_over, s_before[kThreads];
+  __shared__ uint32_t s_free[kThreads * kMasksPer];
+  int turn = 0;
+  s_free[threadIdx.x] = 0;
+  if (threadIdx.x < 32) s_wave.at[0][threadIdx.x] = 0;
   if (!s.hash_page) {
     s.hash_owner = reinterpret_cast<uint64_t*>(s_plan);
     s.hash_page = reinterpret_cast<int*>(s.hash_owner + s.hash_mask + 1);
@@ -363,14 +449,14 @@ __global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanS
       s.hash_owner[i] = 0;
       s.hash_page[i] = -1;
     }
-    __syncthreads();
   }
-  plan_assign<false>(a, s, shift, s_wave, &s_over);
+  __syncthreads();
+  plan_assign<false>(a, s, shift, s_wave, turn, &s_over, s_free, s_before);
 }
 
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s, int shift) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
-  if (a.B <= kHashSeqs) {                                     // the searches' arrays
+  if (a.B <= kStartSeqs) {                                    // the searches' arrays
     int* copy = reinterpret_cast<int*>(s_plan);
     for (int i = threadIdx.x; i <= a.B; i += 256) {
       copy[i] = s.start[i];
@@ -383,7 +469,7 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s,
   const int step = gridDim.x * 256, at = blockIdx.x * 256 + threadIdx.x;
   const int total = s.off[a.B];
   for (int j = at; j < total; j += step) give_page(a, s, shift, j);
-  for (int b = at; b < a.B; b += step) give_copy(a, s, b);
+  for (int b = at; b < a.B; b += step) give_copy(a, s, shift, b);
   for (int t = at; t < a.T; t += step)
     give_token(a, s, shift, t, [&](int first, int n) { return a.parents[first + n]; });
 }
@@ -408,7 +494,7 @@ __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ 
 
 // accept_drafts. Workgroup (sequence, layer): its first wave follows the picks from node 0 down the tree (the first 64 nodes in its
 // lanes, a ballot a step), then the workgroup moves the confirmed nodes' rows of its layer, every head of k and v, to the places
-// behind the sequence's keys: one launch, the walk repeated in every layer. Node d of the path comes to lie at place d <= the
+// behind the sequence's keys: one launch, the walk repeated in every layer (several layers a workgroup: 64 trees, 28 layers, 16.6 us instead of 14.7). Node d of the path comes to lie at place d <= the
 // node's own, so rows are read and written in order of the path, a chunk's all read before one is written.
 constexpr int kMostPath = 1024;
 __device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
@@ -549,11 +635,11 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     const size_t words = (size_t)map_words(a.pages);
     const size_t lds = 4 * (3 * (size_t)places + words + 6 * (size_t)a.B + 2 + kSmallList + kSmallTokens);
     constexpr size_t most = 4 * (3 * 2 * kSmallSeqs + kSmallPages / 32 + 6 * kSmallSeqs + 2 + kSmallList + kSmallTokens);
-    static_assert(most <= 158 * 1024, "LDS");
+    static_assert(most <= 138 * 1024, "LDS");
     static std::atomic<uint64_t> done{0};
     if ((e = allow_lds_once(done, plan_small_kernel, most))) return e;
     const bool few = a.B <= 256 && a.T <= 1024 && (int64_t)a.B * a.width <= 2048 && a.pages <= 32768;
-    e = launch(plan_small_kernel, dim3(1), dim3(few ? 256 : kThreads), lds, st, a, fast_div(a.width), shift, places - 1);
+    e = launch(plan_small_kernel, dim3(1), dim3(few ? 256 : kThreads), lds, st, a, std::min(6, log2_of(a.width)), shift, places - 1);
   } else {
     const bool far = a.B > kHashSeqs;                         // the hash in the workspace
     PlanState s;
@@ -574,16 +660,13 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     e = launch(plan_lens_kernel, dim3((unsigned)(1 + std::min<int64_t>((clear + kThreads - 1) / kThreads, 512))), dim3(kThreads), 0, st,
                a, s, shift, clear);
     const int chunks = (a.width + 1023) / 1024;
+    static_assert(12 * 2 * kHashSeqs + 24 * 1024 <= 64 * 1024, "LDS");
     if (e == hipSuccess) e = launch(plan_mark_kernel, dim3((unsigned)(a.B * chunks)), dim3(256), 0, st, a, s, chunks, shift);
-    if (e == hipSuccess && !far && 12 * places > 65536) {
-      static std::atomic<uint64_t> done{0};
-      e = allow_lds_once(done, plan_assign_kernel, 12 * 2 * kHashSeqs);
-    }
     if (e == hipSuccess) e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places, st, a, s, shift);
     const int64_t items = std::max<int64_t>(a.T, a.B);
     if (e == hipSuccess)
       e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256),
-                 far ? 0 : 8 * (size_t)(a.B + 1), st, a, s, shift);
+                 a.B <= kStartSeqs ? 8 * (size_t)(a.B + 1) : 0, st, a, s, shift);
   }
   if (e != hipSuccess || !a.k) return e;
   return launch(plan_copy_kernel, dim3((unsigned)a.B, (unsigned)a.layers), dim3(256), 0, st, static_cast<const int*>(a.copies),

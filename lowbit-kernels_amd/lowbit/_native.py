@@ -861,11 +861,15 @@ class NativeExt:
             _need_fast(out, "out", torch.int32, (batch, width), index, device)
             if rows is not None and out.data_ptr() == page_table.data_ptr():
                 raise RuntimeError("rows need a table of their own to go to")
-        ints = torch.empty(4 * batch + 2, dtype=torch.int32, device=device)
-        copies, q_starts, kv_lens, missing = ints.split_with_sizes((2 * batch, batch + 1, batch, 1))
-        positions = torch.empty(tokens, dtype=torch.int64, device=device)
-        slots = torch.empty(tokens, dtype=torch.int64, device=device)
-        masks = torch.empty((tokens, words), dtype=torch.int64, device=device) if parents is not None else None
+        # one allocation, whose parts cost less than tensors of their own
+        whole = torch.empty(tokens * (2 + (words if parents is not None else 0)) + 2 * batch + 1, dtype=torch.int64, device=device)
+        if parents is not None:
+            positions, slots, masks, ints = whole.split_with_sizes((tokens, tokens, tokens * words, 2 * batch + 1))
+            masks = masks.view(tokens, words)
+        else:
+            positions, slots, ints = whole.split_with_sizes((tokens, tokens, 2 * batch + 1))
+            masks = None
+        copies, q_starts, kv_lens, missing = ints.view(torch.int32).split_with_sizes((2 * batch, batch + 1, batch, 1))
         nbytes = self._plan_workspace(batch, width, tokens, pages, page_size)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         opt = lambda t: None if t is None else t.data_ptr()                               # noqa: E731
