@@ -13,7 +13,8 @@ cache write inside the q|k|v store, whose rows are permuted per head so that rot
 launches, the attention's partition merge included)
 
 with its own KV cache (forward_paged: rmsnorm -> qkv projection -> rotation + write into the pages -> attention over the pages,
-the rest alike, over the caller's caches). The projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the
+the rest alike, over the caller's caches; verify_trees and beam_search run steps of it whose tables are made on the GPU). The
+projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the
 consumer fused into the store, for up to 64 rows; dequantize + hipBLASLt beyond) or fp16 (hipBLASLt through torch,
 bias and residual folded into addmm, silu * up as two torch ops), so the two variants share every other kernel and
 differ only in the projections. Weights come from a transformers Qwen2ForCausalLM; q|k|v are merged into one
@@ -131,7 +132,7 @@ def _torch_epilogue(x, w, epilogue, aux, out, round_first=False):
 
 class FusedQwen2:
     """Qwen2 forward from the library's kernels (see the module docstring): one sequence (forward, score), or a batch over paged
-    caches (paged_caches, forward_paged).
+    caches (paged_caches, forward_paged), trees of drafted tokens (verify_trees) and beams (beam_search) among them.
 
     build(model, max_len, quant, group, clip_grid): quant = "int4" quantizes every projection with the GPU quantizer
     (the same bits as lowbit.model.quantize_layers) and keeps only the packed weights; quant = "fp16" keeps fp16
@@ -305,13 +306,15 @@ class FusedQwen2:
         return k, torch.zeros_like(k)
 
     @torch.inference_mode()
-    def forward_paged(self, tokens, positions, slots, page_table, q_starts, kv_lens, caches, max_new, max_keys, rows=None):
+    def forward_paged(self, tokens, positions, slots, page_table, q_starts, kv_lens, caches, max_new, max_keys, rows=None,
+                      masks=None):
         """One step of a batch of sequences over paged caches: tokens, positions and slots (int64 [T]) hold the sequences' new
         tokens one after another (prompts or pieces of them, decode tokens, drafts), sequence b's in q_starts[b] ..
         q_starts[b + 1] (int32 [B + 1]); its keys, the new tokens' included, are the first kv_lens[b] (int32 [B]) in the pages
         page_table[b] (int32 [B, width]), and token t's k and v go to slot slots[t] = page * page_size + row (negative: a
         padded token's, nowhere). max_new, max_keys: bounds on a sequence's new tokens and keys. Returns the logits of `rows`
-        (int64, indices into the T tokens; None: of all; may be empty, as T may be 0)."""
+        (int64, indices into the T tokens; None: of all; may be empty, as T may be 0). masks (int64 [T, words], plan_paged's):
+        the new tokens are trees, each attending the nodes of its mask beside the keys before them."""
         ext = ops.ext()
         t = tokens.shape[0]
         h = self._embedding(tokens)
@@ -322,7 +325,11 @@ class FusedQwen2:
             qkv = lay["qkv"](h, EPI_BIAS, lay["qkv"].bias, norm=(lay["in_norm"], self.eps))
             ext.norm_rope_paged(qkv, None, None, self.eps, positions, self.inv_freq, slots, q, k_cache, v_cache, self.hq,
                                 self.hkv, permuted=self.quant in ("int4", "fp16_gemv"))
-            ext.attention_paged(q, k_cache, v_cache, page_table, q_starts, kv_lens, attn, max_new, max_keys, self.scale)
+            if masks is None:
+                ext.attention_paged(q, k_cache, v_cache, page_table, q_starts, kv_lens, attn, max_new, max_keys, self.scale)
+            else:
+                ext.attention_paged_tree(q, k_cache, v_cache, page_table, q_starts, kv_lens, masks, attn, max_new, max_keys,
+                                         self.scale)
             lay["o"](attn.view(t, -1), EPI_RESIDUAL, h, out=h)
             act = lay["gu"](h, EPI_SILU_MUL, norm=(lay["post_norm"], self.eps))
             lay["down"](act, EPI_RESIDUAL, h, out=h)
@@ -331,6 +338,64 @@ class FusedQwen2:
         if h.shape[0] == 0:                                 # (a step of prompt pieces alone asks for no logits)
             return h.new_empty(0, self.head.shape[0])
         return self.logits(ext.rmsnorm(h, self.final_norm, self.eps))
+
+    @torch.inference_mode()
+    def verify_trees(self, tokens, parents, page_table, past, new, caches, max_new, max_keys, longest):
+        """One step over trees of drafted tokens, without the host: sequence b's tree is the next new[b] (int32 [B], at most
+        max_new <= 1024) of tokens (int64 [T]; padded tokens behind the last), its node 0 the token chosen last, every other one
+        below the node parents[t] (int32 [T]) of its sequence. The sequence's past[b] keys (int32 [B]) lie in the pages
+        page_table[b] (int32 [B, width], completed in place). Follows the greedy picks down each tree for at most `longest` nodes
+        and keeps their keys. Returns accepted (int64 [B, longest]: the confirmed tokens after node 0 and the next one, the
+        node 0 to come; -1 behind), counts (int32 [B]: how many) and lens (int32 [B]: the keys kept, the next step's past).
+        What plan_paged could not place for want of pages is told by the last item, missing (int32 [1])."""
+        ext = ops.ext()
+        pages, page_size = caches[0].shape[1], caches[0].shape[3]
+        step = ext.plan_paged(page_table, past, new, tokens.shape[0], pages, page_size, parents=parents,
+                              words=max(1, -(-max_new // 64)), caches=caches, out=page_table)
+        logits = self.forward_paged(tokens, step.positions, step.slots, step.page_table, step.q_starts, step.kv_lens, caches,
+                                    max_new, max_keys, masks=step.masks)
+        picks = logits.argmax(-1)
+        _, counts, accepted, lens = ext.accept_drafts(tokens, picks, parents, step.q_starts, step.kv_lens, step.page_table,
+                                                      caches, longest)
+        return accepted, counts, lens, step.missing
+
+    @torch.inference_mode()
+    def beam_search(self, prompts, beams, steps, eos=None, page_size=64):
+        """The `beams` (at most 32) best continuations of `steps` tokens of each prompt (a list of int64 tensors), as beam search
+        finds them, by their summed log probabilities: tokens (int64 [prompts, beams, steps]) and scores (float32 [prompts,
+        beams]), best first. A beam that takes the token `eos` ends there (eos behind it, its score as it is). Beams share the
+        pages of their common text; only a last page that two of them would write is copied. Nothing waits for the host between
+        the steps."""
+        if not prompts or any(p.dim() != 1 or p.shape[0] < 1 for p in prompts):
+            raise ValueError("beam_search needs prompts of one token or more")
+        if not 1 <= beams <= 32 or steps < 1:
+            raise ValueError("beam_search takes 1..32 beams and a step or more")
+        ext, dev, count = ops.ext(), self.embed.device, len(prompts)
+        lens = [p.shape[0] for p in prompts]
+        own_pages = -(-steps // page_size) + 2              # of a beam: its text, the prompt's last page, a copy in the making
+        pages = sum(-(-n // page_size) for n in lens) + count * beams * own_pages
+        caches = self.paged_caches(pages, page_size)
+        i32 = dict(dtype=torch.int32, device=dev)
+        table = torch.full((count, -(-(max(lens) + steps) // page_size)), -1, **i32)
+        step = ext.plan_paged(table, torch.zeros(count, **i32), torch.tensor(lens, **i32), sum(lens), pages, page_size)
+        logits = self.forward_paged(torch.cat(list(prompts)), step.positions, step.slots, step.page_table, step.q_starts,
+                                    step.kv_lens, caches, max(lens), max(lens), rows=step.q_starts[1:].long() - 1)
+        scores, _, token = ext.beam_select(logits, torch.zeros(count, 1, dtype=torch.float32, device=dev), beams)
+        history = token[:, :, None]
+        finished = token == (-1 if eos is None else eos)
+        first = torch.arange(count, device=dev)[:, None] * beams
+        rows = torch.arange(count, **i32).repeat_interleave(beams)
+        ones = torch.ones(count * beams, **i32)
+        for i in range(1, steps):
+            step = ext.plan_paged(step.page_table, step.kv_lens, ones, count * beams, pages, page_size, rows=rows, caches=caches)
+            logits = self.forward_paged(token.view(-1), step.positions, step.slots, step.page_table, step.q_starts, step.kv_lens,
+                                        caches, 1, max(lens) + i)
+            scores, parent, token = ext.beam_select(logits, scores, beams, finished if eos is not None else None, eos or 0)
+            rows = (first + parent).to(torch.int32).view(-1)
+            history = torch.cat([history.gather(1, parent[:, :, None].expand(-1, -1, i)), token[:, :, None]], 2)
+            if eos is not None:
+                finished = finished.gather(1, parent) | (token == eos)
+        return history, scores
 
 
 class FusedDecoder:
