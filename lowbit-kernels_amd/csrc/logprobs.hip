@@ -246,17 +246,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   auto collect = [&](bool above) {                            // what reaches the bound, or passes it
     for (int g = 0; g * every < steps; ++g) {
       if (!(s_max[g * kThreads + tid] >= bound)) continue;
-      for (int step = g * every; step < min(steps, (g + 1) * every); ++step)
+      for (int step = g * every; step < min(steps, (g + 1) * every); ++step) {
+        u32x4 v[kUnroll];                                     // (asked for at once)
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int64_t i = (int64_t)(step * kUnroll + u) * kThreads + tid;
+          if (i < end) v[u] = load16(body + (v0 + i) * kN);
+        }
+#pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int64_t i = (int64_t)(step * kUnroll + u) * kThreads + tid;
           if (i >= end) continue;
-          const u32x4 v = load16(body + (v0 + i) * kN);
 #pragma unroll
           for (int k = 0; k < kN; ++k) {
-            const float f = value<T>(v, k);
+            const float f = value<T>(v[u], k);
             if (above ? f > bound : f >= bound) push(f, head + (int)(v0 + i) * kN + k);
           }
         }
+      }
     }
     if (single >= 0) {
       const float f = (float)x[single];
@@ -318,6 +325,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       for (int i = tid; i < n; i += kThreads) {
         const uint64_t key = s_list[i];
         int rank = 0;
+#pragma unroll 8
         for (int k = 0; k < n; ++k) rank += s_list[k] > key;
         if (rank < top) give(rank, key);
       }

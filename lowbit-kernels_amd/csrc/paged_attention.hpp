@@ -44,6 +44,7 @@ struct PagedPlan {
   int least;         // blocks of a part at least
   int cap;           // parts of a tile at most (1: no split)
   int most;          // parts of split tiles in all at most (what the workspace holds, twice its share)
+  int units;         // kTree: split tiles at most (what the workspace has room to describe)
   int Hq, Hkv, G;
   FastDiv by_hkv, by_g;
 };
@@ -355,9 +356,9 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
         const PagedSeq s = at == 0 ? s0 : paged_seq<kRows, BK>(bt, G, at + lane);
         split += wave_sum((float)(s.blocks > share ? s.tiles : 0));
       }
-      if (lane == 0) tiles[0].parts = (int)split * Hkv;
+      if (lane == 0) tiles[0].parts = (int)fminf(split * (float)Hkv, (float)plan.units);
     }
-    if (un.parts > 1 && un.pid == 0 && tid == 0)
+    if (un.parts > 1 && un.pid == 0 && tid == 0 && (uint32_t)un.tile_no < (uint32_t)plan.units)
       tiles[1 + un.tile_no] = PagedTile{un.first, un.nq, un.len, un.tile, un.hk, un.parts, un.rec, 0};
   }
   const int rgrp = wave % RG, kgrp = wave / RG;
@@ -843,6 +844,10 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
   const float c2 = score_scale(scale);
   for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
     const PagedTile t = tiles[1 + idx / kChunks];
+    // (with starts that fall, which the caller rules out, a tile may not have been written: never past the buffers)
+    if (t.parts < 2 || t.parts > plan.cap || t.rec < 0 || t.rec > plan.most - t.parts || t.first < 0 || t.nq < 1 ||
+        t.nq > bt.T - t.first || t.tile < 0 || t.tile > (t.nq * plan.G - 1) / kRows || (uint32_t)t.hk >= (uint32_t)plan.Hkv)
+      continue;
     const int r = idx % kChunks * kHere + grp / PG, row = t.tile * kRows + r;
     const float* rec = part + ((size_t)t.rec * kRows + r) * kRec;
     const size_t step = (size_t)kRows * kRec;
@@ -1001,7 +1006,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
   const size_t lds = paged_lds<D, RG, KG>() + (kTree && a.batch.words > 1 ? (size_t)32 * RG * a.batch.words * 8 : 0);
   constexpr int kRows = 32 * RG, kBlock = 32 * KG;
   const int G = a.Hq / a.Hkv;
-  PagedPlan p{l.slots, l.least, 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
+  PagedPlan p{l.slots, l.least, 1, 0, (int)l.units, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
   // kTree: the tiles' descriptions before the records
   const size_t head = kTree ? (size_t)(l.units + 1) * sizeof(PagedTile) : 0;
   p.most = a.ws && a.ws_bytes > head ? (int)std::min<size_t>((size_t)l.records, (a.ws_bytes - head) / paged_record_bytes(RG, D)) : 0;

@@ -265,3 +265,27 @@ def test_strides_streams_graphs(cuda):
         run()
         torch.cuda.synchronize()
         assert torch.equal(got, out)
+
+
+def test_starts_that_do_not_hold(cuda):
+    """Starts past q's rows or below zero are held to them, and nothing outside out is written."""
+    lens = [(4, 50), (3, 40)]
+    x = list(batch(lens, 16, 2, 128, 16, torch.float16, 3))
+    masks = torch.full((7, 1), -1, dtype=torch.int64, device="cuda")
+    room = torch.full((7 + 8, 16, 128), 777.0, dtype=torch.float16, device="cuda")
+    for starts in ([-5, 4, 1000], [0, 4, 7], [7, 7, 7], [900, 900, 900], [-3, -2, -1], [6, 2, 7]):
+        x[4] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        for keys in (50, 1 << 20):
+            room.fill_(777.0)
+            ops.ext().attention_paged_tree(*x[:6], masks, room[4:11], 4, keys, 0.1)
+            torch.cuda.synchronize()
+            assert bool((room[:4] == 777.0).all()) and bool((room[11:] == 777.0).all())
+
+
+def test_many_sequences(cuda):
+    """More sequences than shares are balanced for at once, of equal and of very different lengths."""
+    for n, hq, hkv, d in ((70, 28, 4, 128), (300, 8, 2, 64)):
+        lens = [(1 + i % 7, 1 + i % 7 + (i * 37) % 200) for i in range(n)]
+        lens[3], lens[n - 2] = (40, 5000), (3, 9000)
+        x = batch(lens, hq, hkv, d, 32, torch.float16, n)
+        check(x, lens, [tree_bits(k, i) for i, (k, _) in enumerate(lens)], 1, d ** -0.5)
