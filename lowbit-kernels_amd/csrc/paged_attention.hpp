@@ -729,6 +729,18 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
       for (int v = 0; v < 16; v += 4)
         store_row<T>(dst + 32 * dt + 2 * v, f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]}, den, some);
+  } else if constexpr (kTree) {
+    // in the order of the lanes, 1 KB a store (paged_tree_merge_lanes): the rows' references, their sums, the outputs
+    float* rec = part + ((size_t)un.rec * kRows + 32 * rgrp) * paged_rec<D>();
+    if (h == 0) {
+      rec[j] = ref;
+      rec[32 + j] = den;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<f32x4*>(rec + 64 + 256 * (4 * dt + v / 4) + 4 * lane) = f32x4{o[dt][v], o[dt][v + 1], o[dt][v + 2], o[dt][v + 3]};
   } else {
     float* rec = part + ((size_t)un.rec * kRows + 32 * rgrp + j) * paged_rec<D>();
     if (h == 0) {
@@ -830,6 +842,12 @@ __global__ __launch_bounds__(256) void paged_attention_merge(const float* __rest
   }
 }
 
+// (with starts that fall, which the caller rules out, a tile may not have been written: never past the buffers)
+template <int kRows>
+__device__ __forceinline__ bool tile_holds(const PagedTile& t, const PagedBatch& b, const PagedPlan& p) {
+  return t.parts >= 2 && t.parts <= p.cap && t.rec >= 0 && t.rec <= p.most - t.parts && t.first >= 0 && t.nq >= 1 &&
+         t.nq <= b.T - t.first && t.tile >= 0 && t.tile <= (t.nq * p.G - 1) / kRows && (uint32_t)t.hk < (uint32_t)p.Hkv;
+}
 // The same for trees: the main kernel leaves the split tiles in tiles[], so that no workgroup looks for its own (at 16 sequences, whose
 // share takes some steps to find, the join takes 7.2 us instead of 14.3). PG groups of D / 4 lanes a row, each for a run of the parts: a lane reads the references and sums of one part each, and the
 // output's four values of all of them.
@@ -844,10 +862,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
   const float c2 = score_scale(scale);
   for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
     const PagedTile t = tiles[1 + idx / kChunks];
-    // (with starts that fall, which the caller rules out, a tile may not have been written: never past the buffers)
-    if (t.parts < 2 || t.parts > plan.cap || t.rec < 0 || t.rec > plan.most - t.parts || t.first < 0 || t.nq < 1 ||
-        t.nq > bt.T - t.first || t.tile < 0 || t.tile > (t.nq * plan.G - 1) / kRows || (uint32_t)t.hk >= (uint32_t)plan.Hkv)
-      continue;
+    if (!tile_holds<kRows>(t, bt, plan)) continue;
     const int r = idx % kChunks * kHere + grp / PG, row = t.tile * kRows + r;
     const float* rec = part + ((size_t)t.rec * kRows + r) * kRec;
     const size_t step = (size_t)kRows * kRec;
@@ -919,6 +934,84 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
     un.nq = t.nq;
     un.len = t.len;
     store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den, some_key<true>(bt, un, tok));
+  }
+}
+
+// The same of tiles of 128 rows, whose records are in the order of the lanes: a wave takes four values of each half of 32 rows'
+// lanes (a piece), PG waves a piece, each for a run of the parts. (Records as rows, which the main kernel then writes in pieces of
+// 32 bytes: 2 trees of 36 on 15000 keys 40.5 us instead of 38.5, 16 on 3000 51 instead of 48.7.)
+template <typename T, int D, int kRows, int PG>
+__global__ __launch_bounds__(256) void paged_tree_merge_lanes(const float* __restrict__ part, const PagedTile* __restrict__ tiles,
+                                                              PagedBatch bt, PagedPlan plan, T* __restrict__ out, float scale) {
+  constexpr int kPieces = D / 8, kHere = 4 / PG, kChunks = kRows / 32 * kPieces / kHere, kRec = paged_rec<D>();
+  __shared__ f32x4 s_num[PG > 1 ? 256 : 1];
+  __shared__ float s_top[PG > 1 ? 256 : 1], s_den[PG > 1 ? 256 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
+  const int work = tiles[0].parts * kChunks;
+  const float c2 = score_scale(scale);
+  for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
+    const PagedTile t = tiles[1 + idx / kChunks];
+    if (!tile_holds<kRows>(t, bt, plan)) continue;
+    const int at = idx % kChunks * kHere + wave / PG, rgrp = at / kPieces, piece = at % kPieces, row = t.tile * kRows + 32 * rgrp + j;
+    const float* rec = part + ((size_t)t.rec * kRows + 32 * rgrp) * kRec;
+    const size_t step = (size_t)kRows * kRec;
+    const int per = (t.parts + PG - 1) / PG, p1 = min(t.parts, (wave % PG + 1) * per);
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f, top = -INFINITY;
+    if (row < t.nq * plan.G) {
+      for (int p0 = wave % PG * per; p0 < p1; p0 += 8) {      // eight records' loads in flight
+        float m[8], l[8], nm = top;
+        f32x4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float* from = rec + (size_t)min(p0 + u, p1 - 1) * step;
+          m[u] = from[j];
+          l[u] = from[32 + j];
+          v[u] = *reinterpret_cast<const f32x4*>(from + 64 + 256 * piece + 4 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) nm = fmaxf(nm, m[u]);
+        const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - nm) * c2);
+        den *= f0;
+        num *= f0;
+        top = nm;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (p0 + u >= p1) continue;
+          // (no score of a part's keys above -inf: its sums are zeros, or NaN where a score was, which factor 0 keeps)
+          const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[u] - top) * c2);
+          den = fmaf(f, l[u], den);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) num[e] = fmaf(f, v[u][e], num[e]);
+        }
+      }
+    }
+    if constexpr (PG > 1) {
+      __syncthreads();                                        // (the round before has been read)
+      s_num[threadIdx.x] = num;
+      s_top[threadIdx.x] = top;
+      s_den[threadIdx.x] = den;
+      __syncthreads();
+      if (wave % PG) continue;
+#pragma unroll
+      for (int i = 1; i < PG; ++i) top = fmaxf(top, s_top[threadIdx.x + 64 * i]);
+      num = f32x4{0.f, 0.f, 0.f, 0.f};
+      den = 0.f;
+#pragma unroll
+      for (int i = 0; i < PG; ++i) {
+        const float m = s_top[threadIdx.x + 64 * i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c2);
+        den = fmaf(f, s_den[threadIdx.x + 64 * i], den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, s_num[threadIdx.x + 64 * i][e], num[e]);
+      }
+    }
+    if (row >= t.nq * plan.G) continue;
+    const int tok = div(row, plan.by_g), g = row - tok * plan.G;
+    PagedUnit un{};
+    un.first = t.first;
+    un.nq = t.nq;
+    un.len = t.len;
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 8 * piece + 4 * h, num, den, some_key<true>(bt, un, tok));
   }
 }
 
@@ -1033,6 +1126,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
       return launch(kernel, dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(256), 0, st, static_cast<const float*>(records),
                     static_cast<const PagedTile*>(tiles), a.batch, p, static_cast<T*>(a.out), a.scale);
     };
+    if constexpr (KG == 1) return 4 * work <= 2048 ? join(paged_tree_merge_lanes<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge_lanes<T, D, kRows, 1>, work);
     return 4 * work <= 2048 ? join(paged_tree_merge<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge<T, D, kRows, 1>, work);
   } else {
   constexpr int kHere = paged_merge_rows<D, kRows>();

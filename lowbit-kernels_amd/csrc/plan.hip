@@ -20,6 +20,7 @@ constexpr int kSmallSeqs = 1024, kSmallTokens = 4096, kSmallList = kSmallTokens 
 constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 15;
 constexpr int kHashSeqs = 1024;          // sequences whose hash lies in LDS
 constexpr int kStartSeqs = 4096;         // sequences whose starts every workgroup copies to LDS
+constexpr int kFinishTokens = 8192;      // tokens that the workgroup which hands out the pages numbers too
 
 // The state of a call, in LDS or in the workspace: [B] each but off and start ([B + 1])
 struct PlanState {
@@ -321,7 +322,8 @@ __device__ __forceinline__ void give_token(const PlanArgs& a, const PlanState& s
 
 }  // namespace
 
-// The whole plan by one workgroup.
+// The whole plan by one workgroup: what it takes is its chain of round trips to memory and of barriers (a tree of 26 tokens 6.8 us, 128
+// beams' rows of 141 pages 12.4). Up to kSmallEntries table entries, which one CU reads as fast as the launches beyond take.
 __global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, int lanes_log, int shift, int hash_mask) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
   __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
@@ -398,10 +400,11 @@ __global__ __launch_bounds__(kThreads) void plan_small_kernel(PlanArgs a, int la
   for (int t = tid; t < a.T; t += threads) give_token(a, s, shift, t, [&](int first, int n) { return s_parent[first + n]; });
 }
 
-// The same in four launches, the state in the workspace: the lengths, beside the clearing of what the pages are marked in; the
-// pages kept, 1024 entries of a row a workgroup; the pages handed out; tables and tokens. (256 sequences on 300 .. 30000 keys in pages
-// of 16, us: 2.4, 4.4, 6.2 and 4.1. The pages handed out by the last workgroup that marks, whose marks then go past the L2: 17.9
-// for both.)
+// The same in three launches, the state in the workspace: the lengths, beside the clearing of what the pages are marked in; the pages
+// kept, 1024 entries of a row a workgroup; the pages handed out, tables and tokens. 256 sequences on 300 .. 30000 keys in pages of 16,
+// 4500 tokens: 2.3, 4.3 and 11.1 us, the chain of round trips of one workgroup (its bytes would take 0.5). Beyond kFinishTokens or
+// kHashSeqs the tables and tokens take a launch of their own (6.2 and 4.1 us here, and one launch more of the host's). The pages handed
+// out by the last workgroup that marks, whose marks then go past the L2: 17.9 us for both, not kept.
 __global__ __launch_bounds__(kThreads) void plan_lens_kernel(PlanArgs a, PlanState s, int shift, int64_t clear) {
   __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
   int turn = 0;
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(256) void plan_mark_kernel(PlanArgs a, PlanState s,
   }
 }
 
-__global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanState s, int shift) {
+__global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanState s, int shift, bool finish) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_plan[];
   __shared__ __attribute__((aligned(16))) ScanWaves s_wave;
   __shared__ int s_over, s_before[kThreads];
@@ -449,9 +452,21 @@ __global__ __launch_bounds__(kThreads) void plan_assign_kernel(PlanArgs a, PlanS
       s.hash_owner[i] = 0;
       s.hash_page[i] = -1;
     }
+    if (finish) {                                             // what the searches read, in LDS
+      int* copy = s.hash_page + s.hash_mask + 1;
+      for (int i = threadIdx.x; i <= a.B; i += kThreads) copy[i] = s.start[i];
+      s.start = copy;
+      s.off = copy + a.B + 1;
+    }
   }
   __syncthreads();
   plan_assign<false>(a, s, shift, s_wave, turn, &s_over, s_free, s_before);
+  if (!finish) return;
+  __syncthreads();
+  for (int j = threadIdx.x; j < s.off[a.B]; j += kThreads) give_page(a, s, shift, j);
+  for (int b = threadIdx.x; b < a.B; b += kThreads) give_copy(a, s, shift, b);
+  for (int t = threadIdx.x; t < a.T; t += kThreads)
+    give_token(a, s, shift, t, [&](int first, int n) { return a.parents[first + n]; });
 }
 
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s, int shift) {
@@ -660,11 +675,14 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     e = launch(plan_lens_kernel, dim3((unsigned)(1 + std::min<int64_t>((clear + kThreads - 1) / kThreads, 512))), dim3(kThreads), 0, st,
                a, s, shift, clear);
     const int chunks = (a.width + 1023) / 1024;
-    static_assert(12 * 2 * kHashSeqs + 24 * 1024 <= 64 * 1024, "LDS");
     if (e == hipSuccess) e = launch(plan_mark_kernel, dim3((unsigned)(a.B * chunks)), dim3(256), 0, st, a, s, chunks, shift);
-    if (e == hipSuccess) e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places, st, a, s, shift);
-    const int64_t items = std::max<int64_t>(a.T, a.B);
+    const bool finish = !far && a.T <= kFinishTokens;
+    static_assert(12 * 2 * kHashSeqs + 8 * (kHashSeqs + 1) + 24 * 1024 <= 64 * 1024, "LDS");
     if (e == hipSuccess)
+      e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places + (finish ? 8 * (size_t)(a.B + 1) : 0), st, a, s,
+                 shift, finish);
+    const int64_t items = std::max<int64_t>(a.T, a.B);
+    if (e == hipSuccess && !finish)
       e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256),
                  a.B <= kStartSeqs ? 8 * (size_t)(a.B + 1) : 0, st, a, s, shift);
   }

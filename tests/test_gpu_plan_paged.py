@@ -243,6 +243,9 @@ def test_more_sequences_and_pages_than_one_workgroup_takes(cuda):
     check([[700001, 3]], [17], [40], 40, 700002, ps, wide=False)
     check([[i for i in range(260)]], [16 * 260 - 3], [5000], 5000, 1 << 18, ps, wide=False)
     check([[5, 6]], [20], [4097], 4097, 300, ps, wide=False)
+    check([[5, 6], [7, 9]], [20, 3], [9000, 77], 9080, 900, ps, wide=False)
+    table, past, new, pages = make(rng, 300, 60, ps, share=0.3)
+    check(table, past, [60] * 300, 18000, pages + 2000, ps, parents=[rng.randrange(60) for _ in range(18000)], wide=False)
 
 
 def test_the_same_again_on_streams_and_in_graphs(cuda):
