@@ -1080,9 +1080,12 @@ inline PagedLaunch tree_launch(const PagedAttentionArgs& a) {
   p.rg = small ? 1 : 4;
   p.kg = small ? 4 : 1;
   const int block = 32 * p.kg;
-  p.slots = 256 * paged_per_cu(p.rg, p.kg);
+  // (heads of 64 leave room for a third workgroup of 128 rows a CU, by LDS and registers: 14 / 2 heads, 8 of 200 nodes on 2000 keys
+  // 44 us with two, 39 with three, 40 of 40 on 1000 .. 9000 60.7 / 55; parts of 384 keys at least then, as a block takes less)
+  const bool third = !small && a.D == 64;
+  p.slots = 256 * (third ? 3 : paged_per_cu(p.rg, p.kg));
   p.units = tiles(32 * p.rg);
-  p.least = small ? 1 : kPagedLeast / block;
+  p.least = small ? 1 : (third ? 384 : kPagedLeast) / block;
   const int64_t blocks = ((int64_t)a.max_keys + block - 1) / block;
   const bool whole = small ? a.max_keys <= kPagedWhole || (a.max_keys <= 2 * kPagedWhole && p.units >= 64)
                            : blocks <= 64 && blocks * (p.slots - p.units) <= 5120;
