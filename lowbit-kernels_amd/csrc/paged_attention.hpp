@@ -348,8 +348,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
   PagedUnit un;
   const PagedSeq s0 = paged_seq<kRows, BK>(bt, G, lane);
   const int share = paged_share<kRows, BK, kTree>(bt, plan, s0, lane);
-  if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, share, blockIdx.x, lane, un)) return;
-  if constexpr (kTree) {                                      // for the join: tiles[0].parts is how many follow
+  if constexpr (kTree) {                                      // for the join: tiles[0].parts is how many follow (also where none has work)
     if (plan.cap > 1 && blockIdx.x == 0 && wave == 0) {
       float split = 0.f;                                      // (below 2^24: exact)
       for (int at = 0; at < bt.B; at += 64) {
@@ -358,6 +357,9 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       }
       if (lane == 0) tiles[0].parts = (int)fminf(split * (float)Hkv, (float)plan.units);
     }
+  }
+  if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, share, blockIdx.x, lane, un)) return;
+  if constexpr (kTree) {
     if (un.parts > 1 && un.pid == 0 && tid == 0 && (uint32_t)un.tile_no < (uint32_t)plan.units)
       tiles[1 + un.tile_no] = PagedTile{un.first, un.nq, un.len, un.tile, un.hk, un.parts, un.rec, 0};
   }
@@ -662,7 +664,8 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t w = e < 2 ? p.x : p.y;
-              if ((kTree ? tree_attends(row_mask, bt.words, key - base) : key <= pr) && (odd2<T>(w) >> (16 * (e & 1)) & 0x8000u)) o[v >> 2][4 * (v & 3) + e] += Mfma<T>::half_of(w, e & 1);
+              const bool attends = kTree ? tree_attends(row_mask, bt.words, key - base) : key <= pr;
+              if (attends && (odd2<T>(w) >> (16 * (e & 1)) & 0x8000u)) o[v >> 2][4 * (v & 3) + e] += Mfma<T>::half_of(w, e & 1);
             }
           }
         }
@@ -849,8 +852,8 @@ __device__ __forceinline__ bool tile_holds(const PagedTile& t, const PagedBatch&
          t.nq <= b.T - t.first && t.tile >= 0 && t.tile <= (t.nq * p.G - 1) / kRows && (uint32_t)t.hk < (uint32_t)p.Hkv;
 }
 // The same for trees: the main kernel leaves the split tiles in tiles[], so that no workgroup looks for its own (at 16 sequences, whose
-// share takes some steps to find, the join takes 7.2 us instead of 14.3). PG groups of D / 4 lanes a row, each for a run of the parts: a lane reads the references and sums of one part each, and the
-// output's four values of all of them.
+// share takes some steps to find, the join takes 7.2 us instead of 14.3). PG groups of D / 4 lanes a row, each for a run of the parts:
+// a lane reads the references and sums of one part each, and the output's four values of all of them.
 template <typename T, int D, int kRows, int PG>
 __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict__ part, const PagedTile* __restrict__ tiles,
                                                         PagedBatch bt, PagedPlan plan, T* __restrict__ out, float scale) {
@@ -1129,13 +1132,17 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
       return launch(kernel, dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(256), 0, st, static_cast<const float*>(records),
                     static_cast<const PagedTile*>(tiles), a.batch, p, static_cast<T*>(a.out), a.scale);
     };
-    if constexpr (KG == 1) return 4 * work <= 2048 ? join(paged_tree_merge_lanes<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge_lanes<T, D, kRows, 1>, work);
-    return 4 * work <= 2048 ? join(paged_tree_merge<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge<T, D, kRows, 1>, work);
+    if constexpr (KG == 1) {
+      return 4 * work <= 2048 ? join(paged_tree_merge_lanes<T, D, kRows, 4>, 4 * work)
+                              : join(paged_tree_merge_lanes<T, D, kRows, 1>, work);
+    } else {
+      return 4 * work <= 2048 ? join(paged_tree_merge<T, D, kRows, 4>, 4 * work) : join(paged_tree_merge<T, D, kRows, 1>, work);
+    }
   } else {
-  constexpr int kHere = paged_merge_rows<D, kRows>();
-  const int64_t seqs = std::min(a.batch.B, a.batch.T), chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
-  return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
-                static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.scale);
+    constexpr int kHere = paged_merge_rows<D, kRows>();
+    const int64_t seqs = std::min(a.batch.B, a.batch.T), chunks = (((int64_t)a.batch.T * G + kHere - 1) / kHere + seqs) * a.Hkv;
+    return launch(paged_attention_merge<T, D, kRows, kBlock>, dim3((unsigned)std::min<int64_t>(chunks, 2048)), dim3(256), 0, st,
+                  static_cast<const float*>(a.ws), a.batch, p, static_cast<T*>(a.out), a.scale);
   }
 }
 

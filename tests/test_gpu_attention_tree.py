@@ -289,3 +289,18 @@ def test_many_sequences(cuda):
         lens[3], lens[n - 2] = (40, 5000), (3, 9000)
         x = batch(lens, hq, hkv, d, 32, torch.float16, n)
         check(x, lens, [tree_bits(k, i) for i, (k, _) in enumerate(lens)], 1, d ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (8, 8, 64)])
+def test_a_step_without_new_tokens(cuda, hq, hkv, d):
+    """Every row padded, after a call that leaves its split tiles in memory that the next call may get as its workspace: out stays."""
+    for lens in ([(8, 5000)], [(100, 9000), (60, 7000)]):
+        x = list(batch(lens, hq, hkv, d, 64, torch.float16, 5))
+        bits = [tree_bits(n, b) for b, (n, _) in enumerate(lens)]
+        check(x, lens, bits, 2, d ** -0.5, split=(True,))
+        masks = torch.full((x[0].shape[0], 2), -1, dtype=torch.int64, device="cuda")
+        x[4] = torch.full_like(x[4], x[0].shape[0])
+        for starts in (x[4], torch.zeros_like(x[4])):
+            x[4] = starts
+            out = call(x, masks, d ** -0.5, max(n for n, _ in lens), max(k for _, k in lens))
+            assert bool((out == 777.0).all())
