@@ -378,8 +378,10 @@ size_t lowbit_attention_paged_tree_workspace(int64_t T, int64_t B, int64_t Hq, i
  *   positions, slots [T]: token i of sequence b at position past + i in slot page * page_size + row; -1 without a page. Tokens of
  *     no sequence: 0 and -1;
  *   with parents [T] (NULL: none; node i of a sequence hangs below node parents[its row] < i, or is a root: anything else) the new
- *     tokens are trees: positions are past + depth, and masks [T][words] hold each token's own bit and its ancestors';
+ *     tokens are trees: positions are past + depth, and masks [T][words] hold each token's own bit and its ancestors'; a
+ *     sequence's new tokens past the first 1024, which no mask has room for, have position past and masks of zeros;
  *   missing [1]: pages that were wanted and not there (their table entries and slots are -1).
+ * Every sequence that keeps pages has to be in the call, with no new tokens if it pauses. Outputs overlap no inputs, but for table_out.
  * past and fresh below 0 count as 0, past above the table's width as that. workspace: lowbit_plan_paged_workspace bytes (0 for small
  * calls, NULL then), 16-byte aligned, no initial contents; calls that overlap must not share one. B at most 65536, T 2^28, width *
  * page_size and B * width 2^30. */
@@ -396,7 +398,7 @@ int lowbit_plan_paged(const int32_t* page_table, int64_t R, int64_t width, const
  * (the confirmed tokens, then one more; -1 behind), lens [B] = kv_lens - new + count. A sequence without new tokens has count 0.
  * With k_cache and v_cache (as above) the rows of the path's nodes are moved to the places right behind the sequence's earlier
  * keys, in every layer, so that its first lens[b] keys are those of the confirmed text; sequences' new tokens must lie in pages of
- * their own. One launch. */
+ * their own. Nodes past a sequence's first 1024 are not confirmed. Outputs overlap no inputs. One launch. */
 int lowbit_accept_drafts(const int64_t* tokens, const int64_t* picks, const int32_t* parents, const int32_t* q_starts,
                          const int32_t* kv_lens, const int32_t* page_table, int64_t width, void* k_cache, void* v_cache,
                          int32_t* path, int32_t* counts, int64_t* accepted, int32_t* lens, int64_t T, int64_t B, int64_t longest,

@@ -21,6 +21,7 @@ constexpr int kSmallPages = 1 << 18, kSmallEntries = 1 << 15;
 constexpr int kHashSeqs = 1024;          // sequences whose hash lies in LDS
 constexpr int kStartSeqs = 4096;         // sequences whose starts every workgroup copies to LDS
 constexpr int kFinishTokens = 8192;      // tokens that the workgroup which hands out the pages numbers too
+constexpr int kMostNodes = 64 * kMaxMaskWords;   // of a tree: later ones are attended by none
 
 // The state of a call, in LDS or in the workspace: [B] each but off and start ([B + 1])
 struct PlanState {
@@ -303,15 +304,17 @@ __device__ __forceinline__ void give_token(const PlanArgs& a, const PlanState& s
     a.positions[t] = key;
     return;
   }
-  // up to the root, once a word
-  int depth = 0;
-  for (int w = 0; w < a.words; ++w) {
+  // up to the root, each word's nodes in turn (a node hangs below an earlier one); past the words' most nodes there is no tree
+  int depth = 0, n = i < kMostNodes ? i : -1;
+  for (int w = a.words - 1; w >= 0; --w) {
     uint64_t bits = 0;
-    depth = 0;
-    for (int n = i;;) {
+    while (n >= 64 * w) {
       if (n >> 6 == w) bits |= (uint64_t)1 << (n & 63);
       const int p = parent(first, n);
-      if (p < 0 || p >= n) break;                             // (a node hangs below an earlier one)
+      if (p < 0 || p >= n) {
+        n = -1;
+        break;
+      }
       n = p;
       ++depth;
     }
@@ -489,7 +492,8 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanState s,
     give_token(a, s, shift, t, [&](int first, int n) { return a.parents[first + n]; });
 }
 
-// Workgroup (sequence, layer): the filled rows of the page that is replaced, every head of k and v.
+// Workgroup (sequence, layer): the filled rows of the page that is replaced, every head of k and v. Bound: memory and the
+// launch (some 45 of 128 beams, 28 layers, 2 heads of 128, 19 MB read and written: 4.4 .. 6 us, 4.1 at a large copy's rate).
 __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ copies, const int* __restrict__ q_starts,
                                                         const int* __restrict__ kv_lens, uint8_t* __restrict__ k,
                                                         uint8_t* __restrict__ v, int64_t pages, int Hkv, int row_bytes, int shift) {
@@ -509,8 +513,10 @@ __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ 
 
 // accept_drafts. Workgroup (sequence, layer): its first wave follows the picks from node 0 down the tree (the first 64 nodes in its
 // lanes, a ballot a step), then the workgroup moves the confirmed nodes' rows of its layer, every head of k and v, to the places
-// behind the sequence's keys: one launch, the walk repeated in every layer (several layers a workgroup: 64 trees, 28 layers, 16.6 us instead of 14.7). Node d of the path comes to lie at place d <= the
-// node's own, so rows are read and written in order of the path, a chunk's all read before one is written.
+// behind the sequence's keys: one launch, the walk repeated in every layer. Node d of the path comes to lie at place d <= the node's
+// own, so rows are read and written in order of the path, a chunk's all read before one is written.
+// Bound: without moves the chain of round trips (one tree of 26 4.4 us, 64 trees 3.8); with them rows of 256 bytes at places all over
+// the cache: 64 trees, 28 layers, 26 MB read and written, 14.5 us, 1.8 TB/s (several layers a workgroup 16.6).
 constexpr int kMostPath = 1024;
 __device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
@@ -521,7 +527,7 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
   __shared__ int s_count;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int first = min(max(a.q_starts[b], 0), a.T), nodes = min(max(a.q_starts[b + 1], first), a.T) - first;
-  const int past = a.kv_lens[b] - nodes;
+  const int past = a.kv_lens[b] - nodes, tree = min(nodes, kMostNodes);
   const int* table = a.table + (int64_t)b * a.width;
   const int c0 = max(past, 0) >> shift;                       // s_table: the entries from there on
   if (tid < 64) {
@@ -530,22 +536,22 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
     const int* parents = a.parents ? a.parents + first : nullptr;
     int64_t token = 0, pick = 0;
     int parent = -1;
-    if (lane < nodes) {
+    if (lane < tree) {
       token = tokens[lane];
       pick = picks[lane];
       parent = parents ? parents[lane] : lane - 1;
     }
     int count = 0, cur = 0;
-    while (count < a.longest && cur < nodes) {
+    while (count < a.longest && cur < tree) {
       if (lane == 0) s_path[count] = cur;
       ++count;
       const int64_t want = cur < 64 ? readlane64(pick, cur) : picks[cur];
-      const uint64_t hit = __ballot(lane > cur && lane < nodes && parent == cur && token == want);
-      int next = hit ? __builtin_ctzll(hit) : nodes;
+      const uint64_t hit = __ballot(lane > cur && lane < tree && parent == cur && token == want);
+      int next = hit ? __builtin_ctzll(hit) : tree;
       if (!hit && (parents || cur >= 63)) {
-        for (int n0 = max(64, cur + 1); n0 < nodes && next == nodes; n0 += 64) {
+        for (int n0 = max(64, cur + 1); n0 < tree && next == tree; n0 += 64) {
           const int n = n0 + lane;
-          const uint64_t any = __ballot(n < nodes && (parents ? parents[n] : n - 1) == cur && tokens[n] == want);
+          const uint64_t any = __ballot(n < tree && (parents ? parents[n] : n - 1) == cur && tokens[n] == want);
           if (any) next = n0 + __builtin_ctzll(any);
           if (!parents) break;                                // (a chain: the next token or none)
         }

@@ -828,13 +828,14 @@ class NativeExt:
         """The tables of a step from its sequences' lengths, built on the GPU (a captured step plans itself). Sequence b goes on
         from row r = rows[b] (int32 [B]; None: b) of page_table (int32 [R, width]), whose first past[r] keys (int32 [R]) it keeps
         (r outside the table: none), with new[b] new tokens (int32 [B]); `tokens` is the step's size T (tokens past it are left
-        out). Returns a PagedStep:
+        out). Every sequence that keeps pages has to be in the call, with no new tokens if it pauses. Returns a PagedStep:
           page_table [B, width]  the kept pages, then free ones for the new keys, -1 behind (`out` if given, which may be
                                  page_table itself without rows: entries behind stay then). Free is what no sequence of the call
                                  keeps; the first free of `pages` pages go to the sequences in order
           q_starts [B + 1], kv_lens [B] (int32), positions, slots [T] (int64; 0 and -1 for tokens of no sequence)
           masks [T, words]       with parents (int32 [T]: the node of its sequence, an earlier one, that a new token hangs below;
-                                 else a root): each token's bit and its ancestors' (int64); positions go by depth then. Else None
+                                 else a root): each token's bit and its ancestors' (int64); positions go by depth then, and new
+                                 tokens past a sequence's first 1024 have masks of zeros. Else None
           copies [B, 2]          the page that a sequence's partly filled last page was copied from and to, as it would be
                                  written and another sequence reads it; -1 where there is none. With caches ((k, v) [layers,
                                  pages, hkv, page_size, D]) its rows are copied in every layer
@@ -883,7 +884,7 @@ class NativeExt:
     def accept_drafts(self, tokens, picks, parents, q_starts, kv_lens, page_table, caches, longest):
         """What the model's own picks (int64 [T], its choice after each token) confirm of drafted tokens (int64 [T]; parents as
         plan_paged takes them, None: chains): from each sequence's node 0, the first child whose token is the pick after the
-        node before, and so on, at most `longest` <= 1024 nodes. Returns path (int32 [B, longest], -1 behind), counts (int32
+        node before, and so on, at most `longest` <= 1024 nodes, of the first 1024 of a sequence. Returns path (int32 [B, longest], -1 behind), counts (int32
         [B]), accepted (int64 [B, longest]: the picks after the path's nodes, so the confirmed tokens and one more; -1 behind)
         and lens (int32 [B]: the keys that the sequence keeps, kv_lens - new + counts). With caches ((k, v) [layers, pages,
         hkv, page_size, D]; None: left to the caller) the confirmed nodes' rows are moved together behind the earlier keys."""

@@ -185,3 +185,16 @@ def test_captured(cuda):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
         assert torch.equal(caches[0], want[4][0]) and torch.equal(caches[1], want[4][1])
+
+
+def test_nodes_past_the_masks_are_not_confirmed(cuda):
+    """A child that is the 1024th node or an earlier one is, a later one, which no mask has room for, is not."""
+    n, past = 1200, 3
+    for child, count in ((1023, 2), (1024, 1), (1199, 1)):
+        tokens, parents = [5] * n, [-1] * n
+        tokens[child], parents[child] = 6, 0
+        path, counts, accepted, lens = ops.ext().accept_drafts(
+            i64(tokens), i64([6] * n), i32(parents), i32([0, n]), i32([past + n]), i32([list(range(80))]), None, 4)
+        assert counts.tolist() == [count] and lens.tolist() == [past + count]
+        assert path.tolist() == [([0, child] if count == 2 else [0]) + [-1] * (4 - count)]
+        assert accepted.tolist() == [[6] * count + [-1] * (4 - count)]

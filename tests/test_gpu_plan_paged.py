@@ -284,3 +284,17 @@ def test_the_same_again_on_streams_and_in_graphs(cuda):
             for name, a, b, c in zip(NAMES, step, eager, want):
                 if c is not None:
                     assert torch.equal(a, c) and torch.equal(b, c), (name, i)
+
+
+def test_more_nodes_than_masks_have_room_for(cuda):
+    """A chain of 1024 nodes, whose last one has them all as ancestors; new tokens past the 1024th are outside the tree."""
+    ps, past, sizes = 16, [37, 0, 5], [1500, 1024, 2]
+    for parent in (lambda i: i - 1, lambda i: i // 2 - (i % 2 == 0)):
+        parents = [parent(i) for n in sizes for i in range(n)]
+        need = [-(-(p + n) // ps) for p, n in zip(past, sizes)]
+        table = [[10 * b + i if i < -(-past[b] // ps) else -1 for i in range(max(need))] for b in range(3)]
+        want = oracle(table, past, list(sizes), sum(sizes), sum(need) + 9, ps, None, parents, 16)
+        want[3][1024:1500], want[5][1024:1500] = past[0], 0
+        got = ops.ext().plan_paged(i32(table), i32(past), i32(sizes), sum(sizes), sum(need) + 9, ps, parents=i32(parents), words=16)
+        for name, a, b in zip(NAMES, got, want):
+            assert torch.equal(a, b), name
