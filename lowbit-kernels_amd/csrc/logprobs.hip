@@ -435,6 +435,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
 // first scores, bounds what can be among the n best: of all slices' lists what reaches it is ranked by counting, a few lanes a
 // candidate. Where that is too little (few beams hold anything) or too much (ties), each beam's own n best are made first, a
 // wave a beam, and those ranked.
+// Bound: its chain of round trips and barriers, 4.8 (1 x 4 beams) .. 5.8 us (64 x 8).
 // A beam that holds nothing (a score that is no finite number) or whose row has no distribution has -inf for every token, a
 // finished one its score for `pad` and -inf for the others; equal candidates rank by beam, then by token.
 constexpr int kBeamSlices = 16, kBeamThreads = 512;
@@ -700,9 +701,9 @@ hipError_t token_logprobs_launch(const LogprobArgs& a, hipStream_t st) {
   return go(logprobs_kernel<bf16, false>, logprobs_join_kernel<bf16>, static_cast<const bf16*>(a.logits));
 }
 
-// few slices, whose lists the join has to read: 512 workgroups, two a CU (vocabulary 151936, fp16, graph-timed us with 16 slices a
-// row / 64: 1 x 4 beams 11.0 / 12.9, 1 x 8 17.1 / 20.4; with 512 workgroups in all / 1024: 8 x 4 13.0 / 17.2, 16 x 8 23.7 / 28.2, 32 x 8
-// 32.5 / 37.7, 64 x 8 46.7 / 55.1)
+// few slices, whose lists the join has to read: at most 16 a row and 512 workgroups in all (vocabulary 151936, fp16, graph-timed us, so
+// / otherwise: 1 x 4 beams 11.3, with 64 slices 12.9; 16 x 8 in 4 slices 20.3, in 8 22.1; 32 x 8 in 2 25.9, in 4 27.6; 64 x 8 in 1 38.8, in
+// 2 39.6)
 hipError_t beam_select_launch(const BeamArgs& a, hipStream_t st) {
   const int M = a.requests * a.beams, S = row_slices(M, a.V, a.n, kBeamSlices, 512, a.ws_bytes);
   const size_t lds = slice_lds(a.V, a.dtype, S, sizeof(uint2));

@@ -14,10 +14,9 @@ launches, the attention's partition merge included)
 
 with its own KV cache (forward_paged: rmsnorm -> qkv projection -> rotation + write into the pages -> attention over the pages,
 the rest alike, over the caller's caches; verify_trees and beam_search run steps of it whose tables are made on the GPU). The
-projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the
-consumer fused into the store, for up to 64 rows; dequantize + hipBLASLt beyond) or fp16 (hipBLASLt through torch,
-bias and residual folded into addmm, silu * up as two torch ops), so the two variants share every other kernel and
-differ only in the projections. Weights come from a transformers Qwen2ForCausalLM; q|k|v are merged into one
+projections are either W4A16 (lowbit_w4_linear_fused: GEMV / MFMA kernels with the consumer fused into the store, for up
+to 64 rows; dequantize + hipBLASLt beyond) or fp16 (hipBLASLt through torch, bias and residual folded into addmm, silu * up
+as two torch ops), so the two variants share every other kernel and differ only in the projections. Weights come from a transformers Qwen2ForCausalLM; q|k|v are merged into one
 projection and gate|up into another, their rows interleaved 8 gate / 8 up per 16-row tile for the silu epilogue.
 """
 import math
