@@ -750,8 +750,8 @@ static int attend_pages(const void* q, int dtype, const void* k_cache, const voi
   a.ws = workspace;
   a.ws_bytes = workspace ? workspace_bytes : 0;
   if (!masks) return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
-  a.batch.masks = masks;
-  a.batch.words = (int)words;
+  a.masks = masks;
+  a.words = (int)words;
   return hip_status(attention_paged_tree_launch(a, static_cast<hipStream_t>(stream)), "attention_paged_tree");
 }
 

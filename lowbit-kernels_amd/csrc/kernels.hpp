@@ -384,9 +384,6 @@ struct PagedBatch {
   const int* kv_lens;
   int T, B, table_width, page_size;
   int64_t pages;
-  // attention of a tree: bit i of row t's words (masks + t * words): the token attends its sequence's new token i
-  const uint64_t* masks;
-  int words;
 };
 constexpr int kMaxMaskWords = 16;
 struct PagedAttentionArgs {
@@ -399,6 +396,8 @@ struct PagedAttentionArgs {
   float scale;
   void* ws;
   size_t ws_bytes;
+  const uint64_t* masks;           // of trees: [T][words]
+  int words;
 };
 hipError_t attention_paged_launch(const PagedAttentionArgs& a, hipStream_t st);
 hipError_t attention_paged_tree_launch(const PagedAttentionArgs& a, hipStream_t st);   // (paged_tree.hip)

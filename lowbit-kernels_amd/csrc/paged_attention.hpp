@@ -44,13 +44,23 @@ struct PagedPlan {
   int least;         // blocks of a part at least
   int cap;           // parts of a tile at most (1: no split)
   int most;          // parts of split tiles in all at most (what the workspace holds, twice its share)
-  int units;         // kTree: split tiles at most (what the workspace has room to describe)
   int Hq, Hkv, G;
   FastDiv by_hkv, by_g;
 };
 struct PagedTile {   // kTree: a tile as the join of its parts finds it
   int first, nq, len, tile, hk, parts, rec, unused;
 };
+// what a call over trees has beside: bit i of row t's words (masks + t * words): the token attends its sequence's new token i.
+// (An argument of its own, so that the causal kernels' stay as short as they were: 0.2 .. 0.4 us a call)
+struct PagedTrees {
+  const uint64_t* masks;
+  PagedTile* tiles;
+  int words;
+  int units;         // split tiles at most (what the workspace has room to describe)
+};
+struct PagedNoTrees {};
+template <bool kTree>
+using PagedTreesOf = std::conditional_t<kTree, PagedTrees, PagedNoTrees>;
 struct PagedUnit {
   int seq, first, nq, len, tiles, parts, tile, hk, pid, rec, tile_no;   // tile_no (kTree): of the split tiles; first: the sequence's first row of q; rec: the part's record (parts > 1)
 };
@@ -259,12 +269,12 @@ __device__ __forceinline__ bool tree_attends(const uint64_t* mask, int words, in
 }
 // whether the sequence's token t attends any key
 template <bool kTree>
-__device__ __forceinline__ bool some_key(const PagedBatch& b, const PagedUnit& u, int t) {
+__device__ __forceinline__ bool some_key(const PagedBatch& b, const uint64_t* masks, int words, const PagedUnit& u, int t) {
   const int base = u.len - u.nq;
   if constexpr (!kTree) return base + t >= 0;
   if (base > 0) return true;
-  const uint64_t* mask = b.masks + (int64_t)(u.first + t) * b.words;
-  const int end = min(min(u.nq, 64 * b.words), min(u.len, b.table_width * b.page_size) - base);   // nodes that have a key: -base ..
+  const uint64_t* mask = masks + (int64_t)(u.first + t) * words;
+  const int end = min(min(u.nq, 64 * words), min(u.len, b.table_width * b.page_size) - base);   // nodes that have a key: -base ..
   uint64_t any = 0;
   for (int w = -base >> 6; 64 * w < end; ++w) {
     const int lo = -base - 64 * w, n = end - 64 * w;
@@ -325,7 +335,7 @@ __device__ __forceinline__ float score_scale(float scale) {
 template <typename T, int D, int RG, int KG, bool kTree>
 __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, PagedBatch bt, PagedPlan plan,
-    T* __restrict__ out, float* __restrict__ part, PagedTile* __restrict__ tiles, int shift, float scale) {
+    T* __restrict__ out, float* __restrict__ part, int shift, float scale, PagedTreesOf<kTree> tr) {
   constexpr int NW = RG * KG;
   constexpr int RB = D * 2;                                  // bytes of a row
   constexpr int PR = RB / 16;                                // its pieces
@@ -355,13 +365,13 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
         const PagedSeq s = at == 0 ? s0 : paged_seq<kRows, BK>(bt, G, at + lane);
         split += wave_sum((float)(s.blocks > share ? s.tiles : 0));
       }
-      if (lane == 0) tiles[0].parts = (int)fminf(split * (float)Hkv, (float)plan.units);
+      if (lane == 0) tr.tiles[0].parts = (int)fminf(split * (float)Hkv, (float)tr.units);
     }
   }
   if (!paged_unit<kRows, BK, 0, kTree>(bt, plan, s0, share, blockIdx.x, lane, un)) return;
   if constexpr (kTree) {
-    if (un.parts > 1 && un.pid == 0 && tid == 0 && (uint32_t)un.tile_no < (uint32_t)plan.units)
-      tiles[1 + un.tile_no] = PagedTile{un.first, un.nq, un.len, un.tile, un.hk, un.parts, un.rec, 0};
+    if (un.parts > 1 && un.pid == 0 && tid == 0 && (uint32_t)un.tile_no < (uint32_t)tr.units)
+      tr.tiles[1 + un.tile_no] = PagedTile{un.first, un.nq, un.len, un.tile, un.hk, un.parts, un.rec, 0};
   }
   const int rgrp = wave % RG, kgrp = wave / RG;
   const int cap = bt.table_width * bt.page_size;
@@ -396,18 +406,21 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 
   // ---- kTree: which nodes a row attends ----
   // Its token's first word stays in registers; where there are more, the words of all the tile's tokens lie behind the slots
-  [[maybe_unused]] const uint64_t* row_mask = nullptr;
+  [[maybe_unused]] const uint64_t *masks = nullptr, *row_mask = nullptr;
+  [[maybe_unused]] int words = 1;
   [[maybe_unused]] uint64_t word0 = 0;
   [[maybe_unused]] uint64_t* s_mask = nullptr;
   if constexpr (kTree) {
-    const int tok0 = div(un.tile * kRows, plan.by_g), n = (tok_last - tok0 + 1) * bt.words;
-    row_mask = bt.masks + (int64_t)(un.first + tok) * bt.words;
+    masks = tr.masks;
+    words = tr.words;
+    const int tok0 = div(un.tile * kRows, plan.by_g), n = (tok_last - tok0 + 1) * words;
+    row_mask = masks + (int64_t)(un.first + tok) * words;
     word0 = row_mask[0];
-    if (bt.words > 1) {
+    if (words > 1) {
       s_mask = reinterpret_cast<uint64_t*>(smem + paged_lds<D, RG, KG>());
-      const uint64_t* from = bt.masks + (int64_t)(un.first + tok0) * bt.words;
+      const uint64_t* from = masks + (int64_t)(un.first + tok0) * words;
       for (int i = tid; i < n; i += 64 * NW) s_mask[i] = from[i];
-      s_mask += (tok - tok0) * bt.words;
+      s_mask += (tok - tok0) * words;
       lds_barrier();
     }
     uint32_t lo = (uint32_t)word0, hi = (uint32_t)(word0 >> 32);
@@ -423,7 +436,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
         w = ((uint32_t)word0 << -n0) | ((1u << -n0) - 1u);
       } else {
         const int at = n0 >> 6, sh = n0 & 63;
-        auto word = [&](int i) -> uint64_t { return i >= bt.words ? 0 : i == 0 ? word0 : s_mask[i]; };
+        auto word = [&](int i) -> uint64_t { return i >= words ? 0 : i == 0 ? word0 : s_mask[i]; };
         w = (uint32_t)(word(at) >> sh);
         if (sh > 32) w |= (uint32_t)(word(at + 1) << (64 - sh));
       }
@@ -664,7 +677,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t w = e < 2 ? p.x : p.y;
-              const bool attends = kTree ? tree_attends(row_mask, bt.words, key - base) : key <= pr;
+              const bool attends = kTree ? tree_attends(row_mask, words, key - base) : key <= pr;
               if (attends && (odd2<T>(w) >> (16 * (e & 1)) & 0x8000u)) o[v >> 2][4 * (v & 3) + e] += Mfma<T>::half_of(w, e & 1);
             }
           }
@@ -710,7 +723,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
       }
       const int at_row = un.tile * kRows + r, t = div(at_row, plan.by_g), g = at_row - t * G;
       if (un.parts == 1) {
-        store_row<T>(out + ((int64_t)(un.first + t) * Hq + un.hk * G + g) * D + d, num, all, some_key<kTree>(bt, un, t));
+        store_row<T>(out + ((int64_t)(un.first + t) * Hq + un.hk * G + g) * D + d, num, all, some_key<kTree>(bt, masks, words, un, t));
       } else {
         float* rec = part + ((size_t)un.rec * kRows + r) * paged_rec<D>();
         if (d == 0) {
@@ -726,7 +739,7 @@ __global__ __launch_bounds__(64 * RG * KG, KG > 1 ? 1 : 2) void paged_attention(
   // lane (j, h) holds O^T[32 dt + 8 (v / 4) + 4 h + v % 4][row j]
   if (un.parts == 1) {
     T* dst = out + qrow + 4 * h;
-    const bool some = kTree ? some_key<kTree>(bt, un, tok) : pr >= 0;
+    const bool some = kTree ? some_key<kTree>(bt, masks, words, un, tok) : pr >= 0;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -855,16 +868,16 @@ __device__ __forceinline__ bool tile_holds(const PagedTile& t, const PagedBatch&
 // share takes some steps to find, the join takes 7.2 us instead of 14.3). PG groups of D / 4 lanes a row, each for a run of the parts:
 // a lane reads the references and sums of one part each, and the output's four values of all of them.
 template <typename T, int D, int kRows, int PG>
-__global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict__ part, const PagedTile* __restrict__ tiles,
-                                                        PagedBatch bt, PagedPlan plan, T* __restrict__ out, float scale) {
+__global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict__ part, PagedTrees tr, PagedBatch bt, PagedPlan plan,
+                                                        T* __restrict__ out, float scale) {
   constexpr int kLanes = D / 4, kHere = 256 / kLanes / PG, kChunks = kRows / kHere, kRec = paged_rec<D>();
   __shared__ f32x4 s_num[PG > 1 ? 256 : 1];
   __shared__ float s_top[256 / kLanes], s_den[256 / kLanes];
   const int c = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int work = tiles[0].parts * kChunks;
+  const int work = tr.tiles[0].parts * kChunks;
   const float c2 = score_scale(scale);
   for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
-    const PagedTile t = tiles[1 + idx / kChunks];
+    const PagedTile t = tr.tiles[1 + idx / kChunks];
     if (!tile_holds<kRows>(t, bt, plan)) continue;
     const int r = idx % kChunks * kHere + grp / PG, row = t.tile * kRows + r;
     const float* rec = part + ((size_t)t.rec * kRows + r) * kRec;
@@ -936,7 +949,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
     un.first = t.first;
     un.nq = t.nq;
     un.len = t.len;
-    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den, some_key<true>(bt, un, tok));
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den, some_key<true>(bt, tr.masks, tr.words, un, tok));
   }
 }
 
@@ -944,16 +957,16 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
 // lanes (a piece), PG waves a piece, each for a run of the parts. (Records as rows, which the main kernel then writes in pieces of
 // 32 bytes: 2 trees of 36 on 15000 keys 40.5 us instead of 38.5, 16 on 3000 51 instead of 48.7.)
 template <typename T, int D, int kRows, int PG>
-__global__ __launch_bounds__(256) void paged_tree_merge_lanes(const float* __restrict__ part, const PagedTile* __restrict__ tiles,
-                                                              PagedBatch bt, PagedPlan plan, T* __restrict__ out, float scale) {
+__global__ __launch_bounds__(256) void paged_tree_merge_lanes(const float* __restrict__ part, PagedTrees tr, PagedBatch bt, PagedPlan plan,
+                                                              T* __restrict__ out, float scale) {
   constexpr int kPieces = D / 8, kHere = 4 / PG, kChunks = kRows / 32 * kPieces / kHere, kRec = paged_rec<D>();
   __shared__ f32x4 s_num[PG > 1 ? 256 : 1];
   __shared__ float s_top[PG > 1 ? 256 : 1], s_den[PG > 1 ? 256 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
-  const int work = tiles[0].parts * kChunks;
+  const int work = tr.tiles[0].parts * kChunks;
   const float c2 = score_scale(scale);
   for (int idx = blockIdx.x; idx < work; idx += gridDim.x) {
-    const PagedTile t = tiles[1 + idx / kChunks];
+    const PagedTile t = tr.tiles[1 + idx / kChunks];
     if (!tile_holds<kRows>(t, bt, plan)) continue;
     const int at = idx % kChunks * kHere + wave / PG, rgrp = at / kPieces, piece = at % kPieces, row = t.tile * kRows + 32 * rgrp + j;
     const float* rec = part + ((size_t)t.rec * kRows + 32 * rgrp) * kRec;
@@ -1014,7 +1027,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge_lanes(const float* __res
     un.first = t.first;
     un.nq = t.nq;
     un.len = t.len;
-    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 8 * piece + 4 * h, num, den, some_key<true>(bt, un, tok));
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 8 * piece + 4 * h, num, den, some_key<true>(bt, tr.masks, tr.words, un, tok));
   }
 }
 
@@ -1102,15 +1115,16 @@ inline size_t paged_record_bytes(int rg, int D) { return (size_t)32 * rg * (D ==
 template <typename T, int D, int RG, int KG, bool kTree>
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch& l, hipStream_t st) {
   constexpr size_t most_lds = paged_lds<D, RG, KG>() + (kTree ? (size_t)32 * RG * kMaxMaskWords * 8 : 0);
-  const size_t lds = paged_lds<D, RG, KG>() + (kTree && a.batch.words > 1 ? (size_t)32 * RG * a.batch.words * 8 : 0);
+  const size_t lds = paged_lds<D, RG, KG>() + (kTree && a.words > 1 ? (size_t)32 * RG * a.words * 8 : 0);
   constexpr int kRows = 32 * RG, kBlock = 32 * KG;
   const int G = a.Hq / a.Hkv;
-  PagedPlan p{l.slots, l.least, 1, 0, (int)l.units, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
+  PagedPlan p{l.slots, l.least, 1, 0, a.Hq, a.Hkv, G, fast_div(a.Hkv), fast_div(G)};
   // kTree: the tiles' descriptions before the records
   const size_t head = kTree ? (size_t)(l.units + 1) * sizeof(PagedTile) : 0;
   p.most = a.ws && a.ws_bytes > head ? (int)std::min<size_t>((size_t)l.records, (a.ws_bytes - head) / paged_record_bytes(RG, D)) : 0;
   if (p.most >= 2) p.cap = l.cap;
-  PagedTile* tiles = kTree && p.cap > 1 ? static_cast<PagedTile*>(a.ws) : nullptr;
+  PagedTreesOf<kTree> trees{};
+  if constexpr (kTree) trees = PagedTrees{a.masks, p.cap > 1 ? static_cast<PagedTile*>(a.ws) : nullptr, a.words, (int)l.units};
   float* records = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + head);
   // (paged_share: parts take its free slots beside one a tile, or those of whole rounds)
   const int64_t rounds = (l.units + l.slots - 1) / l.slots * l.slots;
@@ -1123,14 +1137,14 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedLaunch
   const int shift = log2_of(a.batch.page_size);
   hipError_t e = launch(paged_attention<T, D, RG, KG, kTree>, dim3((unsigned)grid), dim3(64 * RG * KG), lds, st,
                         static_cast<const T*>(a.q), static_cast<const T*>(a.k_cache), static_cast<const T*>(a.v_cache),
-                        a.batch, p, static_cast<T*>(a.out), records, tiles, shift, a.scale);
+                        a.batch, p, static_cast<T*>(a.out), records, shift, a.scale, trees);
   if (e != hipSuccess || p.cap == 1) return e;
   if constexpr (kTree) {
     // four groups a row while that many workgroups run at once: few rows of many parts
     const int64_t work = l.units * (kRows * D / 1024);
     auto join = [&](auto kernel, int64_t n) {
       return launch(kernel, dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(256), 0, st, static_cast<const float*>(records),
-                    static_cast<const PagedTile*>(tiles), a.batch, p, static_cast<T*>(a.out), a.scale);
+                    trees, a.batch, p, static_cast<T*>(a.out), a.scale);
     };
     if constexpr (KG == 1) {
       return 4 * work <= 2048 ? join(paged_tree_merge_lanes<T, D, kRows, 4>, 4 * work)
