@@ -62,7 +62,8 @@ struct PagedNoTrees {};
 template <bool kTree>
 using PagedTreesOf = std::conditional_t<kTree, PagedTrees, PagedNoTrees>;
 struct PagedUnit {
-  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec, tile_no;   // tile_no (kTree): of the split tiles; first: the sequence's first row of q; rec: the part's record (parts > 1)
+  int seq, first, nq, len, tiles, parts, tile, hk, pid, rec;   // first: the sequence's first row of q; rec: the part's record (parts > 1)
+  int tile_no;       // kTree: of the split tiles
 };
 
 // sum of the lanes up to and including this one
@@ -949,7 +950,8 @@ __global__ __launch_bounds__(256) void paged_tree_merge(const float* __restrict_
     un.first = t.first;
     un.nq = t.nq;
     un.len = t.len;
-    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den, some_key<true>(bt, tr.masks, tr.words, un, tok));
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 4 * c, num, den,
+                 some_key<true>(bt, tr.masks, tr.words, un, tok));
   }
 }
 
@@ -1027,7 +1029,8 @@ __global__ __launch_bounds__(256) void paged_tree_merge_lanes(const float* __res
     un.first = t.first;
     un.nq = t.nq;
     un.len = t.len;
-    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 8 * piece + 4 * h, num, den, some_key<true>(bt, tr.masks, tr.words, un, tok));
+    store_row<T>(out + ((int64_t)(t.first + tok) * plan.Hq + t.hk * plan.G + g) * D + 8 * piece + 4 * h, num, den,
+                 some_key<true>(bt, tr.masks, tr.words, un, tok));
   }
 }
 

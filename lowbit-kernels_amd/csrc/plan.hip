@@ -645,7 +645,8 @@ static int64_t plan_clear(const PlanArgs& a) {   // 16-byte pieces that have to 
 }
 size_t plan_paged_workspace(const PlanArgs& a) {
   if (plan_is_small(a)) return 0;
-  const int64_t ints = 4 * plan_clear(a) + (a.B > kHashSeqs ? hash_places(a.B) : 0) + 6 * (int64_t)a.B + 2 + list_places(a, log2_of(a.page_size));
+  const int64_t hash = a.B > kHashSeqs ? hash_places(a.B) : 0;
+  const int64_t ints = 4 * plan_clear(a) + hash + 6 * (int64_t)a.B + 2 + list_places(a, log2_of(a.page_size));
   return (size_t)(4 * ints + 15) / 16 * 16;
 }
 
@@ -685,8 +686,8 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     const bool finish = !far && a.T <= kFinishTokens;
     static_assert(12 * 2 * kHashSeqs + 8 * (kHashSeqs + 1) + 24 * 1024 <= 64 * 1024, "LDS");
     if (e == hipSuccess)
-      e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places + (finish ? 8 * (size_t)(a.B + 1) : 0), st, a, s,
-                 shift, finish);
+      e = launch(plan_assign_kernel, dim3(1), dim3(kThreads), far ? 0 : 12 * (size_t)places + (finish ? 8 * (size_t)(a.B + 1) : 0),
+                 st, a, s, shift, finish);
     const int64_t items = std::max<int64_t>(a.T, a.B);
     if (e == hipSuccess && !finish)
       e = launch(plan_fill_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256),
