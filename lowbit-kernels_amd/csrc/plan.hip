@@ -158,6 +158,7 @@ template <bool kLds>
 __device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& s, int shift, ScanWaves& s_wave, int& turn,
                                             int* s_over, uint32_t* s_free, int* s_before) {
   const int tid = threadIdx.x, threads = blockDim.x, words = (int)((a.pages + 31) >> 5);
+  const bool far = !kLds && a.B > kHashSeqs;                  // the hash lies in the workspace
   auto mask = [&](int w) {
     const int64_t left = a.pages - 32 * (int64_t)w;
     return w < words ? free_pages<kLds>(s, w) & (left >= 32 ? ~0u : (1u << left) - 1u) : 0u;
@@ -189,7 +190,13 @@ __device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& 
       break;
     }
   }
+  if (far) vm_drain();                                        // (the owners, which other waves read behind the barrier)
   lds_barrier();
+  // (in the workspace: past the L1, which the atomics above pass by)
+  auto hash_page = [&](int at) { return far ? __hip_atomic_load(s.hash_page + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : s.hash_page[at]; };
+  auto hash_owner = [&](int at) {
+    return far ? __hip_atomic_load(s.hash_owner + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : s.hash_owner[at];
+  };
   int total = 0;
   for (int b0 = 0; b0 < a.B; b0 += threads) {
     const int b = b0 + tid;
@@ -202,8 +209,8 @@ __device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& 
       if (fresh > 0 && page >= 0) {
         copy = page_used<kLds>(s, page);                      // (within another's keys)
         int at = hash_slot(page, s.hash_mask);
-        while (s.hash_page[at] != page) at = (at + 1) & s.hash_mask;
-        copy |= s.hash_owner[at] != owner_key(past, fresh, b);
+        while (hash_page(at) != page) at = (at + 1) & s.hash_mask;
+        copy |= hash_owner(at) != owner_key(past, fresh, b);
       }
       want = min(need, a.width) - have + (copy ? 1 : 0);
       if (need > a.width) atomicAdd(s_over, need - a.width);  // pages that the table has no place for
