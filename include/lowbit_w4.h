@@ -374,7 +374,8 @@ size_t lowbit_attention_paged_tree_workspace(int64_t T, int64_t B, int64_t Hq, i
  *   copies [B][2]: where a sequence's last page is partly filled, is to be written and holds keys of another sequence, the page and
  *     the free one that takes its place (else -1, -1): of several that it is the last one of, the sequence with the most keys, then
  *     the first that writes, keeps it, unless it lies within another's keys. With k_cache and v_cache [layers][pages][Hkv][page_size]
- *     of row_bytes (both or neither NULL) the filled rows are copied too;
+ *     of row_bytes (both or neither NULL) the filled rows are copied too. Where no page is free: the page and -1, and -1 in
+ *     table_out, so a step that goes on from that table (or is made again after a call in place) puts the page back there first;
  *   positions, slots [T]: token i of sequence b at position past + i in slot page * page_size + row; -1 without a page. Tokens of
  *     no sequence: 0 and -1;
  *   with parents [T] (NULL: none; node i of a sequence hangs below node parents[its row] < i, or is a root: anything else) the new

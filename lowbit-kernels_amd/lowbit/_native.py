@@ -838,7 +838,8 @@ class NativeExt:
                                  tokens past a sequence's first 1024 have masks of zeros. Else None
           copies [B, 2]          the page that a sequence's partly filled last page was copied from and to, as it would be
                                  written and another sequence reads it; -1 where there is none. With caches ((k, v) [layers,
-                                 pages, hkv, page_size, D]) its rows are copied in every layer
+                                 pages, hkv, page_size, D]) its rows are copied in every layer. Where no page was free, (page, -1):
+                                 the row has -1 for it too, so a step that goes on from this table puts copies[b, 0] back first
           missing [1]            pages that were wanted and not there"""
         if not page_table.is_cuda or page_table.dim() != 2 or new.dim() != 1:
             raise RuntimeError("page_table [R, width] and new [B] must be CUDA tensors")

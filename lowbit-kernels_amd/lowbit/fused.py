@@ -346,16 +346,19 @@ class FusedQwen2:
         page_table[b] (int32 [B, width], completed in place). Follows the greedy picks down each tree for at most `longest` nodes
         and keeps their keys. Returns accepted (int64 [B, longest]: the confirmed tokens after node 0 and the next one, the
         node 0 to come; -1 behind), counts (int32 [B]: how many) and lens (int32 [B]: the keys kept, the next step's past).
-        What plan_paged could not place for want of pages is told by the last item, missing (int32 [1])."""
+        What plan_paged could not place for want of pages is told by the last item, missing (int32 [1]); the pages of the keys
+        that a sequence has stay in its row of page_table all the same."""
         ext = ops.ext()
         pages, page_size = caches[0].shape[1], caches[0].shape[3]
         step = ext.plan_paged(page_table, past, new, tokens.shape[0], pages, page_size, parents=parents,
-                              words=max(1, -(-max_new // 64)), caches=caches, out=page_table)
+                              words=max(1, -(-max_new // 64)), caches=caches)
         logits = self.forward_paged(tokens, step.positions, step.slots, step.page_table, step.q_starts, step.kv_lens, caches,
                                     max_new, max_keys, masks=step.masks)
         picks = logits.argmax(-1)
         _, counts, accepted, lens = ext.accept_drafts(tokens, picks, parents, step.q_starts, step.kv_lens, step.page_table,
                                                       caches, longest)
+        # (not planned in place: the row of a last page that could not be copied has -1 for it, where the page itself has to stay)
+        torch.where(step.page_table >= 0, step.page_table, page_table, out=page_table)
         return accepted, counts, lens, step.missing
 
     @torch.inference_mode()
