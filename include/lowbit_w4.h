@@ -396,7 +396,8 @@ int lowbit_plan_paged(const int32_t* page_table, int64_t R, int64_t width, const
 /* What the model's own picks (int64 [T]: its choice after each token) confirm of drafted tokens (int64 [T]; parents as above, NULL:
  * chains): sequence b's node 0, then again and again the first child whose token is the pick after the node before, at most
  * `longest` <= 1024 in all: path [B][longest] (-1 behind), counts [B], accepted [B][longest] the picks after the path's nodes
- * (the confirmed tokens, then one more; -1 behind), lens [B] = kv_lens - new + count. A sequence without new tokens has count 0.
+ * (the confirmed tokens, then one more; -1 behind), lens [B] = kv_lens - new + count. A sequence without new tokens has count 0. A
+ * node whose token is negative is not confirmed, node 0 (count 0 then) as any other: that of one without a slot in the cache, say.
  * With k_cache and v_cache (as above) the rows of the path's nodes are moved to the places right behind the sequence's earlier
  * keys, in every layer, so that its first lens[b] keys are those of the confirmed text; sequences' new tokens must lie in pages of
  * their own. Nodes past a sequence's first 1024 are not confirmed. Outputs overlap no inputs. One launch. */

@@ -548,11 +548,12 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
       pick = picks[lane];
       parent = parents ? parents[lane] : lane - 1;
     }
-    int count = 0, cur = 0;
+    int count = 0, cur = readlane64(token, 0) < 0 ? tree : 0;  // (tokens below 0: drafts that cannot be confirmed)
     while (count < a.longest && cur < tree) {
       if (lane == 0) s_path[count] = cur;
       ++count;
       const int64_t want = cur < 64 ? readlane64(pick, cur) : picks[cur];
+      if (want < 0) break;
       const uint64_t hit = __ballot(lane > cur && lane < tree && parent == cur && token == want);
       int next = hit ? __builtin_ctzll(hit) : tree;
       if (!hit && (parents || cur >= 63)) {

@@ -882,13 +882,15 @@ class NativeExt:
             caches[1].data_ptr() if caches else None, layers, hkv, row_bytes, opt(ws), nbytes, stream))
         return PagedStep(out, q_starts, kv_lens, positions, slots, masks, copies.view(batch, 2), missing)
 
-    def accept_drafts(self, tokens, picks, parents, q_starts, kv_lens, page_table, caches, longest):
+    def accept_drafts(self, tokens, picks, parents, q_starts, kv_lens, page_table, caches, longest, slots=None):
         """What the model's own picks (int64 [T], its choice after each token) confirm of drafted tokens (int64 [T]; parents as
         plan_paged takes them, None: chains): from each sequence's node 0, the first child whose token is the pick after the
-        node before, and so on, at most `longest` <= 1024 nodes, of the first 1024 of a sequence. Returns path (int32 [B, longest], -1 behind), counts (int32
-        [B]), accepted (int64 [B, longest]: the picks after the path's nodes, so the confirmed tokens and one more; -1 behind)
-        and lens (int32 [B]: the keys that the sequence keeps, kv_lens - new + counts). With caches ((k, v) [layers, pages,
-        hkv, page_size, D]; None: left to the caller) the confirmed nodes' rows are moved together behind the earlier keys."""
+        node before, and so on, at most `longest` <= 1024 nodes, of the first 1024 of a sequence. Returns path (int32 [B,
+        longest], -1 behind), counts (int32 [B]), accepted (int64 [B, longest]: the picks after the path's nodes, so the
+        confirmed tokens and one more; -1 behind) and lens (int32 [B]: the keys that the sequence keeps, kv_lens - new +
+        counts). With caches ((k, v) [layers, pages, hkv, page_size, D]; None: left to the caller) the confirmed nodes' rows
+        are moved together behind the earlier keys. slots (int64 [T], plan_paged's): a node without one (negative), whose keys
+        are nowhere, is not confirmed, nor is one with a negative token; if that is node 0, the count is 0."""
         if not tokens.is_cuda or tokens.dim() != 1 or page_table.dim() != 2:
             raise RuntimeError("tokens [T] and page_table [B, width] must be CUDA tensors")
         index, device, t, (batch, width) = tokens.get_device(), tokens.device, tokens.shape[0], page_table.shape
@@ -901,6 +903,9 @@ class NativeExt:
         _need_fast(page_table, "page_table", torch.int32, (batch, width), index, device)
         layers, hkv, row_bytes = self._check_layers(caches, None, None, index)
         pages, page_size = (caches[0].shape[-4], caches[0].shape[-2]) if caches is not None else (1, 16)
+        if slots is not None:
+            _need_fast(slots, "slots", torch.int64, (t,), index, device)
+            tokens = tokens.masked_fill(slots < 0, -1)
         longest = int(longest)
         if not 1 <= longest <= 1024:
             raise RuntimeError(f"longest must be 1..1024, got {longest}")

@@ -345,9 +345,10 @@ class FusedQwen2:
         below the node parents[t] (int32 [T]) of its sequence. The sequence's past[b] keys (int32 [B]) lie in the pages
         page_table[b] (int32 [B, width], completed in place). Follows the greedy picks down each tree for at most `longest` nodes
         and keeps their keys. Returns accepted (int64 [B, longest]: the confirmed tokens after node 0 and the next one, the
-        node 0 to come; -1 behind), counts (int32 [B]: how many) and lens (int32 [B]: the keys kept, the next step's past).
-        What plan_paged could not place for want of pages is told by the last item, missing (int32 [1]); the pages of the keys
-        that a sequence has stay in its row of page_table all the same."""
+        node 0 to come; -1 behind), counts (int32 [B]: how many) and lens (int32 [B]: the keys kept, the next step's past). The
+        last item, missing (int32 [1]), says how many pages were wanted and not free. Nodes without a page are not confirmed:
+        a sequence of none has count 0 and its past as lens. What it had, in its row of page_table too, is as before, so that
+        it takes the same node 0 into a step that has pages for it."""
         ext = ops.ext()
         pages, page_size = caches[0].shape[1], caches[0].shape[3]
         step = ext.plan_paged(page_table, past, new, tokens.shape[0], pages, page_size, parents=parents,
@@ -356,7 +357,7 @@ class FusedQwen2:
                                     max_new, max_keys, masks=step.masks)
         picks = logits.argmax(-1)
         _, counts, accepted, lens = ext.accept_drafts(tokens, picks, parents, step.q_starts, step.kv_lens, step.page_table,
-                                                      caches, longest)
+                                                      caches, longest, slots=step.slots)
         # (not planned in place: the row of a last page that could not be copied has -1 for it, where the page itself has to stay)
         torch.where(step.page_table >= 0, step.page_table, page_table, out=page_table)
         return accepted, counts, lens, step.missing

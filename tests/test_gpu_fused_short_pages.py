@@ -77,3 +77,34 @@ def test_a_page_that_cannot_be_copied_stays(cuda):
     accepted, counts, lens, missing = step_of(model, [accepted[0, counts[0] - 1:counts[0]], drafts, empty], table, past, caches)
     assert int(missing) == 0 and int(table[1, 1]) == int(other)
     assert int(counts[1]) == 4 and greedy(model, texts[0], accepted[1, :4])
+
+
+def test_a_step_short_of_pages(cuda):
+    """Three sequences that want six pages of two: the first gets them, the second keeps what fits its last page, the third nothing. When
+    the first has ended, the others go on, and every key is the text's."""
+    model = fused.FusedQwen2(decode.random_model("tiny", seed=12), 128, "int4")
+    texts, caches, table, past = start(model, [14, 15, 17], 5, 6)
+    nodes, longest = 20, 32
+    accepted, counts, lens, missing = step_of(model, [chain(model, t, nodes)[:nodes] for t in texts], table, past, caches, longest)
+    assert int(missing) == 4
+    assert 1 <= int(counts[0]) <= nodes and 1 <= int(counts[1]) <= 2 and int(counts[2]) == 0
+    assert lens.tolist() == [13 + int(counts[0]), 14 + int(counts[1]), 16]
+    assert accepted[2].tolist() == [-1] * longest
+    for turn in range(2):
+        for b in range(3):
+            fresh = accepted[b, :int(counts[b])]
+            if len(fresh):
+                assert greedy(model, texts[b], fresh)
+                texts[b] = torch.cat([texts[b], fresh])
+            assert int(lens[b]) == len(texts[b]) - 1 or (turn and b == 0)
+            if turn and b == 0:
+                continue
+            alone(model, texts[b])
+            for got, plain in zip(keys_of(caches, table, b, int(lens[b])), (model.k_cache, model.v_cache)):
+                assert rel(got, plain[:, :, :int(lens[b])].transpose(1, 2)) < 1e-2
+        if turn:
+            break
+        past = torch.stack([torch.zeros_like(lens[0]), lens[1], lens[2]])
+        trees = [texts[0][:0]] + [chain(model, t, 9)[:9] for t in texts[1:]]
+        accepted, counts, lens, missing = step_of(model, trees, table, past, caches, longest)
+        assert int(missing) == 0 and counts.tolist()[0] == 0 and min(counts.tolist()[1:]) >= 1
