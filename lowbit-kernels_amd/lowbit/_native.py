@@ -840,7 +840,8 @@ class NativeExt:
                                  written and another sequence reads it; -1 where there is none. With caches ((k, v) [layers,
                                  pages, hkv, page_size, D]) its rows are copied in every layer. Where no page was free, (page, -1):
                                  the row has -1 for it too, so a step that goes on from this table puts copies[b, 0] back first
-          missing [1]            pages that were wanted and not there"""
+          missing [1]            pages that were wanted and not there
+        A step may hold no tokens, and no sequences."""
         if not page_table.is_cuda or page_table.dim() != 2 or new.dim() != 1:
             raise RuntimeError("page_table [R, width] and new [B] must be CUDA tensors")
         index, device, (held, width), batch = page_table.get_device(), page_table.device, page_table.shape, new.shape[0]
@@ -850,6 +851,8 @@ class NativeExt:
         _need_fast(new, "new", torch.int32, (batch,), index, device)
         if rows is not None:
             _need_fast(rows, "rows", torch.int32, (batch,), index, device)
+        elif held != batch:
+            raise RuntimeError(f"without rows the table has a row for every sequence, got {held} of {batch}")
         if parents is not None:
             _need_fast(parents, "parents", torch.int32, (tokens,), index, device)
             if not 1 <= words <= MAX_MASK_WORDS:
@@ -863,6 +866,11 @@ class NativeExt:
             _need_fast(out, "out", torch.int32, (batch, width), index, device)
             if rows is not None and out.data_ptr() == page_table.data_ptr():
                 raise RuntimeError("rows need a table of their own to go to")
+        if batch == 0:                                        # (a step of padded tokens alone)
+            i32, i64 = dict(dtype=torch.int32, device=device), dict(dtype=torch.int64, device=device)
+            return PagedStep(out, torch.zeros(1, **i32), torch.zeros(0, **i32), torch.zeros(tokens, **i64),
+                             torch.full((tokens,), -1, **i64), None if parents is None else torch.zeros((tokens, words), **i64),
+                             torch.zeros((0, 2), **i32), torch.zeros(1, **i32))
         # one allocation, whose parts cost less than tensors of their own
         whole = torch.empty(tokens * (2 + (words if parents is not None else 0)) + 2 * batch + 1, dtype=torch.int64, device=device)
         if parents is not None:
@@ -890,7 +898,7 @@ class NativeExt:
         confirmed tokens and one more; -1 behind) and lens (int32 [B]: the keys that the sequence keeps, kv_lens - new +
         counts). With caches ((k, v) [layers, pages, hkv, page_size, D]; None: left to the caller) the confirmed nodes' rows
         are moved together behind the earlier keys. slots (int64 [T], plan_paged's): a node without one (negative), whose keys
-        are nowhere, is not confirmed, nor is one with a negative token; if that is node 0, the count is 0."""
+        are nowhere, is not confirmed, nor is one with a negative token; if that is node 0, the count is 0. T and B may be 0."""
         if not tokens.is_cuda or tokens.dim() != 1 or page_table.dim() != 2:
             raise RuntimeError("tokens [T] and page_table [B, width] must be CUDA tensors")
         index, device, t, (batch, width) = tokens.get_device(), tokens.device, tokens.shape[0], page_table.shape
@@ -903,12 +911,16 @@ class NativeExt:
         _need_fast(page_table, "page_table", torch.int32, (batch, width), index, device)
         layers, hkv, row_bytes = self._check_layers(caches, None, None, index)
         pages, page_size = (caches[0].shape[-4], caches[0].shape[-2]) if caches is not None else (1, 16)
-        if slots is not None:
-            _need_fast(slots, "slots", torch.int64, (t,), index, device)
-            tokens = tokens.masked_fill(slots < 0, -1)
         longest = int(longest)
         if not 1 <= longest <= 1024:
             raise RuntimeError(f"longest must be 1..1024, got {longest}")
+        if slots is not None:
+            _need_fast(slots, "slots", torch.int64, (t,), index, device)
+        if t == 0 or batch == 0:                              # nothing was drafted: every sequence keeps what it has
+            path = torch.full((batch, longest), -1, dtype=torch.int32, device=device)
+            return path, torch.zeros_like(kv_lens), path.long(), kv_lens.clone()
+        if slots is not None:
+            tokens = tokens.masked_fill(slots < 0, -1)
         ints = torch.empty(batch * (longest + 2), dtype=torch.int32, device=device)
         path, counts, lens = ints.split_with_sizes((batch * longest, batch, batch))
         accepted = torch.empty((batch, longest), dtype=torch.int64, device=device)
