@@ -676,15 +676,15 @@ int lowbit_norm_rope_paged(const void* qkv, int64_t qkv_stride, int dtype, const
   return hip_status(norm_rope_paged_launch(a, static_cast<hipStream_t>(stream)), "norm_rope_paged");
 }
 
-static int check_paged_batch(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t table_width, int64_t page_size,
-                             int64_t max_new, int64_t max_keys) {
+static int check_paged_batch(const char* what, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t table_width,
+                             int64_t page_size, int64_t max_new, int64_t max_keys) {
   // (the launch's workgroups and the keys' numbers stay within 32 bits; each workgroup walks the lengths of all sequences before
   // its own, 64 a step: 64 ms for 65536 of 20 keys, 28 / 4 heads, and with the square of B beyond)
   if (T < 1 || B < 1 || table_width < 1 || T > (1 << 28) / Hq || B > 65536 || B > (1 << 22) / Hkv ||
       table_width > (1 << 30) / page_size)
-    return fail(LOWBIT_ERR_SHAPE, "attention_paged: T, B and the table's width must be positive, T * Hq at most 2^28, B 65536, "
-                "B * Hkv 2^22 and the table's keys 2^30");
-  if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "attention_paged: max_new and max_keys must be positive");
+    return fail(LOWBIT_ERR_SHAPE, "%s: T, B and the table's width must be positive, T * Hq at most 2^28, B 65536, "
+                "B * Hkv 2^22 and the table's keys 2^30", what);
+  if (max_new < 1 || max_keys < 1) return fail(LOWBIT_ERR_SHAPE, "%s: max_new and max_keys must be positive", what);
   return LOWBIT_OK;
 }
 
@@ -706,7 +706,7 @@ static PagedAttentionArgs paged_sizes(int64_t T, int64_t B, int64_t Hq, int64_t 
 size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                                         int64_t page_size, int64_t max_new, int64_t max_keys) {
   if (check_paged("attention_paged", LOWBIT_DTYPE_F16, Hq, Hkv, D, 1, page_size) ||
-      check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
+      check_paged_batch("attention_paged", T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
     return 0;
   return attention_paged_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
 }
@@ -714,7 +714,7 @@ size_t lowbit_attention_paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_
 size_t lowbit_attention_paged_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width,
                                              int64_t page_size, int64_t max_new, int64_t max_keys) {
   if (check_paged("attention_paged_tree", LOWBIT_DTYPE_F16, Hq, Hkv, D, 1, page_size) ||
-      check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
+      check_paged_batch("attention_paged_tree", T, B, Hq, Hkv, table_width, page_size, max_new, max_keys))
     return 0;
   return attention_paged_tree_workspace(paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys));
 }
@@ -725,16 +725,17 @@ static int attend_pages(const void* q, int dtype, const void* k_cache, const voi
                         int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t page_size,
                         int64_t max_new, int64_t max_keys, float scale, const uint64_t* masks, int64_t words, void* workspace,
                         size_t workspace_bytes, void* stream) {
+  const char* what = masks ? "attention_paged_tree" : "attention_paged";
   if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
     return fail(LOWBIT_ERR_ARG, "null pointer argument");
-  if (int rc = check_paged("attention_paged", dtype, Hq, Hkv, D, pages, page_size)) return rc;
-  if (int rc = check_paged_batch(T, B, Hq, Hkv, table_width, page_size, max_new, max_keys)) return rc;
+  if (int rc = check_paged(what, dtype, Hq, Hkv, D, pages, page_size)) return rc;
+  if (int rc = check_paged_batch(what, T, B, Hq, Hkv, table_width, page_size, max_new, max_keys)) return rc;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
-    return fail(LOWBIT_ERR_ALIGN, "attention_paged needs 16-byte aligned q, caches and out");
+    return fail(LOWBIT_ERR_ALIGN, "%s needs 16-byte aligned q, caches and out", what);
   if ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(q_starts) |
        reinterpret_cast<uintptr_t>(kv_lens)) & 3)
-    return fail(LOWBIT_ERR_ALIGN, "attention_paged needs naturally aligned page_table, q_starts and kv_lens");
-  if (workspace && !aligned16(workspace)) return fail(LOWBIT_ERR_ARG, "attention_paged: the workspace must be 16-byte aligned");
+    return fail(LOWBIT_ERR_ALIGN, "%s needs naturally aligned page_table, q_starts and kv_lens", what);
+  if (workspace && !aligned16(workspace)) return fail(LOWBIT_ERR_ARG, "%s: the workspace must be 16-byte aligned", what);
   if (int rc = check_device()) return rc;
   PagedAttentionArgs a = paged_sizes(T, B, Hq, Hkv, D, table_width, page_size, max_new, max_keys);
   a.q = q;
@@ -749,10 +750,10 @@ static int attend_pages(const void* q, int dtype, const void* k_cache, const voi
   a.scale = scale;
   a.ws = workspace;
   a.ws_bytes = workspace ? workspace_bytes : 0;
-  if (!masks) return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), "attention_paged");
+  if (!masks) return hip_status(attention_paged_launch(a, static_cast<hipStream_t>(stream)), what);
   a.masks = masks;
   a.words = (int)words;
-  return hip_status(attention_paged_tree_launch(a, static_cast<hipStream_t>(stream)), "attention_paged_tree");
+  return hip_status(attention_paged_tree_launch(a, static_cast<hipStream_t>(stream)), what);
 }
 
 int lowbit_attention_paged(const void* q, int dtype, const void* k_cache, const void* v_cache, const int32_t* page_table,
