@@ -355,7 +355,8 @@ class FusedQwen2:
                               words=max(1, -(-max_new // 64)), caches=caches)
         logits = self.forward_paged(tokens, step.positions, step.slots, step.page_table, step.q_starts, step.kv_lens, caches,
                                     max_new, max_keys, masks=step.masks)
-        picks = logits.argmax(-1)
+        # (us, 26 rows of 151936 in fp16 14, of 60 16, of 768 46, where torch's argmax takes 37, 37 and 67)
+        picks = ext.token_logprobs(logits, tokens, 1)[3].view(-1)
         _, counts, accepted, lens = ext.accept_drafts(tokens, picks, parents, step.q_starts, step.kv_lens, step.page_table,
                                                       caches, longest, slots=step.slots)
         # (not planned in place: the row of a last page that could not be copied has -1 for it, where the page itself has to stay)
