@@ -548,18 +548,19 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a, int shift) {
       pick = picks[lane];
       parent = parents ? parents[lane] : lane - 1;
     }
-    int count = 0, cur = readlane64(token, 0) < 0 ? tree : 0;  // (tokens below 0: drafts that cannot be confirmed)
+    // (a token below 0 cannot be confirmed: no node's child, and nothing if it is node 0's)
+    parent = token < 0 ? -1 : parent;
+    int count = 0, cur = __builtin_amdgcn_readlane((int)(token >> 32), 0) < 0 ? tree : 0;
     while (count < a.longest && cur < tree) {
       if (lane == 0) s_path[count] = cur;
       ++count;
       const int64_t want = cur < 64 ? readlane64(pick, cur) : picks[cur];
-      if (want < 0) break;
       const uint64_t hit = __ballot(lane > cur && lane < tree && parent == cur && token == want);
       int next = hit ? __builtin_ctzll(hit) : tree;
       if (!hit && (parents || cur >= 63)) {
         for (int n0 = max(64, cur + 1); n0 < tree && next == tree; n0 += 64) {
           const int n = n0 + lane;
-          const uint64_t any = __ballot(n < tree && (parents ? parents[n] : n - 1) == cur && tokens[n] == want);
+          const uint64_t any = __ballot(n < tree && want >= 0 && (parents ? parents[n] : n - 1) == cur && tokens[n] == want);
           if (any) next = n0 + __builtin_ctzll(any);
           if (!parents) break;                                // (a chain: the next token or none)
         }
