@@ -99,6 +99,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int G, int se
 // keys far above the mean are cut (us with half a round, one, one and a half and two: 64 decode tokens of 32 / 8 heads on 300 ..
 // 8000 keys 147, 133, 129 and 128; a prompt of 2000 tokens, 28 / 4 heads, 64, 71, 71 and 79; a mixed step 33.8, 34.2, 34.7 and
 // 34.8). s0: the first 64 sequences.
+// Trees look for the least share whose parts fit the rounds that tiles of one part need, up to kEvenSeqs sequences, whose tiles and
+// blocks stay in registers through the search (graph-timed us, so / as above: 28 / 4 heads, trees of 8 .. 16 on 300 .. 8000 keys, 4
+// sequences 27.0 / 28.7, 16 41.0 / 40.5, 32 64.8 / 66.2, 64 151 / 158, 128 281 / 253, 250 511 / 512; 16 / 2 heads, of 16 .. 32 on 1000 ..
+// 30000, 16 94.4 / 94.1, 64 387 / 461; 14 / 2 heads of 64, of 20 .. 60 on 300 .. 8000, 64 92 / 103, 128 206 / 177: ahead where the tiles
+// leave slots free, behind where they nearly fill a round, which then has no parts to even out its long keys with).
 constexpr int kEvenSeqs = 256;
 template <int kRows, int kBlock, bool kTree>
 __device__ __forceinline__ int paged_share(const PagedBatch& b, const PagedPlan& p, const PagedSeq& s0, int lane) {

@@ -669,7 +669,10 @@ hipError_t plan_paged_launch(const PlanArgs& a, hipStream_t st) {
     static_assert(most <= 138 * 1024, "LDS");
     static std::atomic<uint64_t> done{0};
     if ((e = allow_lds_once(done, plan_small_kernel, most))) return e;
-    const bool few = a.B <= 256 && a.T <= 1024 && (int64_t)a.B * a.width <= 2048 && a.pages <= 32768;
+    // a few sequences and tokens are waves that wait for one another at the barriers: 256 threads then (graph-timed us, 256 / 1024: one
+    // sequence of 26 tokens 6.1 / 6.8, 16 of 16 on 2000 keys 7.5 / 8.0, 16 with 256 tokens 7.2 / 7.9; with 1024 tokens 8.7 / 7.9, 32 with
+    // 32 8.7 / 8.5, 48 10.4 / 9.1, 128 beams of 141 pages 23.1 / 13.2)
+    const bool few = a.B <= 16 && a.T <= 256 && (int64_t)a.B * a.width <= 2048 && a.pages <= 32768;
     e = launch(plan_small_kernel, dim3(1), dim3(few ? 256 : kThreads), lds, st, a, std::min(6, log2_of(a.width)), shift, places - 1);
   } else {
     const bool far = a.B > kHashSeqs;                         // the hash in the workspace
