@@ -1095,7 +1095,9 @@ inline PagedLaunch paged_launch(const PagedAttentionArgs& a) {
 // on 300 .. 8000 92 / 50; 14 / 2 heads of 64, 16 of 26 on 300 8.7 / 12.3). One launch, keys not split, where a split and its join (5 to
 // 10 us) cost more than the longest tile's walk is shortened by: 32 rows, whole / split: one tree of 26 on 926 keys, 16 / 2 heads,
 // 16.9 / 13.5, one of 64 on 564 14.3 / 15.9, 4 of 32 on 1000 18.8 / 22.0; 128 rows: 32 of 16 on 500 21.5 / 27.9, 64 of 32 on 1000 54 /
-// 60, 40 of 5 on 2000 51 / 42.
+// 60, 40 of 5 on 2000 51 / 42. Under a bound far above the keys, as a captured step has, calls that go by the keys' own bound to the
+// small tile, or to one launch, may lose that: with 32768 instead of the exact one, a tree of 26 on 926 keys 13.9 -> 15.6, of 64 on 564
+// 14.4 -> 17.4, 16 of 26 on 326, 14 / 2 heads of 64, 8.8 -> 14.3, 16 of 31 .. 63 on 300 .. 8000 the same.
 inline PagedLaunch tree_launch(const PagedAttentionArgs& a) {
   const int64_t G = a.Hq / a.Hkv, seqs = std::min(a.batch.B, a.batch.T), rows = (int64_t)a.batch.T * G;
   auto tiles = [&](int n) { return ((rows + n - 1) / n + seqs) * a.Hkv; };   // at most

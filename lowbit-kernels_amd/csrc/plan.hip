@@ -522,8 +522,9 @@ __global__ __launch_bounds__(256) void plan_copy_kernel(const int* __restrict__ 
 // lanes, a ballot a step), then the workgroup moves the confirmed nodes' rows of its layer, every head of k and v, to the places
 // behind the sequence's keys: one launch, the walk repeated in every layer. Node d of the path comes to lie at place d <= the node's
 // own, so rows are read and written in order of the path, a chunk's all read before one is written.
-// Bound: without moves the chain of round trips (one tree of 26 4.4 us, 64 trees 3.8); with them rows of 256 bytes at places all over
-// the cache: 64 trees, 28 layers, 26 MB read and written, 14.5 us, 1.8 TB/s (several layers a workgroup 16.6).
+// Bound: without moves the chain of round trips (one tree of 26 4.4 us, 64 trees 3.8); with them the chain walk, table, rows, stores,
+// which every workgroup of the one round goes through: 64 trees, 28 layers, 26 MB read and written, 14.6 us, 1.8 TB/s (several layers
+// a workgroup 16.6). Waves wait 63% of their cycles; 2100 of 410000 address translations miss, so scattered rows are not it.
 constexpr int kMostPath = 1024;
 __device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
