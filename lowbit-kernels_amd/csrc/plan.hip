@@ -193,7 +193,9 @@ __device__ __forceinline__ void plan_assign(const PlanArgs& a, const PlanState& 
   if (far) vm_drain();                                        // (the owners, which other waves read behind the barrier)
   lds_barrier();
   // (in the workspace: past the L1, which the atomics above pass by)
-  auto hash_page = [&](int at) { return far ? __hip_atomic_load(s.hash_page + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : s.hash_page[at]; };
+  auto hash_page = [&](int at) {
+    return far ? __hip_atomic_load(s.hash_page + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : s.hash_page[at];
+  };
   auto hash_owner = [&](int at) {
     return far ? __hip_atomic_load(s.hash_owner + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : s.hash_owner[at];
   };
